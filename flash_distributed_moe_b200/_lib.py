@@ -17,6 +17,9 @@ EXPORTED_SYMBOLS = [
     "FlashMoeGetUniqueId", "FlashMoeCreate", "FlashMoeLaunch", "FlashMoeLaunchHost",
     "FlashMoeDestroy", "FlashMoeGetLastStatus", "FlashMoeDebugRead", "FlashMoeTestTaskSystem",
     "FlashMoeTestQueueGemm", "FlashMoeTestStall", "FlashMoeErrorString", "FlashMoeLaunchNoAlloc",
+    "FlashMoeFfnWorkspaceBytes", "FlashMoeFfnForward", "FlashMoeFfnBackward", "FlashMoeMx4ScaleBytes",
+    "FlashMoeMx4Quantize", "FlashMoeMx4Dequantize", "FlashMoeMx4Matmul", "FlashMoeMx4FfnWorkspaceBytes",
+    "FlashMoeMx4FfnForward", "FlashMoeDenseStatus", "FlashMoeTestFfnStall",
 ]
 
 
@@ -24,6 +27,11 @@ class FlashMoeConfig(C.Structure):
     _fields_ = [("hiddenSize", C.c_int32), ("expertIntermediateSize", C.c_int32),
                 ("expertsNum", C.c_int32), ("topk", C.c_int32), ("dtype", C.c_int32),
                 ("reserved", C.c_int32 * 3)]
+
+
+class FlashMoeFfnConfig(C.Structure):
+    _fields_ = [("hiddenSize", C.c_int32), ("intermediateSize", C.c_int32), ("dtype", C.c_int32),
+                ("reserved", C.c_int32 * 5)]
 
 
 _lib = None
@@ -60,6 +68,20 @@ def lib() -> C.CDLL:
                "FlashMoeDestroy", "FlashMoeGetLastStatus", "FlashMoeDebugRead",
                "FlashMoeTestTaskSystem", "FlashMoeTestQueueGemm"):
         getattr(L, fn).restype = C.c_int
+    i64, size, ffn = C.c_int64, C.c_size_t, C.POINTER(FlashMoeFfnConfig)
+    for name, restype, args in (
+            ("FlashMoeFfnWorkspaceBytes", size, [ffn, i64, C.c_int]),
+            ("FlashMoeFfnForward", C.c_int, [ffn] + [vp] * 6 + [size, i64, vp]),
+            ("FlashMoeFfnBackward", C.c_int, [ffn] + [vp] * 9 + [size, i64, vp]),
+            ("FlashMoeMx4ScaleBytes", size, [i64] * 3),
+            ("FlashMoeMx4Quantize", C.c_int, [vp, C.c_int] + [i64] * 5 + [vp] * 3),
+            ("FlashMoeMx4Dequantize", C.c_int, [vp, vp] + [i64] * 3 + [C.c_int, vp, vp]),
+            ("FlashMoeMx4Matmul", C.c_int, [vp] * 5 + [C.c_int] + [i64] * 3 + [C.c_int, vp]),
+            ("FlashMoeMx4FfnWorkspaceBytes", size, [ffn, i64]),
+            ("FlashMoeMx4FfnForward", C.c_int, [ffn] + [vp] * 7 + [size, i64, vp]),
+            ("FlashMoeDenseStatus", C.c_int, [C.POINTER(C.c_uint32), C.c_int]),
+            ("FlashMoeTestFfnStall", C.c_int, [ffn] + [vp] * 5 + [size, i64, vp])):
+        getattr(L, name).argtypes, getattr(L, name).restype = args, restype
     _lib = L
     return L
 

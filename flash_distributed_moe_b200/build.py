@@ -14,8 +14,10 @@ import sys
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 LIB = os.path.join(_HERE, "libflashMoe.so")
-SOURCES = ["moe_kernel.cu", "no_alloc.cu", "launcher.cpp", "bootstrap.cpp"]
-HEADERS = ["moe_types.h", "ptx.cuh", "bootstrap.h", "host_layout.h", "lib.version",
+SOURCES = ["moe_kernel.cu", "no_alloc.cu", "dense_kernels.cu", "mx4_kernels.cu", "launcher.cpp", "dense_ops.cpp",
+           "bootstrap.cpp"]
+HEADERS = ["moe_types.h", "ptx.cuh", "bootstrap.h", "host_layout.h", "lib.version", "dense_types.h",
+           "dense_plan.h", "dense_gemm.cuh", "dense_launch.cuh", "ptx_cluster.cuh",
            os.path.join("..", "..", "include", "iMoeKernelLauncher.h"),
            os.path.join("..", "..", "include", "flashmoe_c.h")]
 

@@ -1,0 +1,597 @@
+// Matrix products of the dense operators on tcgen05, for 16-bit operands (bf16, fp16) and for 4-bit ones with a
+// scale per 32 elements.  Two kernels:
+//
+//   pair_gemm    D[256 x 256] tiles on pairs of CTAs, for results that fill the GPU with such tiles.
+//   stream_gemm  the weights are the M operand (128 rows a tile), up to 128 tokens the N operand, and a cluster of
+//                up to eight CTAs shares the k axis of a tile: for few tokens, where every byte of the weights is
+//                read once and that read has to be spread over all SMs.
+//
+// Both accumulate in fp32 in TMEM over the whole of a CTA's k range; stream_gemm adds the CTAs' partial sums in the
+// order of their ranks, so a call gives the same bits each time.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "dense_types.h"
+#include "ptx_cluster.cuh"
+
+namespace fdmoe {
+namespace dense {
+
+// ------------------------------------------------------------- bounded waits
+// Every wait ends: after `limit_ns` it records what it waited for, raises the CTA's abort flag, and all roles leave.
+struct Waiter {
+  volatile uint32_t* abort_flag;
+  uint32_t* status;
+  uint64_t limit_ns;
+
+  __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint32_t code) const {
+    if (ptx::mbar_try_wait_cluster(bar, parity)) return true;
+    return slow(bar, parity, code);
+  }
+  __device__ __noinline__ bool slow(uint64_t* bar, uint32_t parity, uint32_t code) const {
+    const uint64_t t0 = ptx::globaltimer_ns();
+    for (;;) {
+      for (int i = 0; i < 64; ++i)
+        if (ptx::mbar_try_wait_cluster(bar, parity)) return true;
+      if (*abort_flag) return false;
+      if (ptx::globaltimer_ns() - t0 > limit_ns) {
+        atomicCAS_system(status, 0u, code);
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+  // After an abort: copies and MMAs that were issued before it end within microseconds; the CTA's shared memory and
+  // TMEM are given back two milliseconds later.
+  __device__ __forceinline__ void drain() const {
+    if (!*abort_flag) return;
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+  }
+};
+
+// --------------------------------------------------------------- arithmetic
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
+  uint32_t r;
+  if (bf16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint32_t v, bool bf16, float& lo, float& hi) {
+  if (bf16) {
+    lo = __uint_as_float(v << 16);
+    hi = __uint_as_float(v & 0xFFFF0000u);
+  } else {
+    asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
+        : "=f"(lo), "=f"(hi)
+        : "r"(v));
+  }
+}
+__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
+__device__ __forceinline__ float gate(float g, float u) { return g * sigmoid(g) * u; }
+
+// -------------------------------------------------------------- pair kernel
+// A pair of CTAs (one cluster) works on D[256 x 256] tiles: CTA r holds rows [128 r, 128 r + 128) of A, of D, and
+// half of the rows of B (gated: CTA 0 the gate projection's, CTA 1 the up projection's, so that D holds 128 columns
+// of each), and the even CTA issues MMAs of 256 x 256 x 16 (64 for 4-bit operands) that read both.  Per stage and
+// CTA 32 KB (64 k of 16-bit operands, 256 k of 4-bit ones) serve 512 cycles of MMA, which is what one CTA's tile of
+// 128 x 256 needs 48 KB for.
+constexpr int kPairThreads = 384;
+constexpr int kStageOperand = 16384;  // 128 rows of 128 bytes
+constexpr int kScaleBlock = 512;      // scales of 128 rows and 128 k
+
+template <bool MX4, int EPI>
+struct PairShape {
+  static constexpr bool kThree = EPI == FDMOE_EPI_GATED || EPI == FDMOE_EPI_GATED_GRAD;
+  static constexpr int kStages = MX4 || kThree ? 5 : 6;
+  static constexpr int kAccs = MX4 ? 1 : 2;  // 256 columns each; 4-bit operands' scales need columns too
+  static constexpr int kScales = MX4 ? 6 * kScaleBlock : 0;  // per stage: A 2 blocks, B 4
+  static constexpr int kStaging = kThree && !MX4 ? 6144 : 4096;  // per epilogue warp
+  static constexpr int kBarriers = 256;
+  static constexpr int kSmem =
+      kStages * (2 * kStageOperand + kScales) + 8 * kStaging + kBarriers + 1024;  // 1024: alignment of the base
+};
+
+struct PairTile {
+  int m, n;
+};
+// Tiles in groups of eight row tiles, so that the tiles in flight share operands in L2.
+__device__ __forceinline__ PairTile pair_tile(int tile, int tiles_m, int tiles_n) {
+  const int per_group = 8 * tiles_n, g = tile / per_group, r = tile - g * per_group;
+  const int rows = min(8, tiles_m - g * 8);
+  return {g * 8 + r % rows, r / rows};
+}
+
+// Writes 32 columns of a row of 16-bit results (16 words) to a 32 x 32 staging tile in the 64-byte swizzle.
+__device__ __forceinline__ void stage_half(uint8_t* buf, int lane, const uint32_t (&w)[16]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+        make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+}
+// The same for fp32, 128-byte swizzle.
+__device__ __forceinline__ void stage_f32(uint8_t* buf, int lane, const float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+}
+
+template <bool MX4, int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    pair_gemm(const __grid_constant__ FdmoePairParams p) {
+  using S = PairShape<MX4, EPI>;
+  constexpr bool kGated = EPI == FDMOE_EPI_GATED || EPI == FDMOE_EPI_GATED_F32;
+  constexpr int kAccCols = 256;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t* stages = smem;
+  uint8_t* scales = stages + S::kStages * 2 * kStageOperand;
+  uint8_t* staging = scales + S::kStages * S::kScales;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + 8 * S::kStaging);
+  uint64_t* empty = full + S::kStages;
+  uint64_t* acc_full = empty + S::kStages;
+  uint64_t* acc_empty = acc_full + S::kAccs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + S::kAccs);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_rank();
+  const Waiter wt{abort_flag, p.status, p.timeout_ns};
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      ptx::mbar_init(full + s, 1);
+      ptx::mbar_init(empty + s, 1);
+    }
+    for (int a = 0; a < S::kAccs; ++a) {
+      ptx::mbar_init(acc_full + a, 1);
+      ptx::mbar_init(acc_empty + a, 16);  // eight epilogue warps of each CTA
+    }
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == 2) {
+    ptx::tmem_alloc_pair(tmem_slot, 512);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  ptx::cluster_sync();  // both CTAs' barriers are set up
+  ptx::tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (warp == 0) {
+    // ---- loads: both CTAs fill their own stages; the bytes are counted on the even CTA's barriers
+    if (lane == 0) {
+      ptx::prefetch_tmap(&p.a);
+      ptx::prefetch_tmap(&p.b);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < tiles; tile += step) {
+        const PairTile t = pair_tile(tile, p.tiles_m, p.tiles_n);
+        const int ax = t.m * 256 + (int)rank * 128;
+        const int bx = kGated ? t.n * 128 + (int)rank * p.up_row : t.n * 256 + (int)rank * 128;
+        for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+          const int s = it % S::kStages;
+          const uint32_t ph = (it / S::kStages) & 1;
+          if (!wt.wait(empty + s, ph ^ 1, FDMOE_DENSE_TIMEOUT_EMPTY)) {
+            ok = false;
+            break;
+          }
+          if (p.stall) continue;
+          if (rank == 0) ptx::mbar_expect_tx(full + s, 2 * (2 * kStageOperand + S::kScales));
+          const uint32_t bar = ptx::map_rank(ptx::smem_u32(full + s), 0);
+          const uint32_t sa = ptx::smem_u32(stages + s * 2 * kStageOperand), sb = sa + kStageOperand;
+          if (MX4) {
+            // 128 bytes of a row are 256 elements
+            ptx::tma_load_2d_pair(sa, &p.a, bar, kb * 128, ax);
+            ptx::tma_load_2d_pair(sb, &p.b, bar, kb * 128, bx);
+            const uint32_t sf = ptx::smem_u32(scales + s * S::kScales);
+            ptx::tma_load_2d_pair(sf, &p.sfa, bar, 0, (t.m * 2 + (int)rank) * p.sf_chunks + kb * 2);
+            // both CTAs need the scales of all 256 rows of B
+            const int b0 = kGated ? t.n : t.n * 2, b1 = kGated ? p.sf_up_block + t.n : t.n * 2 + 1;
+            ptx::tma_load_2d_pair(sf + 2 * kScaleBlock, &p.sfb, bar, 0, b0 * p.sf_chunks + kb * 2);
+            ptx::tma_load_2d_pair(sf + 4 * kScaleBlock, &p.sfb, bar, 0, b1 * p.sf_chunks + kb * 2);
+          } else {
+            if (p.a_mn) {
+              ptx::tma_load_2d_pair(sa, &p.a, bar, ax, kb * 64);
+              ptx::tma_load_2d_pair(sa + 8192, &p.a, bar, ax + 64, kb * 64);
+            } else {
+              ptx::tma_load_2d_pair(sa, &p.a, bar, kb * 64, ax);
+            }
+            if (p.b_mn) {
+              ptx::tma_load_2d_pair(sb, &p.b, bar, bx, kb * 64);
+              ptx::tma_load_2d_pair(sb + 8192, &p.b, bar, bx + 64, kb * 64);
+            } else {
+              ptx::tma_load_2d_pair(sb, &p.b, bar, kb * 64, bx);
+            }
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---- MMAs: one thread of the even CTA
+    if (rank == 0 && lane == 0) {
+      const uint32_t idesc = ptx::make_idesc_f16(256, 256, p.bf16, p.a_mn, p.b_mn);
+      // 16 k further: 32 bytes along a row, or 16 rows of 128 bytes
+      const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
+      const uint32_t a_lead = p.a_mn ? 8192 : 16, b_lead = p.b_mn ? 8192 : 16;
+      uint32_t it = 0, n = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < tiles; tile += step, ++n) {
+        const int acc = n % S::kAccs;
+        const uint32_t aph = (n / S::kAccs) & 1;
+        if (!wt.wait(acc_empty + acc, aph ^ 1, FDMOE_DENSE_TIMEOUT_ACC)) break;
+        ptx::tcgen05_fence_after();
+        const uint32_t d = tmem + acc * kAccCols;
+        for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+          const int s = it % S::kStages;
+          if (!wt.wait(full + s, (it / S::kStages) & 1, FDMOE_DENSE_TIMEOUT_FULL)) {
+            ok = false;
+            break;
+          }
+          ptx::tcgen05_fence_after();
+          const uint32_t sa = ptx::smem_u32(stages + s * 2 * kStageOperand), sb = sa + kStageOperand;
+          if (MX4) {
+            const uint32_t sf = ptx::smem_u32(scales + s * S::kScales);
+            // scales have TMEM columns of their own per stage: A 2 x 4, B 2 x 8 (k block, row block)
+            const uint32_t ta = tmem + kAccCols + s * 24, tb = ta + 8;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              ptx::tmem_copy_scales_pair(ta + c * 4, ptx::smem_desc_scales(sf + c * kScaleBlock));
+              ptx::tmem_copy_scales_pair(tb + c * 8, ptx::smem_desc_scales(sf + (2 + c) * kScaleBlock));
+              ptx::tmem_copy_scales_pair(tb + c * 8 + 4, ptx::smem_desc_scales(sf + (4 + c) * kScaleBlock));
+            }
+            const uint64_t da = ptx::smem_desc_sw128(sa, 16), db = ptx::smem_desc_sw128(sb, 16);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              ptx::umma_mx4_pair(d, da + k * 2, db + k * 2, ptx::make_idesc_mx4(256, 256, (k & 1) * 2),
+                                 ta + (k >> 1) * 4, tb + (k >> 1) * 8, (kb | k) != 0);
+          } else {
+            const uint64_t da = ptx::smem_desc_sw128(sa, a_lead), db = ptx::smem_desc_sw128(sb, b_lead);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              ptx::umma_f16_pair(d, da + k * a_step, db + k * b_step, idesc, (kb | k) != 0);
+          }
+          ptx::umma_commit_pair(empty + s);
+        }
+        if (ok) ptx::umma_commit_pair(acc_full + acc);
+      }
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue: warps w and w + 4 read the same 32 lanes, each half of the columns
+    const int w = warp - 4, quad = warp & 3, half = w >> 2;
+    uint8_t* buf = staging + w * S::kStaging;
+    const uint32_t sbuf = ptx::smem_u32(buf);
+    uint32_t n = 0;
+    for (int tile = first; tile < tiles; tile += step, ++n) {
+      const PairTile t = pair_tile(tile, p.tiles_m, p.tiles_n);
+      const int acc = n % S::kAccs;
+      if (!wt.wait(acc_full + acc, (n / S::kAccs) & 1, FDMOE_DENSE_TIMEOUT_DONE)) break;
+      ptx::tcgen05_fence_after();
+      const uint32_t d = tmem + acc * kAccCols + (uint32_t(quad * 32) << 16);
+      const int row0 = t.m * 256 + (int)rank * 128 + quad * 32;
+      constexpr int kChunks = kGated ? 2 : 4;  // of 32 result columns
+#pragma unroll 1
+      for (int c = 0; c < kChunks; ++c) {
+        const int in = half * kChunks * 32 + c * 32;               // column in the tile
+        const int col = t.n * (kGated ? 128 : 256) + in;           // column of the result
+        uint32_t v[32];
+        ptx::tmem_ld_32x32(d + in, v);
+        if constexpr (kGated) {
+          uint32_t u[32];
+          ptx::tmem_ld_32x32(d + 128 + in, u);
+          ptx::tmem_ld_wait();
+          if constexpr (EPI == FDMOE_EPI_GATED_F32) {
+            float h[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) h[i] = gate(__uint_as_float(v[i]), __uint_as_float(u[i]));
+            if (lane == 0) ptx::bulk_wait_group_read0();
+            __syncwarp();
+            stage_f32(buf, lane, h);
+            ptx::fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0 && row0 < p.rows && col < p.cols) ptx::tma_store_2d(&p.out[0], sbuf, col, row0);
+          } else {
+            uint32_t h[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              h[i] = pack2(gate(__uint_as_float(v[2 * i]), __uint_as_float(u[2 * i])),
+                           gate(__uint_as_float(v[2 * i + 1]), __uint_as_float(u[2 * i + 1])), p.bf16);
+            if (!MX4 && p.save_gu) {
+              // kept for the backward pass, rounded like every other activation
+              if (lane == 0) ptx::bulk_wait_group_read0();
+              __syncwarp();
+              stage_half(buf, lane, h);
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                h[i] = pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), p.bf16);
+              stage_half(buf + 2048, lane, h);
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                h[i] = pack2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]), p.bf16);
+              stage_half(buf + 4096, lane, h);
+              ptx::fence_proxy_async_shared();
+              __syncwarp();
+              if (lane == 0 && row0 < p.rows && col < p.cols) {
+                ptx::tma_store_2d(&p.out[0], sbuf, col, row0);
+                ptx::tma_store_2d(&p.out[1], sbuf + 2048, col, row0);
+                ptx::tma_store_2d(&p.out[2], sbuf + 4096, col, row0);
+              }
+            } else {
+              if (lane == 0) ptx::bulk_wait_group_read1();
+              __syncwarp();
+              stage_half(buf + (c & 1) * 2048, lane, h);
+              ptx::fence_proxy_async_shared();
+              __syncwarp();
+              if (lane == 0 && row0 < p.rows && col < p.cols)
+                ptx::tma_store_2d(&p.out[0], sbuf + (c & 1) * 2048, col, row0);
+            }
+          }
+        } else if constexpr (EPI == FDMOE_EPI_GATED_GRAD) {
+          // g and u of this row's 32 columns; columns come in eights because every row starts on 16 bytes
+          uint4 gw[4], uw[4];
+          const int row = row0 + lane;
+          const uint8_t* g0 = static_cast<const uint8_t*>(p.gu) + ((int64_t)row * 2 * p.cols + col) * 2;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool in_range = row < p.rows && col + 8 * j < p.cols;
+            gw[j] = in_range ? __ldg(reinterpret_cast<const uint4*>(g0) + j) : make_uint4(0, 0, 0, 0);
+            uw[j] = in_range ? __ldg(reinterpret_cast<const uint4*>(g0 + (int64_t)p.cols * 2) + j) : make_uint4(0, 0, 0, 0);
+          }
+          ptx::tmem_ld_wait();
+          uint32_t dg[16], du[16], h[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t gp = reinterpret_cast<const uint32_t*>(gw)[i], up = reinterpret_cast<const uint32_t*>(uw)[i];
+            float g[2], u[2], a[2], b[2], e[2];
+            unpack2(gp, p.bf16, g[0], g[1]);
+            unpack2(up, p.bf16, u[0], u[1]);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const float dh = __uint_as_float(v[2 * i + q]), s = sigmoid(g[q]), silu = g[q] * s;
+              a[q] = dh * u[q] * s * (1.0f + g[q] * (1.0f - s));
+              b[q] = dh * silu;
+              e[q] = silu * u[q];
+            }
+            dg[i] = pack2(a[0], a[1], p.bf16);
+            du[i] = pack2(b[0], b[1], p.bf16);
+            h[i] = pack2(e[0], e[1], p.bf16);
+          }
+          if (lane == 0) ptx::bulk_wait_group_read0();
+          __syncwarp();
+          stage_half(buf, lane, dg);
+          stage_half(buf + 2048, lane, du);
+          stage_half(buf + 4096, lane, h);
+          ptx::fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0 && row0 < p.rows && col < p.cols) {
+            ptx::tma_store_2d(&p.out[0], sbuf, col, row0);
+            ptx::tma_store_2d(&p.out[1], sbuf + 2048, col, row0);
+            ptx::tma_store_2d(&p.out[2], sbuf + 4096, col, row0);
+          }
+        } else if constexpr (EPI == FDMOE_EPI_F32) {
+          ptx::tmem_ld_wait();
+          float f[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+          if (lane == 0) ptx::bulk_wait_group_read0();
+          __syncwarp();
+          stage_f32(buf, lane, f);
+          ptx::fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0 && row0 < p.rows && col < p.cols) ptx::tma_store_2d(&p.out[0], sbuf, col, row0);
+        } else {
+          ptx::tmem_ld_wait();
+          uint32_t h[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) h[i] = pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), p.bf16);
+          if (lane == 0) ptx::bulk_wait_group_read1();
+          __syncwarp();
+          stage_half(buf + (c & 1) * 2048, lane, h);
+          ptx::fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0 && row0 < p.rows && col < p.cols)
+            ptx::tma_store_2d(&p.out[0], sbuf + (c & 1) * 2048, col, row0);
+        }
+        if (lane == 0) ptx::bulk_commit_group();
+      }
+      ptx::tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(acc_empty + acc), 0));
+    }
+    if (lane == 0) ptx::bulk_wait_group0();
+  }
+  __syncwarp();
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  wt.drain();
+  ptx::cluster_sync();  // neither CTA leaves while the other may still read its operands or arrive on its barriers
+  ptx::tcgen05_fence_after();
+  if (warp == 2) ptx::tmem_dealloc_pair(tmem, 512);
+}
+
+// ------------------------------------------------------------ stream kernel
+// One CTA: D[128 weight rows x tile_tokens] (gated: two such accumulators, gate and up) over its part of the k axis.
+// The cluster's partial sums meet in shared memory: CTA r adds those of tokens r, r + split, ... over all CTAs.
+constexpr int kStreamThreads = 192;  // 4 epilogue warps, loads, MMAs
+
+template <bool MX4, int EPI>
+__global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_constant__ FdmoeStreamParams p) {
+  constexpr bool kGated = EPI == FDMOE_EPI_GATED || EPI == FDMOE_EPI_GATED_F32;
+  constexpr int kParts = kGated ? 2 : 1;
+  constexpr int kScales = MX4 ? (kParts + 1) * 2 * kScaleBlock : 0;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
+  const int nt = p.tile_tokens;
+  const uint32_t stage_bytes = kParts * kStageOperand + nt * 128 + kScales;  // a multiple of 1024: nt of 16
+  __shared__ uint64_t full[FDMOE_STREAM_STAGES], empty[FDMOE_STREAM_STAGES], acc_full;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile uint32_t abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x;  // in the cluster (split, 1, 1)
+  const int row0 = blockIdx.y * FDMOE_STREAM_ROWS, tok0 = blockIdx.z * nt;
+  const int kb0 = (int)((int64_t)p.kblocks * rank / p.split), kb1 = (int)((int64_t)p.kblocks * (rank + 1) / p.split);
+  const Waiter wt{&abort_flag, p.status, p.timeout_ns};
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      ptx::mbar_init(full + s, 1);
+      ptx::mbar_init(empty + s, 1);
+    }
+    ptx::mbar_init(&acc_full, 1);
+    abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == 4) {
+    ptx::tmem_alloc(&tmem_slot, p.tmem_cols);
+    ptx::tmem_relinquish();
+  }
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  ptx::tcgen05_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 4) {
+    if (lane == 0) {
+      ptx::grid_launch_dependents();
+      auto load_weights = [&](int s, int kb) {
+        uint64_t* bar = full + s;
+        uint8_t* sa = smem + s * stage_bytes;
+        uint8_t* sf = sa + kParts * kStageOperand + nt * 128;
+        ptx::mbar_expect_tx(bar, stage_bytes);
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) {
+          ptx::tma_load_2d(sa + q * kStageOperand, &p.a, bar, kb * (MX4 ? 128 : 64), row0 + q * p.up_row);
+          if (MX4)
+            ptx::tma_load_2d(sf + q * 2 * kScaleBlock, &p.sfa, bar, 0,
+                             ((int)blockIdx.y + q * p.sf_up_block) * p.sf_chunks + kb * 2);
+        }
+      };
+      // The weights of the first stages may be read while the launch before this one still writes the tokens.
+      int ahead = 0;
+      if (p.early_weights)
+        for (; ahead < p.stages && kb0 + ahead < kb1; ++ahead) load_weights(ahead, kb0 + ahead);
+      ptx::grid_wait_dependency();
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int i = kb - kb0, s = i % p.stages;
+        if (i >= ahead) {
+          if (!wt.wait(empty + s, ((i / p.stages) & 1) ^ 1, FDMOE_DENSE_TIMEOUT_EMPTY)) break;
+          load_weights(s, kb);
+        }
+        uint8_t* sb = smem + s * stage_bytes + kParts * kStageOperand;
+        ptx::tma_load_2d(sb, &p.b, full + s, kb * (MX4 ? 128 : 64), tok0);
+        if (MX4) ptx::tma_load_2d(sb + nt * 128 + kParts * 2 * kScaleBlock, &p.sfb, full + s, 0,
+                                  (tok0 >> 7) * p.sf_chunks + kb * 2);
+      }
+    }
+  } else if (warp == 5) {
+    if (lane == 0) {
+      const uint32_t idesc = ptx::make_idesc_f16(128, nt, p.bf16, false, false);
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int i = kb - kb0, s = i % p.stages;
+        if (!wt.wait(full + s, (i / p.stages) & 1, FDMOE_DENSE_TIMEOUT_FULL)) {
+          ok = false;
+          break;
+        }
+        ptx::tcgen05_fence_after();
+        const uint32_t sa = ptx::smem_u32(smem + s * stage_bytes), sb = sa + kParts * kStageOperand;
+        const uint64_t db = ptx::smem_desc_sw128(sb, 16);
+        if (MX4) {
+          const uint32_t sf = sb + nt * 128;
+          const uint32_t tsf = tmem + kParts * nt + s * (kParts + 1) * 8;  // columns of this stage's scales
+#pragma unroll
+          for (int q = 0; q < 2 * (kParts + 1); ++q)
+            ptx::tmem_copy_scales(tsf + q * 4, ptx::smem_desc_scales(sf + q * kScaleBlock));
+          // tokens of a tile may start inside their block of 128: every 32 of them are one column of scales
+          const uint32_t tsb = tsf + kParts * 8 + ((tok0 & 127) >> 5);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t id = ptx::make_idesc_mx4(128, nt, (k & 1) * 2);
+#pragma unroll
+            for (int q = 0; q < kParts; ++q)
+              ptx::umma_mx4(tmem + q * nt, ptx::smem_desc_sw128(sa + q * kStageOperand, 16) + k * 2, db + k * 2, id,
+                            tsf + q * 8 + (k >> 1) * 4, tsb + (k >> 1) * 4, (i | k) != 0);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int q = 0; q < kParts; ++q)
+              ptx::umma_bf16(tmem + q * nt, ptx::smem_desc_sw128(sa + q * kStageOperand, 16) + k * 2, db + k * 2,
+                             idesc, (i | k) != 0);
+        }
+        ptx::umma_commit(empty + s);
+      }
+      if (ok) ptx::umma_commit(&acc_full);
+    }
+  } else {
+    // ---- partial sums to shared memory, [token][part][row]: all MMAs have read the stages, which make room for them
+    if (wt.wait(&acc_full, 0, FDMOE_DENSE_TIMEOUT_DONE)) {
+      ptx::tcgen05_fence_after();
+      const int count = min(nt, p.tokens - tok0);
+      float* part = reinterpret_cast<float*>(smem);
+      const uint32_t d = tmem + (uint32_t(warp * 32) << 16);
+#pragma unroll
+      for (int q = 0; q < kParts; ++q)
+        for (int c = 0; c < count; c += 16) {
+          uint32_t v[16];
+          ptx::tmem_ld_32x16(d + q * nt + c, v);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (c + i < count) part[((c + i) * kParts + q) * 128 + warp * 32 + lane] = __uint_as_float(v[i]);
+        }
+    }
+  }
+  __syncwarp();
+  ptx::tcgen05_fence_before();
+  ptx::cluster_sync();
+  if (warp < 4 && !abort_flag) {
+    const int row = row0 + warp * 32 + lane;
+    const int count = min(nt, p.tokens - tok0);
+    const uint32_t base = ptx::smem_u32(smem) + (warp * 32 + lane) * 4;
+    for (int t = rank; t < count; t += p.split) {
+      float sum[kParts];
+#pragma unroll
+      for (int q = 0; q < kParts; ++q) {
+        float v[FDMOE_STREAM_SPLIT];
+#pragma unroll
+        for (int r = 0; r < FDMOE_STREAM_SPLIT; ++r)
+          if (r < p.split) v[r] = ptx::ld_cluster_f32(ptx::map_rank(base + (t * kParts + q) * 512, r));
+        sum[q] = v[0];
+#pragma unroll
+        for (int r = 1; r < FDMOE_STREAM_SPLIT; ++r)
+          if (r < p.split) sum[q] += v[r];
+      }
+      float y;
+      if constexpr (kGated)
+        y = gate(sum[0], sum[1]);
+      else
+        y = sum[0];
+      if (row < p.rows) {
+        const int64_t at = (int64_t)(tok0 + t) * p.ld + row;
+        if constexpr (EPI == FDMOE_EPI_F32 || EPI == FDMOE_EPI_GATED_F32)
+          static_cast<float*>(p.out)[at] = y;
+        else
+          static_cast<uint16_t*>(p.out)[at] = static_cast<uint16_t>(pack2(y, 0.0f, p.bf16));
+      }
+    }
+  }
+  wt.drain();
+  ptx::cluster_sync();  // a CTA's partial sums stay until every other has read them
+  ptx::tcgen05_fence_after();
+  if (warp == 4) ptx::tmem_dealloc(tmem, p.tmem_cols);
+}
+
+}  // namespace dense
+}  // namespace fdmoe

@@ -1,0 +1,479 @@
+// Host side of the dense operators: argument checks, TMA descriptors, workspaces and launches of the gated
+// feed-forward block (forward, backward) and of the 4-bit microscaled products.  Every call only enqueues work on the
+// caller's stream, keeps nothing between calls and takes all scratch from the caller, so calls on different streams
+// may overlap and every call can be captured into a CUDA graph.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdio.h>
+#include <stdlib.h>
+#include <string.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "../../include/flashmoe_c.h"
+#include "dense_plan.h"
+#include "dense_types.h"
+#include "host_layout.h"
+
+#undef MOE_ERROR_LOG
+#define MOE_ERROR_LOG(...)                                   \
+  do {                                                       \
+    fprintf(stderr, "[MOE ERROR: %s:%d] ", __FILE__, __LINE__); \
+    fprintf(stderr, __VA_ARGS__);                            \
+    fprintf(stderr, "\n");                                   \
+  } while (0)
+
+#define DENSE_CHECK(expr)                                                                              \
+  do {                                                                                                 \
+    const cudaError_t _e = static_cast<cudaError_t>(expr);                                             \
+    if (_e != cudaSuccess) {                                                                           \
+      fprintf(stderr, "[MOE CUDA ERROR: %s:%d] %s\n", __FILE__, __LINE__, cudaGetErrorString(_e));     \
+      return (int)_e;                                                                                  \
+    }                                                                                                  \
+  } while (0)
+
+namespace {
+
+using fdmoe::EncodeTiledFn;
+
+enum { kBf16 = 0, kF32 = 1, kF16 = 2 };  // FlashMoeConfig's numbering, and fp16
+
+// One word of mapped host memory: the first device-side error of any dense call in this process.
+struct Shared {
+  std::mutex mutex;
+  uint32_t* status = nullptr;
+  EncodeTiledFn encode = nullptr;
+  int sms[64] = {0};
+} g_shared;
+
+struct Call {
+  uint32_t* status;
+  EncodeTiledFn encode;
+  int sms;
+  uint64_t timeout_ns;
+  cudaStream_t stream;
+};
+
+int BeginCall(Call* c, void* stream) {
+  int dev = 0;
+  DENSE_CHECK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
+  // a thread that has made no CUDA call yet (autograd's) has no context, which the descriptors need
+  DENSE_CHECK(cudaSetDevice(dev));
+  std::lock_guard<std::mutex> lock(g_shared.mutex);
+  if (!g_shared.status) {
+    // the first call of the process may be inside a stream capture, which this allocation is no part of
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    DENSE_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    void* p = nullptr;
+    const cudaError_t e = cudaHostAlloc(&p, 64, cudaHostAllocMapped | cudaHostAllocPortable);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    DENSE_CHECK(e);
+    memset(p, 0, 64);
+    g_shared.status = static_cast<uint32_t*>(p);
+  }
+  if (!g_shared.encode) g_shared.encode = fdmoe::GetEncodeTiled();
+  if (!g_shared.encode) {
+    MOE_ERROR_LOG("cuTensorMapEncodeTiled is not available from this driver");
+    return (int)cudaErrorUnknown;
+  }
+  if (!g_shared.sms[dev])
+    DENSE_CHECK(cudaDeviceGetAttribute(&g_shared.sms[dev], cudaDevAttrMultiProcessorCount, dev));
+  const uint32_t seen = *static_cast<volatile uint32_t*>(g_shared.status);
+  if (seen) {
+    MOE_ERROR_LOG("refused after device-side error %u; see FlashMoeDenseStatus", seen);
+    return (int)cudaErrorUnknown;
+  }
+  c->status = g_shared.status;
+  c->encode = g_shared.encode;
+  c->sms = g_shared.sms[dev];
+  const char* env = getenv("FLASHMOE_TIMEOUT_MS");
+  c->timeout_ns = (uint64_t)std::max(1, env && *env ? atoi(env) : 2000) * 1000000ull;
+  c->stream = static_cast<cudaStream_t>(stream);
+  return 0;
+}
+
+// Row-major matrix [rows, cols] of `size`-byte elements, rows `stride` bytes apart.
+int MakeMap(const Call& c, FdmoeTensorMap* out, const void* base, int size, int64_t rows, int64_t cols, int64_t stride,
+            int box_cols, int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType type = size == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : size == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  const int span = box_cols * size;  // bytes of a row in shared memory
+  const CUtensorMapSwizzle swizzle = span == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : span == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                  : CU_TENSOR_MAP_SWIZZLE_NONE;
+  const CUresult r = c.encode(reinterpret_cast<CUtensorMap*>(out), type, 2, const_cast<void*>(base), dims, strides, box,
+                              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    MOE_ERROR_LOG("cuTensorMapEncodeTiled failed with %d (rows %lld cols %lld)", (int)r, (long long)rows, (long long)cols);
+    return (int)cudaErrorInvalidValue;
+  }
+  return 0;
+}
+
+#define DENSE_TRY(expr)          \
+  do {                           \
+    const int _r = (expr);       \
+    if (_r != 0) return _r;      \
+  } while (0)
+
+bool Aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// ------------------------------------------------------ products of 16-bit operands
+struct Operand {
+  const void* base;
+  int64_t rows, cols;  // as stored
+  bool mn;             // rows run along M (N): stored [k, m] instead of [m, k]
+};
+
+int OperandMap(const Call& c, FdmoeTensorMap* out, const Operand& o, int box_rows) {
+  return MakeMap(c, out, o.base, 2, o.rows, o.cols, o.cols * 2, 64, o.mn ? 64 : box_rows);
+}
+
+void PairShape(FdmoePairParams& p, const Call& c, int64_t rows, int64_t cols, int64_t k, int tile_cols, int stage_k) {
+  p.status = c.status;
+  p.timeout_ns = c.timeout_ns;
+  p.rows = (int32_t)rows;
+  p.cols = (int32_t)cols;
+  p.tiles_m = (int32_t)((rows + FDMOE_PAIR_TILE - 1) / FDMOE_PAIR_TILE);
+  p.tiles_n = (int32_t)((cols + tile_cols - 1) / tile_cols);
+  p.kblocks = (int32_t)((k + stage_k - 1) / stage_k);
+}
+
+// out[rows, cols] = A B^T, both given as stored.
+int PairProduct(const Call& c, const Operand& a, const Operand& b, void* out, bool bf16) {
+  FdmoePairParams p;
+  memset(&p, 0, sizeof(p));
+  const int64_t rows = a.mn ? a.cols : a.rows, cols = b.mn ? b.cols : b.rows, k = a.mn ? a.rows : a.cols;
+  PairShape(p, c, rows, cols, k, FDMOE_PAIR_TILE, 64);
+  DENSE_TRY(OperandMap(c, &p.a, a, 128));
+  DENSE_TRY(OperandMap(c, &p.b, b, 128));
+  DENSE_TRY(MakeMap(c, &p.out[0], out, 2, rows, cols, cols * 2, 32, 32));
+  p.a_mn = a.mn;
+  p.b_mn = b.mn;
+  p.bf16 = bf16;
+  return fdmoe_pair_launch(&p, FDMOE_EPI_HALF, 0, c.sms, c.stream);
+}
+
+// out[tokens, rows] = x w^T (gated: silu(x w[:rows]^T) * (x w[rows:]^T)) for few tokens.
+int StreamProduct(const Call& c, const void* x, const void* w, void* out, int64_t tokens, int64_t rows, int64_t k,
+                  bool gated, bool bf16, bool dependent) {
+  FdmoeStreamParams p;
+  memset(&p, 0, sizeof(p));
+  const int kblocks = (int)((k + 63) / 64);
+  const fdmoe::StreamPlan s = fdmoe::MakeStreamPlan((int)rows, (int)tokens, kblocks, gated, false, c.sms);
+  DENSE_TRY(MakeMap(c, &p.a, w, 2, gated ? 2 * rows : rows, k, k * 2, 64, 128));
+  DENSE_TRY(MakeMap(c, &p.b, x, 2, tokens, k, k * 2, 64, s.tile_tokens));
+  p.out = out;
+  p.status = c.status;
+  p.timeout_ns = c.timeout_ns;
+  p.ld = rows;
+  p.rows = (int32_t)rows;
+  p.tokens = (int32_t)tokens;
+  p.tile_tokens = s.tile_tokens;
+  p.split = s.split;
+  p.kblocks = kblocks;
+  p.stages = s.stages;
+  p.up_row = (int32_t)rows;
+  p.bf16 = bf16;
+  p.tmem_cols = s.tmem_cols;
+  p.early_weights = dependent;
+  return fdmoe_stream_launch(&p, gated ? FDMOE_EPI_GATED : FDMOE_EPI_HALF, 0, s.smem, dependent, c.stream);
+}
+
+// h[T, I] = silu(g) * u with [g, u] = x w13^T; also g and u to gu [T, 2I] where that is given.
+int GatedProduct(const Call& c, const void* x, const void* w13, void* h, void* gu, int64_t T, int64_t H, int64_t I,
+                 bool bf16, bool stall) {
+  FdmoePairParams p;
+  memset(&p, 0, sizeof(p));
+  PairShape(p, c, T, I, H, 128, 64);
+  DENSE_TRY(MakeMap(c, &p.a, x, 2, T, H, H * 2, 64, 128));
+  DENSE_TRY(MakeMap(c, &p.b, w13, 2, 2 * I, H, H * 2, 64, 128));
+  DENSE_TRY(MakeMap(c, &p.out[0], h, 2, T, I, I * 2, 32, 32));
+  if (gu) {
+    // two matrices side by side: what a tile has beyond column I of the gate projection is not stored
+    DENSE_TRY(MakeMap(c, &p.out[1], gu, 2, T, I, I * 4, 32, 32));
+    DENSE_TRY(MakeMap(c, &p.out[2], static_cast<uint8_t*>(gu) + I * 2, 2, T, I, I * 4, 32, 32));
+  }
+  p.up_row = (int32_t)I;
+  p.bf16 = bf16;
+  p.save_gu = gu != nullptr;
+  p.stall = stall;
+  return fdmoe_pair_launch(&p, FDMOE_EPI_GATED, 0, c.sms, c.stream);
+}
+
+// From dy: dgu [T, 2I] and h [T, I].
+int GatedGradient(const Call& c, const void* dy, const void* w2, const void* gu, void* dgu, void* h, int64_t T, int64_t H,
+                  int64_t I, bool bf16) {
+  FdmoePairParams p;
+  memset(&p, 0, sizeof(p));
+  PairShape(p, c, T, I, H, FDMOE_PAIR_TILE, 64);
+  DENSE_TRY(MakeMap(c, &p.a, dy, 2, T, H, H * 2, 64, 128));
+  DENSE_TRY(MakeMap(c, &p.b, w2, 2, H, I, I * 2, 64, 64));
+  DENSE_TRY(MakeMap(c, &p.out[0], dgu, 2, T, I, I * 4, 32, 32));
+  DENSE_TRY(MakeMap(c, &p.out[1], static_cast<uint8_t*>(dgu) + I * 2, 2, T, I, I * 4, 32, 32));
+  DENSE_TRY(MakeMap(c, &p.out[2], h, 2, T, I, I * 2, 32, 32));
+  p.gu = gu;
+  p.b_mn = 1;
+  p.bf16 = bf16;
+  return fdmoe_pair_launch(&p, FDMOE_EPI_GATED_GRAD, 0, c.sms, c.stream);
+}
+
+// ------------------------------------------------------ products of 4-bit operands
+struct Mx4 {
+  const void *values, *scales;
+  int64_t rows;   // of one matrix
+  int64_t batch;  // matrices one after another
+};
+
+int Mx4Maps(const Call& c, FdmoeTensorMap* values, FdmoeTensorMap* scales, const Mx4& m, int64_t k, int box_rows) {
+  const int64_t chunks = fdmoe::ScaleChunks(k), blocks = m.batch * ((m.rows + 127) / 128);
+  if (blocks * chunks > INT32_MAX) return (int)cudaErrorInvalidValue;  // a coordinate has 32 bits
+  DENSE_TRY(MakeMap(c, values, m.values, 1, m.batch * m.rows, k / 2, k / 2, 128, box_rows));
+  return MakeMap(c, scales, m.scales, 4, blocks * chunks, 128, 512, 128, 2);
+}
+
+int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, int64_t k, bool gated, bool dependent,
+               bool early_weights) {
+  const int64_t tokens = a.rows, rows = b.rows;
+  const int kblocks = (int)((k + FDMOE_MX4_STAGE_K - 1) / FDMOE_MX4_STAGE_K);
+  const int chunks = (int)fdmoe::ScaleChunks(k), up_block = (int)((rows + 127) / 128);
+  const int epi = gated ? (dtype == kF32 ? FDMOE_EPI_GATED_F32 : FDMOE_EPI_GATED)
+                        : (dtype == kF32 ? FDMOE_EPI_F32 : FDMOE_EPI_HALF);
+  if (fdmoe::UseStream((int)std::min<int64_t>(tokens, 1 << 30)) || (dtype == kF32 ? rows % 4 : rows % 8) != 0) {
+    FdmoeStreamParams p;
+    memset(&p, 0, sizeof(p));
+    const fdmoe::StreamPlan s = fdmoe::MakeStreamPlan((int)rows, (int)tokens, kblocks, gated, true, c.sms);
+    DENSE_TRY(Mx4Maps(c, &p.a, &p.sfa, b, k, 128));
+    DENSE_TRY(Mx4Maps(c, &p.b, &p.sfb, a, k, s.tile_tokens));
+    p.out = out;
+    p.status = c.status;
+    p.timeout_ns = c.timeout_ns;
+    p.ld = rows;
+    p.rows = (int32_t)rows;
+    p.tokens = (int32_t)tokens;
+    p.tile_tokens = s.tile_tokens;
+    p.split = s.split;
+    p.kblocks = kblocks;
+    p.stages = s.stages;
+    p.up_row = (int32_t)rows;
+    p.sf_chunks = chunks;
+    p.sf_up_block = up_block;
+    p.bf16 = dtype == kBf16;
+    p.tmem_cols = s.tmem_cols;
+    p.early_weights = early_weights;
+    return fdmoe_stream_launch(&p, epi, 1, s.smem, dependent, c.stream);
+  }
+  FdmoePairParams p;
+  memset(&p, 0, sizeof(p));
+  PairShape(p, c, tokens, rows, k, gated ? 128 : FDMOE_PAIR_TILE, FDMOE_MX4_STAGE_K);
+  DENSE_TRY(Mx4Maps(c, &p.a, &p.sfa, a, k, 128));
+  DENSE_TRY(Mx4Maps(c, &p.b, &p.sfb, b, k, 128));
+  const int size = dtype == kF32 ? 4 : 2;
+  DENSE_TRY(MakeMap(c, &p.out[0], out, size, tokens, rows, rows * size, 32, 32));
+  p.up_row = (int32_t)rows;
+  p.sf_chunks = chunks;
+  p.sf_up_block = up_block;
+  p.bf16 = dtype == kBf16;
+  return fdmoe_pair_launch(&p, epi, 1, c.sms, c.stream);
+}
+
+// ------------------------------------------------------------------- checks
+constexpr int64_t kMaxDim = 1 << 20;      // of a layer: hidden, intermediate, columns
+constexpr int64_t kMaxTokens = 1 << 30;
+
+int CheckFfn(const FlashMoeFfnConfig* cfg, int64_t tokens) {
+  if (!cfg) return (int)cudaErrorInvalidValue;
+  const int64_t H = cfg->hiddenSize, I = cfg->intermediateSize;
+  if (H <= 0 || I <= 0 || H % 8 || I % 8 || H > kMaxDim || I > kMaxDim || (cfg->dtype != kBf16 && cfg->dtype != kF16)) {
+    MOE_ERROR_LOG("unsupported block hidden=%lld intermediate=%lld dtype=%d (sizes multiples of 8; bf16 or fp16)",
+                  (long long)H, (long long)I, cfg->dtype);
+    return (int)cudaErrorInvalidValue;
+  }
+  if (tokens < 0 || tokens > kMaxTokens) return (int)cudaErrorInvalidValue;
+  return 0;
+}
+
+int CheckMx4(int64_t batch, int64_t rows, int64_t cols) {
+  if (batch < 0 || batch > 65535 || rows < 0 || rows > kMaxTokens || cols <= 0 || cols % FDMOE_MX4_BLOCK || cols > kMaxDim ||
+      batch * rows > kMaxTokens) {
+    MOE_ERROR_LOG("unsupported matrix batch=%lld rows=%lld cols=%lld (columns: a multiple of 32)", (long long)batch,
+                  (long long)rows, (long long)cols);
+    return (int)cudaErrorInvalidValue;
+  }
+  return 0;
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------- C exports
+extern "C" int FlashMoeDenseStatus(uint32_t* code, int reset) {
+  std::lock_guard<std::mutex> lock(g_shared.mutex);
+  volatile uint32_t* s = g_shared.status;
+  if (code) *code = s ? *s : 0;
+  if (reset && s) *s = 0;
+  return 0;
+}
+
+extern "C" size_t FlashMoeFfnWorkspaceBytes(const FlashMoeFfnConfig* cfg, int64_t tokensNum, int backward) {
+  if (CheckFfn(cfg, tokensNum) != 0) return 0;
+  const size_t h = fdmoe::AlignBytes((size_t)tokensNum * cfg->intermediateSize * 2);
+  return backward ? h + fdmoe::AlignBytes((size_t)tokensNum * cfg->intermediateSize * 4) : h;
+}
+
+static int FfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y, void* gateUp,
+                      void* workspace, size_t workspaceBytes, int64_t T, void* stream, bool stall) {
+  DENSE_TRY(CheckFfn(cfg, T));
+  if (T == 0) return 0;
+  if (!x || !w13 || !w2 || !y || !workspace || !Aligned(x) || !Aligned(w13) || !Aligned(w2) || !Aligned(y) ||
+      !Aligned(gateUp) || !Aligned(workspace) || workspaceBytes < FlashMoeFfnWorkspaceBytes(cfg, T, 0))
+    return (int)cudaErrorInvalidValue;
+  Call c;
+  DENSE_TRY(BeginCall(&c, stream));
+  const int64_t H = cfg->hiddenSize, I = cfg->intermediateSize;
+  const bool bf16 = cfg->dtype == kBf16;
+  if (!gateUp && !stall && fdmoe::UseStream((int)T)) {
+    DENSE_TRY(StreamProduct(c, x, w13, workspace, T, I, H, true, bf16, false));
+    return StreamProduct(c, workspace, w2, y, T, H, I, false, bf16, true);
+  }
+  DENSE_TRY(GatedProduct(c, x, w13, workspace, gateUp, T, H, I, bf16, stall));
+  if (stall) return 0;
+  return PairProduct(c, {workspace, T, I, false}, {w2, H, I, false}, y, bf16);
+}
+
+extern "C" int FlashMoeFfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y,
+                                  void* gateUp, void* workspace, size_t workspaceBytes, int64_t tokensNum, void* stream) {
+  return FfnForward(cfg, x, w13, w2, y, gateUp, workspace, workspaceBytes, tokensNum, stream, false);
+}
+
+extern "C" int FlashMoeTestFfnStall(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y,
+                                    void* workspace, size_t workspaceBytes, int64_t tokensNum, void* stream) {
+  return FfnForward(cfg, x, w13, w2, y, nullptr, workspace, workspaceBytes, tokensNum, stream, true);
+}
+
+extern "C" int FlashMoeFfnBackward(const FlashMoeFfnConfig* cfg, const void* dy, const void* x, const void* w13,
+                                   const void* w2, const void* gateUp, void* dx, void* dw13, void* dw2, void* workspace,
+                                   size_t workspaceBytes, int64_t T, void* stream) {
+  DENSE_TRY(CheckFfn(cfg, T));
+  const int64_t H = cfg->hiddenSize, I = cfg->intermediateSize;
+  if (!Aligned(dx) || !Aligned(dw13) || !Aligned(dw2)) return (int)cudaErrorInvalidValue;
+  if (T == 0) {
+    if (dw13) DENSE_CHECK(cudaMemsetAsync(dw13, 0, (size_t)(2 * I * H) * 2, static_cast<cudaStream_t>(stream)));
+    if (dw2) DENSE_CHECK(cudaMemsetAsync(dw2, 0, (size_t)(I * H) * 2, static_cast<cudaStream_t>(stream)));
+    return 0;
+  }
+  if (!dy || !x || !w13 || !w2 || !gateUp || !workspace || !Aligned(dy) || !Aligned(x) || !Aligned(w13) || !Aligned(w2) ||
+      !Aligned(gateUp) || !Aligned(workspace) || workspaceBytes < FlashMoeFfnWorkspaceBytes(cfg, T, 1))
+    return (int)cudaErrorInvalidValue;
+  if (!dx && !dw13 && !dw2) return 0;
+  Call c;
+  DENSE_TRY(BeginCall(&c, stream));
+  const bool bf16 = cfg->dtype == kBf16;
+  void* h = workspace;
+  void* dgu = static_cast<uint8_t*>(workspace) + fdmoe::AlignBytes((size_t)T * I * 2);
+  DENSE_TRY(GatedGradient(c, dy, w2, gateUp, dgu, h, T, H, I, bf16));
+  if (dx) DENSE_TRY(PairProduct(c, {dgu, T, 2 * I, false}, {w13, 2 * I, H, true}, dx, bf16));
+  if (dw13) DENSE_TRY(PairProduct(c, {dgu, T, 2 * I, true}, {x, T, H, true}, dw13, bf16));
+  if (dw2) DENSE_TRY(PairProduct(c, {dy, T, H, true}, {h, T, I, true}, dw2, bf16));
+  return 0;
+}
+
+extern "C" size_t FlashMoeMx4ScaleBytes(int64_t batch, int64_t rows, int64_t cols) {
+  if (CheckMx4(batch, rows, cols) != 0) return 0;
+  return fdmoe::ScaleBytes(batch, rows, cols);
+}
+
+extern "C" int FlashMoeMx4Quantize(const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols,
+                                   int64_t batchStride, int64_t rowStride, void* values, void* scales, void* stream) {
+  DENSE_TRY(CheckMx4(batch, rows, cols));
+  if (dtype != kBf16 && dtype != kF32 && dtype != kF16) return (int)cudaErrorInvalidValue;
+  if (batch == 0 || rows == 0) return 0;
+  const int64_t per16 = dtype == kF32 ? 4 : 8;
+  if (!x || !values || !scales || !Aligned(x) || !Aligned(values) || !Aligned(scales) || batchStride < 0 || rowStride < 0 ||
+      batchStride % per16 || rowStride % per16)
+    return (int)cudaErrorInvalidValue;
+  return fdmoe_mx4_quantize(x, dtype, batch, rows, cols, batchStride, rowStride, values, scales, stream);
+}
+
+extern "C" int FlashMoeMx4Dequantize(const void* values, const void* scales, int64_t batch, int64_t rows, int64_t cols,
+                                     int dtype, void* out, void* stream) {
+  DENSE_TRY(CheckMx4(batch, rows, cols));
+  if (dtype != kBf16 && dtype != kF32 && dtype != kF16) return (int)cudaErrorInvalidValue;
+  if (batch == 0 || rows == 0) return 0;
+  if (!values || !scales || !out || !Aligned(values) || !Aligned(scales) || !Aligned(out)) return (int)cudaErrorInvalidValue;
+  return fdmoe_mx4_dequantize(values, scales, batch, rows, cols, dtype, out, stream);
+}
+
+extern "C" int FlashMoeMx4Matmul(const void* aValues, const void* aScales, const void* bValues, const void* bScales,
+                                 void* out, int dtype, int64_t m, int64_t n, int64_t k, int gated, void* stream) {
+  DENSE_TRY(CheckMx4(1, m, k));
+  DENSE_TRY(CheckMx4(gated ? 2 : 1, n, k));
+  if (dtype != kBf16 && dtype != kF32 && dtype != kF16) return (int)cudaErrorInvalidValue;
+  if (m == 0 || n == 0) return 0;
+  if (!aValues || !aScales || !bValues || !bScales || !out || !Aligned(aValues) || !Aligned(aScales) || !Aligned(bValues) ||
+      !Aligned(bScales) || !Aligned(out))
+    return (int)cudaErrorInvalidValue;
+  Call c;
+  DENSE_TRY(BeginCall(&c, stream));
+  return Mx4Product(c, {aValues, aScales, m, 1}, {bValues, bScales, n, gated ? 2 : 1}, out, dtype, k, gated != 0, false,
+                    false);
+}
+
+// Workspace of the block on 4-bit weights: 4-bit tokens, activations, 4-bit activations.
+namespace {
+struct Mx4FfnLayout {
+  size_t xv, xs, h, hv, hs, total;
+};
+Mx4FfnLayout MakeMx4FfnLayout(int64_t T, int64_t H, int64_t I) {
+  Mx4FfnLayout l;
+  size_t at = 0;
+  l.xv = at;
+  at += fdmoe::AlignBytes((size_t)T * H / 2);
+  l.xs = at;
+  at += fdmoe::AlignBytes(fdmoe::ScaleBytes(1, T, H));
+  l.h = at;
+  at += fdmoe::AlignBytes((size_t)T * I * 2);
+  l.hv = at;
+  at += fdmoe::AlignBytes((size_t)T * I / 2);
+  l.hs = at;
+  at += fdmoe::AlignBytes(fdmoe::ScaleBytes(1, T, I));
+  l.total = at;
+  return l;
+}
+}  // namespace
+
+extern "C" size_t FlashMoeMx4FfnWorkspaceBytes(const FlashMoeFfnConfig* cfg, int64_t tokensNum) {
+  if (CheckFfn(cfg, tokensNum) != 0 || cfg->hiddenSize % FDMOE_MX4_BLOCK || cfg->intermediateSize % FDMOE_MX4_BLOCK) return 0;
+  return MakeMx4FfnLayout(tokensNum, cfg->hiddenSize, cfg->intermediateSize).total;
+}
+
+extern "C" int FlashMoeMx4FfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w13Values,
+                                     const void* w13Scales, const void* w2Values, const void* w2Scales, void* y,
+                                     void* workspace, size_t workspaceBytes, int64_t T, void* stream) {
+  DENSE_TRY(CheckFfn(cfg, T));
+  const int64_t H = cfg->hiddenSize, I = cfg->intermediateSize;
+  DENSE_TRY(CheckMx4(1, T, H));
+  DENSE_TRY(CheckMx4(2, I, H));
+  DENSE_TRY(CheckMx4(1, H, I));
+  if (T == 0) return 0;
+  if (!x || !w13Values || !w13Scales || !w2Values || !w2Scales || !y || !workspace || !Aligned(x) || !Aligned(w13Values) ||
+      !Aligned(w13Scales) || !Aligned(w2Values) || !Aligned(w2Scales) || !Aligned(y) || !Aligned(workspace) ||
+      workspaceBytes < FlashMoeMx4FfnWorkspaceBytes(cfg, T))
+    return (int)cudaErrorInvalidValue;
+  Call c;
+  DENSE_TRY(BeginCall(&c, stream));
+  const Mx4FfnLayout l = MakeMx4FfnLayout(T, H, I);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  DENSE_TRY(fdmoe_mx4_quantize(x, cfg->dtype, 1, T, H, 0, H, ws + l.xv, ws + l.xs, stream));
+  DENSE_TRY(Mx4Product(c, {ws + l.xv, ws + l.xs, T, 1}, {w13Values, w13Scales, I, 2}, ws + l.h, cfg->dtype, H, true, false,
+                       false));
+  DENSE_TRY(fdmoe_mx4_quantize(ws + l.h, cfg->dtype, 1, T, I, 0, I, ws + l.hv, ws + l.hs, stream));
+  return Mx4Product(c, {ws + l.hv, ws + l.hs, T, 1}, {w2Values, w2Scales, H, 1}, y, cfg->dtype, I, false, false, false);
+}

@@ -1,0 +1,92 @@
+// Plain structs shared by the host side (dense_ops.cpp) and the device side (dense_kernels.cu, mx4_kernels.cu) of the
+// dense gated feed-forward block and of the 4-bit microscaled products.
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+#include "moe_types.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+enum {
+  FDMOE_PAIR_TILE = 256,      // rows and columns of a tile of the pair kernel
+  FDMOE_STREAM_ROWS = 128,    // weight rows of a tile of the streaming kernel
+  FDMOE_STREAM_TOKENS = 128,  // most tokens of a tile of the streaming kernel
+  FDMOE_STREAM_SPLIT = 8,     // most CTAs that share the k axis of a tile of the streaming kernel
+  FDMOE_STREAM_STAGES = 12,   // most shared-memory stages of the streaming kernel
+  FDMOE_MX4_BLOCK = 32,       // elements that share a scale
+  FDMOE_MX4_STAGE_K = 256,    // elements of k per stage: 128 bytes of 4-bit values
+};
+
+// What the epilogue makes of a tile.
+enum {
+  FDMOE_EPI_HALF = 0,        // rounded to bf16 or fp16
+  FDMOE_EPI_F32 = 1,         // as it is
+  FDMOE_EPI_GATED = 2,       // silu(gate) * up, rounded to bf16 or fp16
+  FDMOE_EPI_GATED_F32 = 3,   // silu(gate) * up
+  FDMOE_EPI_GATED_GRAD = 4,  // gradients of gate and up, and silu(gate) * up
+};
+
+// Status codes of the dense kernels (first error wins).
+enum {
+  FDMOE_DENSE_TIMEOUT_EMPTY = 21,  // a stage was not freed
+  FDMOE_DENSE_TIMEOUT_FULL = 22,   // a stage was not filled
+  FDMOE_DENSE_TIMEOUT_ACC = 23,    // an accumulator was not freed
+  FDMOE_DENSE_TIMEOUT_DONE = 24,   // an accumulator was not completed
+};
+
+typedef struct {
+  FdmoeTensorMap a, b;        // operands; `a` gives the rows of the result, `b` its columns
+  FdmoeTensorMap sfa, sfb;    // their scales (4-bit operands)
+  FdmoeTensorMap out[3];      // results: the tile | h, gate, up | d gate, d up, h
+  const void* gu;             // gate and up projections [rows, 2 * cols] (FDMOE_EPI_GATED_GRAD)
+  uint32_t* status;
+  uint64_t timeout_ns;
+  int32_t rows, cols;         // of the result
+  int32_t tiles_m, tiles_n;
+  int32_t kblocks;
+  int32_t a_mn, b_mn;         // operand stored with its rows along M (N) instead of along K
+  int32_t up_row;             // row of `b` at which the up projection starts (gated)
+  int32_t sf_chunks;          // 512-byte blocks of scales per 128 rows
+  int32_t sf_up_block;        // block of 128 rows at which the up projection's scales start
+  int32_t bf16;               // 16-bit operands and results are bf16, otherwise fp16
+  int32_t save_gu;            // gated: also write the gate and up projections
+  int32_t stall;              // test hook: nothing is loaded, every wait runs out
+  int32_t reserved;
+} FdmoePairParams;
+
+typedef struct {
+  FdmoeTensorMap a, b;        // weights (rows of the tile) and tokens (columns of the tile)
+  FdmoeTensorMap sfa, sfb;
+  void* out;                  // [tokens, rows], row stride `ld` elements
+  uint32_t* status;
+  uint64_t timeout_ns;
+  int64_t ld;
+  int32_t rows, tokens;
+  int32_t tile_tokens;        // 16..128, a multiple of 16
+  int32_t split;              // CTAs per tile along k: the cluster
+  int32_t kblocks;
+  int32_t stages;
+  int32_t up_row;
+  int32_t sf_chunks;
+  int32_t sf_up_block;
+  int32_t bf16;
+  int32_t tmem_cols;
+  int32_t early_weights;      // the launch before this one does not write the weights: load them before it has ended
+} FdmoeStreamParams;
+
+// Launchers; return a cudaError_t.  `mx4` selects 4-bit operands.
+int fdmoe_pair_launch(const FdmoePairParams* p, int epi, int mx4, int sms, void* stream);
+// `dependent`: may start before the launch before it has ended (it waits for that by itself).
+int fdmoe_stream_launch(const FdmoeStreamParams* p, int epi, int mx4, int smem, int dependent, void* stream);
+
+int fdmoe_mx4_quantize(const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols, int64_t batch_stride,
+                       int64_t row_stride, void* values, void* scales, void* stream);
+int fdmoe_mx4_dequantize(const void* values, const void* scales, int64_t batch, int64_t rows, int64_t cols, int dtype,
+                         void* out, void* stream);
+
+#ifdef __cplusplus
+}
+#endif

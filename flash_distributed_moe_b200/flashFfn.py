@@ -1,0 +1,150 @@
+"""The gated feed-forward block (SwiGLU) of a dense layer or of a shared expert, with its gradient.
+
+    y = gated_ffn(x, w13, w2)       # (silu(x w13[:I]^T) * (x w13[I:]^T)) w2^T
+
+`w13` and `w2` are laid out as one expert of the mixture-of-experts layer: [2I, H] with the gate projection's rows
+first, and [H, I].  bf16 or fp16, or, without gradients, 4-bit weights (`quantize_ffn_weights`).
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Tuple, Union
+
+import torch
+
+from . import _lib
+from .flashMoeLauncher import _stream_ptr
+from .flashMx4 import Mx4Tensor, mx4_quantize
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 2}
+Weight = Union[torch.Tensor, Mx4Tensor]
+
+
+def _config(hidden: int, inter: int, dtype: torch.dtype):
+    return C.byref(_lib.FlashMoeFfnConfig(hidden, inter, _DTYPES[dtype], (C.c_int32 * 5)()))
+
+
+def _check(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} tensor is undefined")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if t.dtype not in _DTYPES:
+        raise RuntimeError(f"{name} must be bfloat16 or float16")
+    if t.dtype != like.dtype or t.device != like.device:
+        raise RuntimeError(f"{name} must have the dtype and device of x")
+
+
+def _check_weights(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> None:
+    _check(w13, "w13", x)
+    _check(w2, "w2", x)
+    for t, name in ((w13, "w13"), (w2, "w2")):
+        if not t.is_contiguous() or t.data_ptr() % 16:
+            raise RuntimeError(f"{name} must be contiguous and start on 16 bytes")
+    if w2.dim() != 2 or tuple(w13.shape) != (2 * w2.shape[1], w2.shape[0]) or x.shape[-1] != w2.shape[0]:
+        raise RuntimeError("x, w13 and w2 must be [..., hidden], [2*inter, hidden] and [hidden, inter]")
+    if w2.shape[0] % 8 or w2.shape[1] % 8 or w2.numel() == 0:
+        raise RuntimeError("hidden and inter must be multiples of 8")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[..., n] as contiguous rows on 16 bytes; a copy only where the tensor is neither."""
+    t = t.reshape(-1, t.shape[-1]).contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _forward(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, save: bool):
+    (hidden, inter), tokens, lib = w2.shape, x.shape[0], _lib.lib()
+    y = torch.empty_like(x)
+    gate_up = torch.empty((tokens, 2 * inter), dtype=x.dtype, device=x.device) if save else None
+    with torch.cuda.device(x.device):
+        cfg = _config(hidden, inter, x.dtype)
+        ws = torch.empty(lib.FlashMoeFfnWorkspaceBytes(cfg, tokens, 0), dtype=torch.uint8, device=x.device)
+        _lib.check(lib.FlashMoeFfnForward(cfg, x.data_ptr(), w13.data_ptr(), w2.data_ptr(), y.data_ptr(),
+                                          gate_up.data_ptr() if save else None, ws.data_ptr(), ws.numel(), tokens,
+                                          _stream_ptr()), "FfnForward")
+    return y, gate_up
+
+
+class _GatedFfn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w13, w2):
+        y, gate_up = _forward(x, w13, w2, save=True)
+        ctx.save_for_backward(x, w13, w2, gate_up)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w13, w2, gate_up = ctx.saved_tensors
+        (hidden, inter), tokens, lib = w2.shape, x.shape[0], _lib.lib()
+        dy = _rows(dy)
+        grads = [torch.empty_like(t) if need else None for t, need in zip((x, w13, w2), ctx.needs_input_grad)]
+        with torch.cuda.device(x.device):
+            cfg = _config(hidden, inter, x.dtype)
+            ws = torch.empty(lib.FlashMoeFfnWorkspaceBytes(cfg, tokens, 1), dtype=torch.uint8, device=x.device)
+            _lib.check(lib.FlashMoeFfnBackward(cfg, dy.data_ptr(), x.data_ptr(), w13.data_ptr(), w2.data_ptr(),
+                                               gate_up.data_ptr(), *[None if g is None else g.data_ptr() for g in grads],
+                                               ws.data_ptr(), ws.numel(), tokens, _stream_ptr()), "FfnBackward")
+        return tuple(grads)
+
+
+def gated_ffn(x: torch.Tensor, w13: Weight, w2: Weight) -> torch.Tensor:
+    """x [..., H] -> [..., H].  Asynchronous on the current torch stream of x's device.  Differentiable in x, w13 and w2:
+    the gate and up projections of the tokens are kept for the backward pass, rounded to the dtype.  With Mx4Tensor
+    weights (w13 [2, I, H], w2 [H, I]) x and the activations are quantised to 4 bits too, and there is no gradient.
+
+    A training step may be captured into a CUDA graph.  As with every torch operator, capture it while no eager graph
+    of the same leaves is alive (torch keeps the gradient accumulators of such a graph on its stream, which must not
+    join the capture), or take the gradients with `torch.autograd.grad`."""
+    if not isinstance(x, torch.Tensor):
+        raise RuntimeError("x tensor is undefined")
+    _check(x, "x", x)
+    if x.dim() < 1:
+        raise RuntimeError("x must be [..., hidden]")
+    if isinstance(w13, Mx4Tensor) or isinstance(w2, Mx4Tensor):
+        return _mx4_ffn(x, w13, w2)
+    _check_weights(x, w13, w2)
+    rows = _rows(x)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w13, w2)):
+        y = _GatedFfn.apply(rows, w13, w2)
+    else:
+        y, _ = _forward(rows, w13, w2, save=False)
+    return y.reshape(x.shape)
+
+
+def quantize_ffn_weights(w13: torch.Tensor, w2: torch.Tensor) -> Tuple[Mx4Tensor, Mx4Tensor]:
+    """[2I, H] and [H, I] weights of a block as 4-bit matrices for gated_ffn; H and I multiples of 32."""
+    if w13.dim() != 2 or w2.dim() != 2 or tuple(w13.shape) != (2 * w2.shape[1], w2.shape[0]):
+        raise RuntimeError("w13 and w2 must be [2*inter, hidden] and [hidden, inter]")
+    return mx4_quantize(w13.view(2, w2.shape[1], w2.shape[0])), mx4_quantize(w2)
+
+
+def _mx4_ffn(x: torch.Tensor, w13: Mx4Tensor, w2: Mx4Tensor) -> torch.Tensor:
+    if not isinstance(w13, Mx4Tensor) or not isinstance(w2, Mx4Tensor):
+        raise RuntimeError("w13 and w2 must both be 4-bit weights or neither")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError("gated_ffn has no gradient with 4-bit weights")
+    if w13.device != x.device or w2.device != x.device:
+        raise RuntimeError("x, w13 and w2 must be on the same device")
+    if len(w2.shape) != 2 or tuple(w13.shape) != (2, w2.shape[1], w2.shape[0]) or x.shape[-1] != w2.shape[0]:
+        raise RuntimeError("x, w13 and w2 must be [..., hidden], [2, inter, hidden] and [hidden, inter]")
+    if w2.shape[0] % 32:
+        raise RuntimeError("hidden and inter must be multiples of 32")
+    rows, (hidden, inter), lib = _rows(x.detach()), w2.shape, _lib.lib()
+    y = torch.empty_like(rows)
+    with torch.cuda.device(x.device):
+        cfg = _config(hidden, inter, x.dtype)
+        ws = torch.empty(lib.FlashMoeMx4FfnWorkspaceBytes(cfg, rows.shape[0]), dtype=torch.uint8, device=x.device)
+        _lib.check(lib.FlashMoeMx4FfnForward(cfg, rows.data_ptr(), w13.values.data_ptr(), w13.scales.data_ptr(),
+                                             w2.values.data_ptr(), w2.scales.data_ptr(), y.data_ptr(), ws.data_ptr(),
+                                             ws.numel(), rows.shape[0], _stream_ptr()), "Mx4FfnForward")
+    return y.reshape(x.shape)
+
+
+def dense_status(reset: bool = False) -> int:
+    """Code of the first device-side error of the dense operators in this process, 0 if none.  After one, calls are
+    refused until reset."""
+    code = C.c_uint32(0)
+    _lib.check(_lib.lib().FlashMoeDenseStatus(C.byref(code), int(reset)), "DenseStatus")
+    return int(code.value)

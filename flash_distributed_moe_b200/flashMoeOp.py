@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import torch
 
+from .flashFfn import gated_ffn, quantize_ffn_weights
 from .flashMoeLauncher import MoeKernelLauncher
 
 
@@ -38,3 +39,22 @@ class FlashMoeBlockWrapper(torch.nn.Module):
             return hidden_states
         # larger batches go to the wrapped block (the reference calls a non-existent super().forward here)
         return self.qwen3MoeSparseMoeBlockModule(hidden_states)
+
+
+class FlashFfnBlockWrapper(torch.nn.Module):
+    """The same for a dense block: any module exposing `gate_up_proj.weight` [2I,H] (gate rows first) and
+    `down_proj.weight` [H,I], e.g. the dense layers and shared experts of the same models.  With `fourBit` the
+    weights are quantised once, here, and the forward pass reads them at half a byte per value."""
+
+    def __init__(self, mlpModule: torch.nn.Module, fourBit: bool = False):
+        super().__init__()
+        self.mlpModule = mlpModule
+        self.fourBitWeights = None
+        if fourBit:
+            self.fourBitWeights = quantize_ffn_weights(mlpModule.gate_up_proj.weight.detach(),
+                                                       mlpModule.down_proj.weight.detach())
+
+    def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
+        if self.fourBitWeights is not None:
+            return gated_ffn(hidden_states, *self.fourBitWeights)
+        return gated_ffn(hidden_states, self.mlpModule.gate_up_proj.weight, self.mlpModule.down_proj.weight)

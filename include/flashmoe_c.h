@@ -109,6 +109,73 @@ int FlashMoeLaunchNoAlloc(const void* gateWeights, const void* ffn1ExpertWeights
                           const void* ffn2ExpertWeights, const void* tokens, void* output, int tokensNum,
                           const FlashMoeConfig* config, void* stream);
 
+/* ---------------------------------------------------------------- dense operators
+ * The gated feed-forward block of a dense layer or of a shared expert, its gradient, and 4-bit
+ * microscaled weights for it (the reference has no counterpart; its experts' FFN is
+ * src/hip/kernel/moeKernel.h).  These entries need no handle: every call enqueues its work on `stream`,
+ * takes scratch from the caller and can be captured into a CUDA graph; calls with different workspaces
+ * may overlap.  Matrices are contiguous, row-major, on the current device, and start on 16 bytes.
+ * Results are deterministic: the same call gives the same bits. */
+typedef struct {
+  int32_t hiddenSize;       /* H, a multiple of 8 (4-bit weights: 32) */
+  int32_t intermediateSize; /* I, a multiple of 8 (4-bit weights: 32) */
+  int32_t dtype;            /* 0 bf16, 2 fp16 */
+  int32_t reserved[5];      /* zero */
+} FlashMoeFfnConfig;
+
+/* Bytes of scratch for a forward (backward == 0) or backward call; 0 for an unsupported config. */
+size_t FlashMoeFfnWorkspaceBytes(const FlashMoeFfnConfig* config, int64_t tokensNum, int backward);
+
+/* y[T,H] = (silu(x Wg^T) * (x Wu^T)) W2^T with w13 = [Wg; Wu] [2I,H], w2 [H,I].  `gateUp` [T,2I], if not
+ * NULL, receives x Wg^T and x Wu^T for FlashMoeFfnBackward.  `y` may be `x`.  The projections, the
+ * activation and both products are accumulated in fp32; h = silu(g) * u is rounded to the dtype. */
+int FlashMoeFfnForward(const FlashMoeFfnConfig* config, const void* x, const void* w13, const void* w2,
+                       void* y, void* gateUp, void* workspace, size_t workspaceBytes, int64_t tokensNum,
+                       void* stream);
+
+/* Gradients of x [T,H], w13 [2I,H] and w2 [H,I] from that of y; each of the three may be NULL.  With no
+ * tokens the gradients of the weights are zero. */
+int FlashMoeFfnBackward(const FlashMoeFfnConfig* config, const void* dy, const void* x, const void* w13,
+                        const void* w2, const void* gateUp, void* dx, void* dw13, void* dw2,
+                        void* workspace, size_t workspaceBytes, int64_t tokensNum, void* stream);
+
+/* 4-bit microscaled matrices: E2M1 values, two to a byte (even element low), [batch, rows, cols / 2], and
+ * one E8M0 scale per 32 elements of a row in blocks of 512 bytes for 128 rows and 128 columns (the scale of
+ * row r and column block c is byte (r % 32) * 16 + (r / 32) * 4 + c), an even number of blocks per 128
+ * rows.  cols is a multiple of 32.  FlashMoeMx4ScaleBytes gives the size of the scales, 0 if unsupported. */
+size_t FlashMoeMx4ScaleBytes(int64_t batch, int64_t rows, int64_t cols);
+
+/* x (dtype 0 bf16, 1 fp32, 2 fp16; strides in elements, multiples of 16 bytes) to values and scales: the
+ * scale is 2^(floor(log2(largest magnitude)) - 2), elements are rounded to nearest even and saturate at 6.
+ * A block with a NaN or an infinity stands for NaN. */
+int FlashMoeMx4Quantize(const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols,
+                        int64_t batchStride, int64_t rowStride, void* values, void* scales, void* stream);
+
+/* The values that a 4-bit matrix stands for, contiguous. */
+int FlashMoeMx4Dequantize(const void* values, const void* scales, int64_t batch, int64_t rows, int64_t cols,
+                          int dtype, void* out, void* stream);
+
+/* out[m,n] = a[m,k] b[n,k]^T, accumulated in fp32.  gated != 0: b is a batch of two matrices [2,n,k], gate
+ * and up projection, and out = silu(a b0^T) * (a b1^T).  dtype of out: 0 bf16, 1 fp32, 2 fp16. */
+int FlashMoeMx4Matmul(const void* aValues, const void* aScales, const void* bValues, const void* bScales,
+                      void* out, int dtype, int64_t m, int64_t n, int64_t k, int gated, void* stream);
+
+/* The block with 4-bit weights (w13 as a batch of two [2,I,H], w2 [H,I]): x and h are quantised on the way. */
+size_t FlashMoeMx4FfnWorkspaceBytes(const FlashMoeFfnConfig* config, int64_t tokensNum);
+int FlashMoeMx4FfnForward(const FlashMoeFfnConfig* config, const void* x, const void* w13Values,
+                          const void* w13Scales, const void* w2Values, const void* w2Scales, void* y,
+                          void* workspace, size_t workspaceBytes, int64_t tokensNum, void* stream);
+
+/* First device-side error of the dense operators in this process (0 == none; a bounded wait that ran out,
+ * FLASHMOE_TIMEOUT_MS); does not synchronise.  After one, dense calls are refused with cudaErrorUnknown
+ * until `reset` != 0 clears it. */
+int FlashMoeDenseStatus(uint32_t* code, int reset);
+
+/* Test hook: a forward call whose loads are left out, so that every wait runs out after
+ * FLASHMOE_TIMEOUT_MS.  Nothing faults or hangs. */
+int FlashMoeTestFfnStall(const FlashMoeFfnConfig* config, const void* x, const void* w13, const void* w2,
+                         void* y, void* workspace, size_t workspaceBytes, int64_t tokensNum, void* stream);
+
 const char* FlashMoeErrorString(int code);
 
 #ifdef __cplusplus

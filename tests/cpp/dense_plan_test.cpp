@@ -1,0 +1,52 @@
+// Checks the launch plans of the streaming kernel over the range of sizes: shared memory, TMEM columns, stages and the
+// split of the k axis stay within what the kernel and the hardware allow.
+#include <cstdio>
+#include <cstdlib>
+
+#include "../../flash_distributed_moe_b200/csrc/dense_plan.h"
+
+#define CHECK(cond)                                                                                              \
+  do {                                                                                                           \
+    if (!(cond)) {                                                                                               \
+      std::printf("line %d: %s (rows %d tokens %d kblocks %d gated %d mx4 %d)\n", __LINE__, #cond, rows, tokens, \
+                  kb, gated, mx4);                                                                               \
+      return 1;                                                                                                  \
+    }                                                                                                            \
+  } while (0)
+
+int main() {
+  using namespace fdmoe;
+  const int row_list[] = {1, 8, 127, 128, 129, 768, 1544, 4096, 12288, 65536};
+  const int token_list[] = {1, 2, 15, 16, 17, 31, 33, 48, 63, 64, 65, 80, 96, 100, 112, 127, 128, 129, 255, 256, 1531, 8192, 65536};
+  const int kb_list[] = {1, 2, 3, 5, 8, 12, 16, 33, 64, 192, 1000};
+  for (int rows : row_list)
+    for (int tokens : token_list)
+      for (int kb : kb_list)
+        for (int gated = 0; gated < 2; ++gated)
+          for (int mx4 = 0; mx4 < 2; ++mx4)
+            for (int sms : {148, 132, 8}) {
+              const StreamPlan s = MakeStreamPlan(rows, tokens, kb, gated, mx4, sms);
+              const int parts = gated ? 2 : 1;
+              const int stage = parts * 16384 + s.tile_tokens * 128 + (mx4 ? (parts + 1) * 1024 : 0);
+              CHECK(s.tile_tokens % 16 == 0 && s.tile_tokens >= 16 && s.tile_tokens <= FDMOE_STREAM_TOKENS);
+              CHECK((int64_t)s.tile_tokens * s.token_tiles >= tokens && (int64_t)s.tile_tokens * (s.token_tiles - 1) < tokens);
+              // a tile of tokens lies within one block of 128 rows of scales and starts on a column of them
+              if (s.token_tiles > 1) CHECK(s.tile_tokens == 128 || (128 % s.tile_tokens == 0 && s.tile_tokens % 32 == 0));
+              CHECK(s.row_tiles * FDMOE_STREAM_ROWS >= rows && s.row_tiles <= 65535);
+              CHECK(s.split >= 1 && s.split <= FDMOE_STREAM_SPLIT && s.split <= kb);
+              CHECK(s.stages >= 1 && s.stages <= FDMOE_STREAM_STAGES);
+              CHECK(s.stages * stage + kStreamSlack <= s.smem);
+              CHECK((tokens < s.tile_tokens ? tokens : s.tile_tokens) * parts * 512 + kStreamSlack <= s.smem);
+              CHECK(s.smem <= 226 * 1024 && (s.per_sm == 1 || s.smem <= 112 * 1024));
+              const int cols = parts * s.tile_tokens + (mx4 ? s.stages * (parts + 1) * 8 : 0);
+              CHECK(s.tmem_cols >= cols && s.tmem_cols >= 32 && (s.tmem_cols & (s.tmem_cols - 1)) == 0);
+              CHECK(s.tmem_cols * s.per_sm <= 512);
+            }
+  {
+    const int rows = 0, tokens = 0, kb = 0, gated = 0, mx4 = 0;
+    CHECK(ScaleChunks(32) == 2 && ScaleChunks(256) == 2 && ScaleChunks(288) == 4);
+    CHECK(ScaleBytes(1, 1, 32) == 1024 && ScaleBytes(2, 129, 512) == 2 * 2 * 4 * 512 && ScaleBytes(1, 0, 32) == 0);
+  }
+  std::printf("ok\n");
+  return 0;
+}
