@@ -90,6 +90,20 @@ def error_string(code: int) -> str:
     return lib().FlashMoeErrorString(int(code)).decode()
 
 
+def run(device_index: int, name: str, *args) -> None:
+    """Calls entry `name` of the dense operators with `args` and the current torch stream of the device, which is made
+    current for the call if it is not; raises on an error code."""
+    import torch
+    fn = getattr(_lib or lib(), name)
+    if torch._C._cuda_getDevice() == device_index:
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(device_index))
+    else:
+        with torch.cuda.device(device_index):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(device_index))
+    if code != 0:
+        check(code, name)
+
+
 def check(code: int, what: str) -> None:
     """Non-zero return codes become exceptions, as the reference binding does with TORCH_CHECK
     (python/pyMoeLauncherTorch.cpp:14-22)."""

@@ -1,7 +1,7 @@
 // Matrix products of the dense operators on tcgen05, for 16-bit operands (bf16, fp16) and for 4-bit ones with a
 // scale per 32 elements.  Two kernels:
 //
-//   pair_gemm    D[256 x 256] tiles on pairs of CTAs, for results that fill the GPU with such tiles.
+//   pair_gemm    D[256 x 256] or D[256 x 128] tiles on pairs of CTAs.
 //   stream_gemm  the weights are the M operand (128 rows a tile), up to 128 tokens the N operand, and a cluster of
 //                up to eight CTAs shares the k axis of a tile: for few tokens, where every byte of the weights is
 //                read once and that read has to be spread over all SMs.
@@ -74,11 +74,12 @@ __device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f
 __device__ __forceinline__ float gate(float g, float u) { return g * sigmoid(g) * u; }
 
 // -------------------------------------------------------------- pair kernel
-// A pair of CTAs (one cluster) works on D[256 x 256] tiles: CTA r holds rows [128 r, 128 r + 128) of A, of D, and
-// half of the rows of B (gated: CTA 0 the gate projection's, CTA 1 the up projection's, so that D holds 128 columns
-// of each), and the even CTA issues MMAs of 256 x 256 x 16 (64 for 4-bit operands) that read both.  Per stage and
-// CTA 32 KB (64 k of 16-bit operands, 256 k of 4-bit ones) serve 512 cycles of MMA, which is what one CTA's tile of
-// 128 x 256 needs 48 KB for.
+// A pair of CTAs works on D[256 x tile_n] tiles: CTA r holds rows [128 r, 128 r + 128) of A, of D, and half of the
+// rows of B (gated: CTA 0 the gate projection's, CTA 1 the up projection's, so that D holds tile_n / 2 columns of
+// each), and the even CTA issues MMAs of 256 x tile_n x 16 (64 for 4-bit operands) that read both.  With tile_n = 256
+// 32 KB per stage and CTA (64 k of 16-bit operands, 256 k of 4-bit ones) serve 512 cycles of MMA, which is what one
+// CTA's tile of 128 x 256 needs 48 KB for.  Two rules make it fit few tiles (MakePairPlan): tile_n = 128, and a
+// cluster of two or four pairs that share the k axis of a tile and add their partial sums through shared memory.
 constexpr int kPairThreads = 384;
 constexpr int kStageOperand = 16384;  // 128 rows of 128 bytes
 constexpr int kScaleBlock = 512;      // scales of 128 rows and 128 k
@@ -121,8 +122,7 @@ __device__ __forceinline__ void stage_f32(uint8_t* buf, int lane, const float (&
 }
 
 template <bool MX4, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-    pair_gemm(const __grid_constant__ FdmoePairParams p) {
+__global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_constant__ FdmoePairParams p) {
   using S = PairShape<MX4, EPI>;
   constexpr bool kGated = EPI == FDMOE_EPI_GATED || EPI == FDMOE_EPI_GATED_F32;
   constexpr int kAccCols = 256;
@@ -139,7 +139,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = ptx::cluster_rank();
+  // A cluster is `split` pairs, which share the k axis of a tile.
+  const uint32_t cta = ptx::cluster_rank(), rank = cta & 1, leader = cta & ~1u, part = cta >> 1;
+  const int split = p.split;
+  const int kb0 = p.kblocks * (int)part / split, kb1 = p.kblocks * ((int)part + 1) / split;
+  const int half_n = p.tile_n >> 1;  // rows of B per CTA; gated: columns of each projection
   const Waiter wt{abort_flag, p.status, p.timeout_ns};
 
   if (threadIdx.x == 0) {
@@ -163,9 +167,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   ptx::cluster_sync();  // both CTAs' barriers are set up
   ptx::tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
+  ptx::grid_wait_dependency();  // nothing of global memory is touched before this
+  ptx::grid_launch_dependents();
 
   const int tiles = p.tiles_m * p.tiles_n;
-  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const int first = blockIdx.x / (2 * split), step = gridDim.x / (2 * split);
 
   if (warp == 0) {
     // ---- loads: both CTAs fill their own stages; the bytes are counted on the even CTA's barriers
@@ -177,8 +183,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       for (int tile = first; ok && tile < tiles; tile += step) {
         const PairTile t = pair_tile(tile, p.tiles_m, p.tiles_n);
         const int ax = t.m * 256 + (int)rank * 128;
-        const int bx = kGated ? t.n * 128 + (int)rank * p.up_row : t.n * 256 + (int)rank * 128;
-        for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+        const int bx = kGated ? t.n * half_n + (int)rank * p.up_row : t.n * p.tile_n + (int)rank * half_n;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % S::kStages;
           const uint32_t ph = (it / S::kStages) & 1;
           if (!wt.wait(empty + s, ph ^ 1, FDMOE_DENSE_TIMEOUT_EMPTY)) {
@@ -186,8 +192,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             break;
           }
           if (p.stall) continue;
-          if (rank == 0) ptx::mbar_expect_tx(full + s, 2 * (2 * kStageOperand + S::kScales));
-          const uint32_t bar = ptx::map_rank(ptx::smem_u32(full + s), 0);
+          if (rank == 0) ptx::mbar_expect_tx(full + s, 2 * (kStageOperand + half_n * 128 + S::kScales));
+          const uint32_t bar = ptx::map_rank(ptx::smem_u32(full + s), leader);
           const uint32_t sa = ptx::smem_u32(stages + s * 2 * kStageOperand), sb = sa + kStageOperand;
           if (MX4) {
             // 128 bytes of a row are 256 elements
@@ -208,7 +214,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
             if (p.b_mn) {
               ptx::tma_load_2d_pair(sb, &p.b, bar, bx, kb * 64);
-              ptx::tma_load_2d_pair(sb + 8192, &p.b, bar, bx + 64, kb * 64);
+              if (half_n > 64) ptx::tma_load_2d_pair(sb + 8192, &p.b, bar, bx + 64, kb * 64);
             } else {
               ptx::tma_load_2d_pair(sb, &p.b, bar, kb * 64, bx);
             }
@@ -219,7 +225,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   } else if (warp == 1) {
     // ---- MMAs: one thread of the even CTA
     if (rank == 0 && lane == 0) {
-      const uint32_t idesc = ptx::make_idesc_f16(256, 256, p.bf16, p.a_mn, p.b_mn);
+      const uint32_t idesc = ptx::make_idesc_f16(256, p.tile_n, p.bf16, p.a_mn, p.b_mn);
       // 16 k further: 32 bytes along a row, or 16 rows of 128 bytes
       const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
       const uint32_t a_lead = p.a_mn ? 8192 : 16, b_lead = p.b_mn ? 8192 : 16;
@@ -231,7 +237,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         if (!wt.wait(acc_empty + acc, aph ^ 1, FDMOE_DENSE_TIMEOUT_ACC)) break;
         ptx::tcgen05_fence_after();
         const uint32_t d = tmem + acc * kAccCols;
-        for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % S::kStages;
           if (!wt.wait(full + s, (it / S::kStages) & 1, FDMOE_DENSE_TIMEOUT_FULL)) {
             ok = false;
@@ -253,41 +259,78 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               ptx::umma_mx4_pair(d, da + k * 2, db + k * 2, ptx::make_idesc_mx4(256, 256, (k & 1) * 2),
-                                 ta + (k >> 1) * 4, tb + (k >> 1) * 8, (kb | k) != 0);
+                                 ta + (k >> 1) * 4, tb + (k >> 1) * 8, kb != kb0 || k != 0);
           } else {
             const uint64_t da = ptx::smem_desc_sw128(sa, a_lead), db = ptx::smem_desc_sw128(sb, b_lead);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              ptx::umma_f16_pair(d, da + k * a_step, db + k * b_step, idesc, (kb | k) != 0);
+              ptx::umma_f16_pair(d, da + k * a_step, db + k * b_step, idesc, kb != kb0 || k != 0);
           }
-          ptx::umma_commit_pair(empty + s);
+          ptx::umma_commit_pair(empty + s, leader);
         }
-        if (ok) ptx::umma_commit_pair(acc_full + acc);
+        if (ok) ptx::umma_commit_pair(acc_full + acc, leader);
       }
     }
   } else if (warp >= 4) {
-    // ---- epilogue: warps w and w + 4 read the same 32 lanes, each half of the columns
+    // ---- epilogue: warps w and w + 4 read the same 32 lanes and take turns with the columns, 32 at a time
     const int w = warp - 4, quad = warp & 3, half = w >> 2;
     uint8_t* buf = staging + w * S::kStaging;
     const uint32_t sbuf = ptx::smem_u32(buf);
+    const int tile_cols = kGated ? half_n : p.tile_n, chunks = tile_cols >> 5;
     uint32_t n = 0;
     for (int tile = first; tile < tiles; tile += step, ++n) {
       const PairTile t = pair_tile(tile, p.tiles_m, p.tiles_n);
       const int acc = n % S::kAccs;
-      if (!wt.wait(acc_full + acc, (n / S::kAccs) & 1, FDMOE_DENSE_TIMEOUT_DONE)) break;
+      const bool done = wt.wait(acc_full + acc, (n / S::kAccs) & 1, FDMOE_DENSE_TIMEOUT_DONE);
       ptx::tcgen05_fence_after();
       const uint32_t d = tmem + acc * kAccCols + (uint32_t(quad * 32) << 16);
       const int row0 = t.m * 256 + (int)rank * 128 + quad * 32;
-      constexpr int kChunks = kGated ? 2 : 4;  // of 32 result columns
+      if (split > 1) {
+        // the cluster's only tile: the partial sums go where the stages were, [column / 4][row][4]
+        if (done)
+          for (int c = half; c < p.tile_n >> 5; c += 2) {
+            uint32_t v[32];
+            ptx::tmem_ld_32x32(d + c * 32, v);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<uint4*>(stages + ((c * 8 + j) * 128 + quad * 32 + lane) * 16) =
+                  make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          }
+        ptx::cluster_sync();
+      }
+      if (!done) break;
+      // 32 columns of the tile from the accumulator, or from all pairs' partial sums in the order of their ranks
+      auto load = [&](int column, uint32_t (&v)[32]) {
+        if (split == 1) {
+          ptx::tmem_ld_32x32(d + column, v);
+          return;
+        }
+        const uint32_t at = ptx::smem_u32(stages) + ((column >> 2) * 128 + quad * 32 + lane) * 16;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0;
+        for (int r = 0; r < split; ++r) {
+          const uint32_t from = ptx::map_rank(at, 2 * r + rank);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 f = ptx::ld_cluster_f32x4(from + j * 2048);
+            v[4 * j] = __float_as_uint(__uint_as_float(v[4 * j]) + f.x);
+            v[4 * j + 1] = __float_as_uint(__uint_as_float(v[4 * j + 1]) + f.y);
+            v[4 * j + 2] = __float_as_uint(__uint_as_float(v[4 * j + 2]) + f.z);
+            v[4 * j + 3] = __float_as_uint(__uint_as_float(v[4 * j + 3]) + f.w);
+          }
+        }
+      };
+      int used = 0;  // staging buffers written
 #pragma unroll 1
-      for (int c = 0; c < kChunks; ++c) {
-        const int in = half * kChunks * 32 + c * 32;               // column in the tile
-        const int col = t.n * (kGated ? 128 : 256) + in;           // column of the result
+      for (int c = half * split + (int)part; c < chunks; c += 2 * split, ++used) {
+        const int in = c * 32;                        // column in the tile
+        const int col = t.n * tile_cols + in;         // column of the result
         uint32_t v[32];
-        ptx::tmem_ld_32x32(d + in, v);
+        load(in, v);
         if constexpr (kGated) {
           uint32_t u[32];
-          ptx::tmem_ld_32x32(d + 128 + in, u);
+          load(half_n + in, u);
           ptx::tmem_ld_wait();
           if constexpr (EPI == FDMOE_EPI_GATED_F32) {
             float h[32];
@@ -328,11 +371,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             } else {
               if (lane == 0) ptx::bulk_wait_group_read1();
               __syncwarp();
-              stage_half(buf + (c & 1) * 2048, lane, h);
+              stage_half(buf + (used & 1) * 2048, lane, h);
               ptx::fence_proxy_async_shared();
               __syncwarp();
               if (lane == 0 && row0 < p.rows && col < p.cols)
-                ptx::tma_store_2d(&p.out[0], sbuf + (c & 1) * 2048, col, row0);
+                ptx::tma_store_2d(&p.out[0], sbuf + (used & 1) * 2048, col, row0);
             }
           }
         } else if constexpr (EPI == FDMOE_EPI_GATED_GRAD) {
@@ -395,21 +438,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           for (int i = 0; i < 16; ++i) h[i] = pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), p.bf16);
           if (lane == 0) ptx::bulk_wait_group_read1();
           __syncwarp();
-          stage_half(buf + (c & 1) * 2048, lane, h);
+          stage_half(buf + (used & 1) * 2048, lane, h);
           ptx::fence_proxy_async_shared();
           __syncwarp();
           if (lane == 0 && row0 < p.rows && col < p.cols)
-            ptx::tma_store_2d(&p.out[0], sbuf + (c & 1) * 2048, col, row0);
+            ptx::tma_store_2d(&p.out[0], sbuf + (used & 1) * 2048, col, row0);
         }
         if (lane == 0) ptx::bulk_commit_group();
       }
       ptx::tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(acc_empty + acc), 0));
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(acc_empty + acc), leader));
     }
     if (lane == 0) ptx::bulk_wait_group0();
   }
   __syncwarp();
+  if (warp < 4 && split > 1) ptx::cluster_sync();  // the epilogue warps' exchange of partial sums
   ptx::tcgen05_fence_before();
   __syncthreads();
   wt.drain();
@@ -462,7 +506,6 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
 
   if (warp == 4) {
     if (lane == 0) {
-      ptx::grid_launch_dependents();
       auto load_weights = [&](int s, int kb) {
         uint64_t* bar = full + s;
         uint8_t* sa = smem + s * stage_bytes;
@@ -481,6 +524,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
       if (p.early_weights)
         for (; ahead < p.stages && kb0 + ahead < kb1; ++ahead) load_weights(ahead, kb0 + ahead);
       ptx::grid_wait_dependency();
+      // Only now may the next launch start: what it reads early was written before this launch's predecessor ended.
+      ptx::grid_launch_dependents();
       for (int kb = kb0; kb < kb1; ++kb) {
         const int i = kb - kb0, s = i % p.stages;
         if (i >= ahead) {

@@ -20,41 +20,47 @@ cudaError_t prepare_kernel(F kernel, int smem, std::atomic<uint64_t>& done) {
   return e;
 }
 
+// A launch with clusters of `cluster` CTAs along x.
+struct LaunchConfig {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  LaunchConfig(dim3 grid, int threads, int smem, int cluster, cudaStream_t stream) {
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+  }
+};
+
 template <bool MX4, int EPI>
-cudaError_t launch_pair(const FdmoePairParams& p, int sms, cudaStream_t stream) {
+cudaError_t launch_pair(const FdmoePairParams& p, int clusters, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
   constexpr int smem = PairShape<MX4, EPI>::kSmem;
   cudaError_t e = prepare_kernel(pair_gemm<MX4, EPI>, smem, done);
   if (e != cudaSuccess) return e;
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
-  pair_gemm<MX4, EPI><<<2 * pairs, kPairThreads, smem, stream>>>(p);
-  return cudaGetLastError();
+  const LaunchConfig l(dim3(clusters * 2 * p.split), kPairThreads, smem, 2 * p.split, stream);
+  return cudaLaunchKernelEx(&l.cfg, pair_gemm<MX4, EPI>, p);
 }
 
 constexpr int kStreamSmemMax = 227 * 1024 - 1024;  // beside the barriers in static shared memory
 
 template <bool MX4, int EPI>
-cudaError_t launch_stream(const FdmoeStreamParams& p, int smem, bool dependent, cudaStream_t stream) {
+cudaError_t launch_stream(const FdmoeStreamParams& p, int smem, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
   cudaError_t e = prepare_kernel(stream_gemm<MX4, EPI>, kStreamSmemMax, done);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.split, (p.rows + FDMOE_STREAM_ROWS - 1) / FDMOE_STREAM_ROWS,
-                     (p.tokens + p.tile_tokens - 1) / p.tile_tokens);
-  cfg.blockDim = dim3(kStreamThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = dependent ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, stream_gemm<MX4, EPI>, p);
+  const LaunchConfig l(dim3(p.split, (p.rows + FDMOE_STREAM_ROWS - 1) / FDMOE_STREAM_ROWS,
+                            (p.tokens + p.tile_tokens - 1) / p.tile_tokens),
+                       kStreamThreads, smem, p.split, stream);
+  return cudaLaunchKernelEx(&l.cfg, stream_gemm<MX4, EPI>, p);
 }
 
 }  // namespace dense

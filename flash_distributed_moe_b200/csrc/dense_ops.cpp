@@ -44,13 +44,14 @@ struct Shared {
   std::mutex mutex;
   uint32_t* status = nullptr;
   EncodeTiledFn encode = nullptr;
-  int sms[64] = {0};
+  bool known[64] = {};
+  fdmoe::DeviceSlots slots[64];
 } g_shared;
 
 struct Call {
   uint32_t* status;
   EncodeTiledFn encode;
-  int sms;
+  const fdmoe::DeviceSlots* slots;
   uint64_t timeout_ns;
   cudaStream_t stream;
 };
@@ -78,8 +79,15 @@ int BeginCall(Call* c, void* stream) {
     MOE_ERROR_LOG("cuTensorMapEncodeTiled is not available from this driver");
     return (int)cudaErrorUnknown;
   }
-  if (!g_shared.sms[dev])
-    DENSE_CHECK(cudaDeviceGetAttribute(&g_shared.sms[dev], cudaDevAttrMultiProcessorCount, dev));
+  if (!g_shared.known[dev]) {
+    fdmoe::DeviceSlots& d = g_shared.slots[dev];
+    for (int n = 1; n <= FDMOE_STREAM_SPLIT; ++n) {
+      DENSE_CHECK(fdmoe_stream_clusters(n, fdmoe::kStreamSmemOne, &d.stream_one[n]));
+      DENSE_CHECK(fdmoe_stream_clusters(n, fdmoe::kStreamSmemTwo, &d.stream_two[n]));
+    }
+    for (int n = 1; n <= FDMOE_PAIR_SPLIT; n *= 2) DENSE_CHECK(fdmoe_pair_clusters(2 * n, &d.pair[n]));
+    g_shared.known[dev] = true;
+  }
   const uint32_t seen = *static_cast<volatile uint32_t*>(g_shared.status);
   if (seen) {
     MOE_ERROR_LOG("refused after device-side error %u; see FlashMoeDenseStatus", seen);
@@ -87,7 +95,7 @@ int BeginCall(Call* c, void* stream) {
   }
   c->status = g_shared.status;
   c->encode = g_shared.encode;
-  c->sms = g_shared.sms[dev];
+  c->slots = &g_shared.slots[dev];
   const char* env = getenv("FLASHMOE_TIMEOUT_MS");
   c->timeout_ns = (uint64_t)std::max(1, env && *env ? atoi(env) : 2000) * 1000000ull;
   c->stream = static_cast<cudaStream_t>(stream);
@@ -137,14 +145,20 @@ int OperandMap(const Call& c, FdmoeTensorMap* out, const Operand& o, int box_row
   return MakeMap(c, out, o.base, 2, o.rows, o.cols, o.cols * 2, 64, o.mn ? 64 : box_rows);
 }
 
-void PairShape(FdmoePairParams& p, const Call& c, int64_t rows, int64_t cols, int64_t k, int tile_cols, int stage_k) {
+// The shape of a launch of the pair kernel; returns its number of clusters.
+int PairShape(FdmoePairParams& p, const Call& c, int64_t rows, int64_t cols, int64_t k, bool gated, bool mx4) {
+  const int stage_k = mx4 ? FDMOE_MX4_STAGE_K : 64;
   p.status = c.status;
   p.timeout_ns = c.timeout_ns;
   p.rows = (int32_t)rows;
   p.cols = (int32_t)cols;
-  p.tiles_m = (int32_t)((rows + FDMOE_PAIR_TILE - 1) / FDMOE_PAIR_TILE);
-  p.tiles_n = (int32_t)((cols + tile_cols - 1) / tile_cols);
   p.kblocks = (int32_t)((k + stage_k - 1) / stage_k);
+  const fdmoe::PairPlan plan = fdmoe::MakePairPlan(rows, cols, p.kblocks, gated, mx4, *c.slots);
+  p.tile_n = plan.tile_n;
+  p.split = plan.split;
+  p.tiles_m = plan.tiles_m;
+  p.tiles_n = plan.tiles_n;
+  return plan.clusters;
 }
 
 // out[rows, cols] = A B^T, both given as stored.
@@ -152,23 +166,23 @@ int PairProduct(const Call& c, const Operand& a, const Operand& b, void* out, bo
   FdmoePairParams p;
   memset(&p, 0, sizeof(p));
   const int64_t rows = a.mn ? a.cols : a.rows, cols = b.mn ? b.cols : b.rows, k = a.mn ? a.rows : a.cols;
-  PairShape(p, c, rows, cols, k, FDMOE_PAIR_TILE, 64);
+  const int clusters = PairShape(p, c, rows, cols, k, false, false);
   DENSE_TRY(OperandMap(c, &p.a, a, 128));
-  DENSE_TRY(OperandMap(c, &p.b, b, 128));
+  DENSE_TRY(OperandMap(c, &p.b, b, p.tile_n / 2));
   DENSE_TRY(MakeMap(c, &p.out[0], out, 2, rows, cols, cols * 2, 32, 32));
   p.a_mn = a.mn;
   p.b_mn = b.mn;
   p.bf16 = bf16;
-  return fdmoe_pair_launch(&p, FDMOE_EPI_HALF, 0, c.sms, c.stream);
+  return fdmoe_pair_launch(&p, FDMOE_EPI_HALF, 0, clusters, c.stream);
 }
 
 // out[tokens, rows] = x w^T (gated: silu(x w[:rows]^T) * (x w[rows:]^T)) for few tokens.
 int StreamProduct(const Call& c, const void* x, const void* w, void* out, int64_t tokens, int64_t rows, int64_t k,
-                  bool gated, bool bf16, bool dependent) {
+                  bool gated, bool bf16, bool early_weights) {
   FdmoeStreamParams p;
   memset(&p, 0, sizeof(p));
   const int kblocks = (int)((k + 63) / 64);
-  const fdmoe::StreamPlan s = fdmoe::MakeStreamPlan((int)rows, (int)tokens, kblocks, gated, false, c.sms);
+  const fdmoe::StreamPlan s = fdmoe::MakeStreamPlan((int)rows, (int)tokens, kblocks, gated, false, *c.slots);
   DENSE_TRY(MakeMap(c, &p.a, w, 2, gated ? 2 * rows : rows, k, k * 2, 64, 128));
   DENSE_TRY(MakeMap(c, &p.b, x, 2, tokens, k, k * 2, 64, s.tile_tokens));
   p.out = out;
@@ -184,8 +198,8 @@ int StreamProduct(const Call& c, const void* x, const void* w, void* out, int64_
   p.up_row = (int32_t)rows;
   p.bf16 = bf16;
   p.tmem_cols = s.tmem_cols;
-  p.early_weights = dependent;
-  return fdmoe_stream_launch(&p, gated ? FDMOE_EPI_GATED : FDMOE_EPI_HALF, 0, s.smem, dependent, c.stream);
+  p.early_weights = early_weights;
+  return fdmoe_stream_launch(&p, gated ? FDMOE_EPI_GATED : FDMOE_EPI_HALF, 0, s.smem, c.stream);
 }
 
 // h[T, I] = silu(g) * u with [g, u] = x w13^T; also g and u to gu [T, 2I] where that is given.
@@ -193,9 +207,9 @@ int GatedProduct(const Call& c, const void* x, const void* w13, void* h, void* g
                  bool bf16, bool stall) {
   FdmoePairParams p;
   memset(&p, 0, sizeof(p));
-  PairShape(p, c, T, I, H, 128, 64);
+  const int clusters = PairShape(p, c, T, I, H, true, false);
   DENSE_TRY(MakeMap(c, &p.a, x, 2, T, H, H * 2, 64, 128));
-  DENSE_TRY(MakeMap(c, &p.b, w13, 2, 2 * I, H, H * 2, 64, 128));
+  DENSE_TRY(MakeMap(c, &p.b, w13, 2, 2 * I, H, H * 2, 64, p.tile_n / 2));
   DENSE_TRY(MakeMap(c, &p.out[0], h, 2, T, I, I * 2, 32, 32));
   if (gu) {
     // two matrices side by side: what a tile has beyond column I of the gate projection is not stored
@@ -206,7 +220,7 @@ int GatedProduct(const Call& c, const void* x, const void* w13, void* h, void* g
   p.bf16 = bf16;
   p.save_gu = gu != nullptr;
   p.stall = stall;
-  return fdmoe_pair_launch(&p, FDMOE_EPI_GATED, 0, c.sms, c.stream);
+  return fdmoe_pair_launch(&p, FDMOE_EPI_GATED, 0, clusters, c.stream);
 }
 
 // From dy: dgu [T, 2I] and h [T, I].
@@ -214,7 +228,7 @@ int GatedGradient(const Call& c, const void* dy, const void* w2, const void* gu,
                   int64_t I, bool bf16) {
   FdmoePairParams p;
   memset(&p, 0, sizeof(p));
-  PairShape(p, c, T, I, H, FDMOE_PAIR_TILE, 64);
+  const int clusters = PairShape(p, c, T, I, H, false, false);
   DENSE_TRY(MakeMap(c, &p.a, dy, 2, T, H, H * 2, 64, 128));
   DENSE_TRY(MakeMap(c, &p.b, w2, 2, H, I, I * 2, 64, 64));
   DENSE_TRY(MakeMap(c, &p.out[0], dgu, 2, T, I, I * 4, 32, 32));
@@ -223,7 +237,7 @@ int GatedGradient(const Call& c, const void* dy, const void* w2, const void* gu,
   p.gu = gu;
   p.b_mn = 1;
   p.bf16 = bf16;
-  return fdmoe_pair_launch(&p, FDMOE_EPI_GATED_GRAD, 0, c.sms, c.stream);
+  return fdmoe_pair_launch(&p, FDMOE_EPI_GATED_GRAD, 0, clusters, c.stream);
 }
 
 // ------------------------------------------------------ products of 4-bit operands
@@ -240,7 +254,7 @@ int Mx4Maps(const Call& c, FdmoeTensorMap* values, FdmoeTensorMap* scales, const
   return MakeMap(c, scales, m.scales, 4, blocks * chunks, 128, 512, 128, 2);
 }
 
-int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, int64_t k, bool gated, bool dependent,
+int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, int64_t k, bool gated,
                bool early_weights) {
   const int64_t tokens = a.rows, rows = b.rows;
   const int kblocks = (int)((k + FDMOE_MX4_STAGE_K - 1) / FDMOE_MX4_STAGE_K);
@@ -250,7 +264,7 @@ int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, 
   if (fdmoe::UseStream((int)std::min<int64_t>(tokens, 1 << 30)) || (dtype == kF32 ? rows % 4 : rows % 8) != 0) {
     FdmoeStreamParams p;
     memset(&p, 0, sizeof(p));
-    const fdmoe::StreamPlan s = fdmoe::MakeStreamPlan((int)rows, (int)tokens, kblocks, gated, true, c.sms);
+    const fdmoe::StreamPlan s = fdmoe::MakeStreamPlan((int)rows, (int)tokens, kblocks, gated, true, *c.slots);
     DENSE_TRY(Mx4Maps(c, &p.a, &p.sfa, b, k, 128));
     DENSE_TRY(Mx4Maps(c, &p.b, &p.sfb, a, k, s.tile_tokens));
     p.out = out;
@@ -269,11 +283,11 @@ int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, 
     p.bf16 = dtype == kBf16;
     p.tmem_cols = s.tmem_cols;
     p.early_weights = early_weights;
-    return fdmoe_stream_launch(&p, epi, 1, s.smem, dependent, c.stream);
+    return fdmoe_stream_launch(&p, epi, 1, s.smem, c.stream);
   }
   FdmoePairParams p;
   memset(&p, 0, sizeof(p));
-  PairShape(p, c, tokens, rows, k, gated ? 128 : FDMOE_PAIR_TILE, FDMOE_MX4_STAGE_K);
+  const int clusters = PairShape(p, c, tokens, rows, k, gated, true);
   DENSE_TRY(Mx4Maps(c, &p.a, &p.sfa, a, k, 128));
   DENSE_TRY(Mx4Maps(c, &p.b, &p.sfb, b, k, 128));
   const int size = dtype == kF32 ? 4 : 2;
@@ -282,7 +296,7 @@ int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, 
   p.sf_chunks = chunks;
   p.sf_up_block = up_block;
   p.bf16 = dtype == kBf16;
-  return fdmoe_pair_launch(&p, epi, 1, c.sms, c.stream);
+  return fdmoe_pair_launch(&p, epi, 1, clusters, c.stream);
 }
 
 // ------------------------------------------------------------------- checks
@@ -422,8 +436,7 @@ extern "C" int FlashMoeMx4Matmul(const void* aValues, const void* aScales, const
     return (int)cudaErrorInvalidValue;
   Call c;
   DENSE_TRY(BeginCall(&c, stream));
-  return Mx4Product(c, {aValues, aScales, m, 1}, {bValues, bScales, n, gated ? 2 : 1}, out, dtype, k, gated != 0, false,
-                    false);
+  return Mx4Product(c, {aValues, aScales, m, 1}, {bValues, bScales, n, gated ? 2 : 1}, out, dtype, k, gated != 0, false);
 }
 
 // Workspace of the block on 4-bit weights: 4-bit tokens, activations, 4-bit activations.
@@ -472,8 +485,7 @@ extern "C" int FlashMoeMx4FfnForward(const FlashMoeFfnConfig* cfg, const void* x
   const Mx4FfnLayout l = MakeMx4FfnLayout(T, H, I);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   DENSE_TRY(fdmoe_mx4_quantize(x, cfg->dtype, 1, T, H, 0, H, ws + l.xv, ws + l.xs, stream));
-  DENSE_TRY(Mx4Product(c, {ws + l.xv, ws + l.xs, T, 1}, {w13Values, w13Scales, I, 2}, ws + l.h, cfg->dtype, H, true, false,
-                       false));
+  DENSE_TRY(Mx4Product(c, {ws + l.xv, ws + l.xs, T, 1}, {w13Values, w13Scales, I, 2}, ws + l.h, cfg->dtype, H, true, true));
   DENSE_TRY(fdmoe_mx4_quantize(ws + l.h, cfg->dtype, 1, T, I, 0, I, ws + l.hv, ws + l.hs, stream));
-  return Mx4Product(c, {ws + l.hv, ws + l.hs, T, 1}, {w2Values, w2Scales, H, 1}, y, cfg->dtype, I, false, false, false);
+  return Mx4Product(c, {ws + l.hv, ws + l.hs, T, 1}, {w2Values, w2Scales, H, 1}, y, cfg->dtype, I, false, true);
 }

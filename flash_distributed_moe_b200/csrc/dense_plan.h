@@ -19,8 +19,14 @@ struct StreamPlan {
 
 inline int RoundUp(int v, int m) { return (v + m - 1) / m * m; }
 
+// What the device runs at once: clusters of n CTAs of the streaming kernel with one or two CTAs per SM, and of the
+// pair kernel with n pairs.  A GPC's SMs hold whole clusters only, so these are fewer than the SMs would give.
+struct DeviceSlots {
+  int stream_one[FDMOE_STREAM_SPLIT + 1], stream_two[FDMOE_STREAM_SPLIT + 1], pair[FDMOE_PAIR_SPLIT + 1];
+};
+
 // `rows` weight rows (gated: of each projection), `tokens` >= 1, `kblocks` stages of k in all.
-inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, bool mx4, int sms) {
+inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, bool mx4, const DeviceSlots& dev) {
   StreamPlan s;
   const int parts = gated ? 2 : 1;
   s.token_tiles = (tokens + FDMOE_STREAM_TOKENS - 1) / FDMOE_STREAM_TOKENS;
@@ -35,8 +41,9 @@ inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, 
   double best = 0;
   s.split = 1;
   for (int n = 1; n <= FDMOE_STREAM_SPLIT && n <= kblocks; ++n) {
-    const int64_t ctas = (int64_t)s.row_tiles * s.token_tiles * n, slots = (int64_t)sms * s.per_sm;
-    const double t = (double)((ctas + slots - 1) / slots) * ((kblocks + n - 1) / n + 6);
+    const int64_t clusters = (int64_t)s.row_tiles * s.token_tiles;
+    const int64_t slots = std::max(1, s.per_sm == 2 ? dev.stream_two[n] : dev.stream_one[n]);
+    const double t = (double)((clusters + slots - 1) / slots) * ((kblocks + n - 1) / n + 6);
     if (n == 1 || t < best) best = t, s.split = n;
   }
   s.stages = std::min(std::min(room / stage, (int)FDMOE_STREAM_STAGES), (kblocks + s.split - 1) / s.split);
@@ -50,8 +57,37 @@ inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, 
   return s;
 }
 
+struct PairPlan {
+  int tile_n, split, tiles_m, tiles_n, clusters;
+};
+
+// `cols`: of the result; `kblocks` stages of k.  Time in cycles: the waves of tiles, each its k blocks' MMAs, and once
+// per launch (per cluster where pairs share a tile) its beginning and end.
+inline PairPlan MakePairPlan(int64_t rows, int64_t cols, int kblocks, bool gated, bool mx4, const DeviceSlots& dev) {
+  PairPlan best = {};
+  double best_time = 0;
+  for (int tile_n = 256; tile_n >= (mx4 ? 256 : 128); tile_n /= 2)
+    for (int split = 1; split <= FDMOE_PAIR_SPLIT && split <= kblocks; split *= 2) {
+      PairPlan p;
+      p.tile_n = tile_n;
+      p.split = split;
+      p.tiles_m = (int)((rows + FDMOE_PAIR_TILE - 1) / FDMOE_PAIR_TILE);
+      const int tile_cols = gated ? tile_n / 2 : tile_n;
+      p.tiles_n = (int)((cols + tile_cols - 1) / tile_cols);
+      const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, slots = std::max(1, dev.pair[split]);
+      const double waves = (double)((tiles + slots - 1) / slots);
+      const double block = tile_n == 256 ? 512 : 330;
+      const double k = (double)((kblocks + split - 1) / split) * block;
+      const double t = split == 1 ? waves * k + 3000 : waves * (k + 6000);
+      p.clusters = (int)(split == 1 ? std::min(tiles, slots) : tiles);
+      if (best_time == 0 || t < best_time) best = p, best_time = t;
+    }
+  return best;
+}
+
 // Whether the streaming kernel takes a product instead of the pair kernel.
 inline bool UseStream(int tokens) { return tokens <= FDMOE_STREAM_TOKENS; }
+
 
 inline size_t AlignBytes(size_t v) { return (v + 255) / 256 * 256; }
 

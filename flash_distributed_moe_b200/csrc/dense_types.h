@@ -11,7 +11,8 @@ extern "C" {
 #endif
 
 enum {
-  FDMOE_PAIR_TILE = 256,      // rows and columns of a tile of the pair kernel
+  FDMOE_PAIR_TILE = 256,      // rows of a tile of the pair kernel, and most columns
+  FDMOE_PAIR_SPLIT = 4,       // most pairs that share the k axis of a tile of the pair kernel
   FDMOE_STREAM_ROWS = 128,    // weight rows of a tile of the streaming kernel
   FDMOE_STREAM_TOKENS = 128,  // most tokens of a tile of the streaming kernel
   FDMOE_STREAM_SPLIT = 8,     // most CTAs that share the k axis of a tile of the streaming kernel
@@ -46,6 +47,8 @@ typedef struct {
   uint64_t timeout_ns;
   int32_t rows, cols;         // of the result
   int32_t tiles_m, tiles_n;
+  int32_t tile_n;             // 256 or 128 (4-bit operands: 256)
+  int32_t split;              // 1, 2 or 4 pairs per tile; above 1 a launch has a cluster per tile
   int32_t kblocks;
   int32_t a_mn, b_mn;         // operand stored with its rows along M (N) instead of along K
   int32_t up_row;             // row of `b` at which the up projection starts (gated)
@@ -54,7 +57,6 @@ typedef struct {
   int32_t bf16;               // 16-bit operands and results are bf16, otherwise fp16
   int32_t save_gu;            // gated: also write the gate and up projections
   int32_t stall;              // test hook: nothing is loaded, every wait runs out
-  int32_t reserved;
 } FdmoePairParams;
 
 typedef struct {
@@ -78,9 +80,15 @@ typedef struct {
 } FdmoeStreamParams;
 
 // Launchers; return a cudaError_t.  `mx4` selects 4-bit operands.
-int fdmoe_pair_launch(const FdmoePairParams* p, int epi, int mx4, int sms, void* stream);
-// `dependent`: may start before the launch before it has ended (it waits for that by itself).
-int fdmoe_stream_launch(const FdmoeStreamParams* p, int epi, int mx4, int smem, int dependent, void* stream);
+// Every kernel of the dense operators may start before the launch before it on the stream has ended, and waits for
+// that itself before it touches global memory (programmatic dependent launch): set-up and launch latency overlap.
+int fdmoe_pair_launch(const FdmoePairParams* p, int epi, int mx4, int clusters, void* stream);
+int fdmoe_stream_launch(const FdmoeStreamParams* p, int epi, int mx4, int smem, void* stream);
+
+// Clusters of `size` CTAs of the pair kernel, or of the streaming kernel with `smem` bytes, that the current device
+// runs at once.
+int fdmoe_pair_clusters(int size, int* out);
+int fdmoe_stream_clusters(int size, int smem, int* out);
 
 int fdmoe_mx4_quantize(const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols, int64_t batch_stride,
                        int64_t row_stride, void* values, void* scales, void* stream);

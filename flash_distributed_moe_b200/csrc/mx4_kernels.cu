@@ -64,6 +64,8 @@ struct QuantParams {
 template <bool F32>
 __global__ void __launch_bounds__(kQuantThreads) mx4_quantize_kernel(const QuantParams p) {
   __shared__ __align__(16) uint8_t sc[2 * kScaleBlock];
+  ptx::grid_wait_dependency();
+  ptx::grid_launch_dependents();
   const int64_t batch = blockIdx.z, row0 = (int64_t)blockIdx.x * kQuantRows;
   const int64_t blocks = p.cols / FDMOE_MX4_BLOCK, blk0 = (int64_t)blockIdx.y * kQuantBlocks;
   const int rows = (int)min((int64_t)kQuantRows, p.rows - row0);
@@ -115,6 +117,8 @@ struct DequantParams {
 template <bool F32>
 __global__ void __launch_bounds__(kQuantThreads) mx4_dequantize_kernel(const DequantParams p) {
   __shared__ __align__(16) uint8_t sc[2 * kScaleBlock];
+  ptx::grid_wait_dependency();
+  ptx::grid_launch_dependents();
   const int64_t batch = blockIdx.z, row0 = (int64_t)blockIdx.x * kQuantRows;
   const int64_t blocks = p.cols / FDMOE_MX4_BLOCK, blk0 = (int64_t)blockIdx.y * kQuantBlocks;
   const int rows = (int)min((int64_t)kQuantRows, p.rows - row0);
@@ -163,43 +167,33 @@ extern "C" int fdmoe_mx4_quantize(const void* x, int dtype, int64_t batch, int64
                                   int64_t batch_stride, int64_t row_stride, void* values, void* scales, void* stream) {
   const QuantParams p{x, static_cast<uint8_t*>(values), static_cast<uint8_t*>(scales), rows, cols, batch_stride,
                       row_stride, dtype};
-  const dim3 grid = quant_grid(batch, rows, cols);
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == 1)
-    mx4_quantize_kernel<true><<<grid, kQuantThreads, 0, s>>>(p);
-  else
-    mx4_quantize_kernel<false><<<grid, kQuantThreads, 0, s>>>(p);
-  return cudaGetLastError();
+  const LaunchConfig l(quant_grid(batch, rows, cols), kQuantThreads, 0, 1, static_cast<cudaStream_t>(stream));
+  return dtype == 1 ? cudaLaunchKernelEx(&l.cfg, mx4_quantize_kernel<true>, p) : cudaLaunchKernelEx(&l.cfg, mx4_quantize_kernel<false>, p);
 }
 
 extern "C" int fdmoe_mx4_dequantize(const void* values, const void* scales, int64_t batch, int64_t rows, int64_t cols,
                                     int dtype, void* out, void* stream) {
   const DequantParams p{static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(scales), out, rows, cols, dtype};
-  const dim3 grid = quant_grid(batch, rows, cols);
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == 1)
-    mx4_dequantize_kernel<true><<<grid, kQuantThreads, 0, s>>>(p);
-  else
-    mx4_dequantize_kernel<false><<<grid, kQuantThreads, 0, s>>>(p);
-  return cudaGetLastError();
+  const LaunchConfig l(quant_grid(batch, rows, cols), kQuantThreads, 0, 1, static_cast<cudaStream_t>(stream));
+  return dtype == 1 ? cudaLaunchKernelEx(&l.cfg, mx4_dequantize_kernel<true>, p) : cudaLaunchKernelEx(&l.cfg, mx4_dequantize_kernel<false>, p);
 }
 
-cudaError_t fdmoe_pair_launch_mx4(const FdmoePairParams& p, int epi, int sms, cudaStream_t s) {
+cudaError_t fdmoe_pair_launch_mx4(const FdmoePairParams& p, int epi, int clusters, cudaStream_t s) {
   switch (epi) {
-    case FDMOE_EPI_HALF: return launch_pair<true, FDMOE_EPI_HALF>(p, sms, s);
-    case FDMOE_EPI_F32: return launch_pair<true, FDMOE_EPI_F32>(p, sms, s);
-    case FDMOE_EPI_GATED: return launch_pair<true, FDMOE_EPI_GATED>(p, sms, s);
-    case FDMOE_EPI_GATED_F32: return launch_pair<true, FDMOE_EPI_GATED_F32>(p, sms, s);
+    case FDMOE_EPI_HALF: return launch_pair<true, FDMOE_EPI_HALF>(p, clusters, s);
+    case FDMOE_EPI_F32: return launch_pair<true, FDMOE_EPI_F32>(p, clusters, s);
+    case FDMOE_EPI_GATED: return launch_pair<true, FDMOE_EPI_GATED>(p, clusters, s);
+    case FDMOE_EPI_GATED_F32: return launch_pair<true, FDMOE_EPI_GATED_F32>(p, clusters, s);
   }
   return cudaErrorInvalidValue;
 }
 
-cudaError_t fdmoe_stream_launch_mx4(const FdmoeStreamParams& p, int epi, int smem, bool dependent, cudaStream_t s) {
+cudaError_t fdmoe_stream_launch_mx4(const FdmoeStreamParams& p, int epi, int smem, cudaStream_t s) {
   switch (epi) {
-    case FDMOE_EPI_HALF: return launch_stream<true, FDMOE_EPI_HALF>(p, smem, dependent, s);
-    case FDMOE_EPI_F32: return launch_stream<true, FDMOE_EPI_F32>(p, smem, dependent, s);
-    case FDMOE_EPI_GATED: return launch_stream<true, FDMOE_EPI_GATED>(p, smem, dependent, s);
-    case FDMOE_EPI_GATED_F32: return launch_stream<true, FDMOE_EPI_GATED_F32>(p, smem, dependent, s);
+    case FDMOE_EPI_HALF: return launch_stream<true, FDMOE_EPI_HALF>(p, smem, s);
+    case FDMOE_EPI_F32: return launch_stream<true, FDMOE_EPI_F32>(p, smem, s);
+    case FDMOE_EPI_GATED: return launch_stream<true, FDMOE_EPI_GATED>(p, smem, s);
+    case FDMOE_EPI_GATED_F32: return launch_stream<true, FDMOE_EPI_GATED_F32>(p, smem, s);
   }
   return cudaErrorInvalidValue;
 }

@@ -8,61 +8,62 @@ first, and [H, I].  bf16 or fp16, or, without gradients, 4-bit weights (`quantiz
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Tuple, Union
 
 import torch
 
 from . import _lib
-from .flashMoeLauncher import _stream_ptr
 from .flashMx4 import Mx4Tensor, mx4_quantize
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 2}
 Weight = Union[torch.Tensor, Mx4Tensor]
 
 
+@functools.lru_cache(maxsize=1024)
 def _config(hidden: int, inter: int, dtype: torch.dtype):
     return C.byref(_lib.FlashMoeFfnConfig(hidden, inter, _DTYPES[dtype], (C.c_int32 * 5)()))
 
 
-def _check(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
+def _check(t: torch.Tensor, name: str) -> None:
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name} tensor is undefined")
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor")
     if t.dtype not in _DTYPES:
         raise RuntimeError(f"{name} must be bfloat16 or float16")
-    if t.dtype != like.dtype or t.device != like.device:
-        raise RuntimeError(f"{name} must have the dtype and device of x")
 
 
 def _check_weights(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> None:
-    _check(w13, "w13", x)
-    _check(w2, "w2", x)
     for t, name in ((w13, "w13"), (w2, "w2")):
+        _check(t, name)
+        if t.dtype != x.dtype or t.device != x.device:
+            raise RuntimeError(f"{name} must have the dtype and device of x")
         if not t.is_contiguous() or t.data_ptr() % 16:
             raise RuntimeError(f"{name} must be contiguous and start on 16 bytes")
-    if w2.dim() != 2 or tuple(w13.shape) != (2 * w2.shape[1], w2.shape[0]) or x.shape[-1] != w2.shape[0]:
+    shape = w2.shape
+    if len(shape) != 2 or w13.shape != (2 * shape[1], shape[0]) or x.shape[-1] != shape[0]:
         raise RuntimeError("x, w13 and w2 must be [..., hidden], [2*inter, hidden] and [hidden, inter]")
-    if w2.shape[0] % 8 or w2.shape[1] % 8 or w2.numel() == 0:
+    if shape[0] % 8 or shape[1] % 8 or shape[0] == 0 or shape[1] == 0:
         raise RuntimeError("hidden and inter must be multiples of 8")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., n] as contiguous rows on 16 bytes; a copy only where the tensor is neither."""
-    t = t.reshape(-1, t.shape[-1]).contiguous()
+    if t.dim() != 2 or not t.is_contiguous():
+        t = t.reshape(-1, t.shape[-1]).contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _forward(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, save: bool):
-    (hidden, inter), tokens, lib = w2.shape, x.shape[0], _lib.lib()
+    (hidden, inter), tokens = w2.shape, x.shape[0]
+    cfg = _config(hidden, inter, x.dtype)
     y = torch.empty_like(x)
     gate_up = torch.empty((tokens, 2 * inter), dtype=x.dtype, device=x.device) if save else None
-    with torch.cuda.device(x.device):
-        cfg = _config(hidden, inter, x.dtype)
-        ws = torch.empty(lib.FlashMoeFfnWorkspaceBytes(cfg, tokens, 0), dtype=torch.uint8, device=x.device)
-        _lib.check(lib.FlashMoeFfnForward(cfg, x.data_ptr(), w13.data_ptr(), w2.data_ptr(), y.data_ptr(),
-                                          gate_up.data_ptr() if save else None, ws.data_ptr(), ws.numel(), tokens,
-                                          _stream_ptr()), "FfnForward")
+    nbytes = _lib.lib().FlashMoeFfnWorkspaceBytes(cfg, tokens, 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _lib.run(x.get_device(), "FlashMoeFfnForward", cfg, x.data_ptr(), w13.data_ptr(), w2.data_ptr(), y.data_ptr(),
+             gate_up.data_ptr() if save else None, ws.data_ptr(), nbytes, tokens)
     return y, gate_up
 
 
@@ -77,15 +78,14 @@ class _GatedFfn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, w13, w2, gate_up = ctx.saved_tensors
-        (hidden, inter), tokens, lib = w2.shape, x.shape[0], _lib.lib()
+        (hidden, inter), tokens = w2.shape, x.shape[0]
+        cfg = _config(hidden, inter, x.dtype)
         dy = _rows(dy)
         grads = [torch.empty_like(t) if need else None for t, need in zip((x, w13, w2), ctx.needs_input_grad)]
-        with torch.cuda.device(x.device):
-            cfg = _config(hidden, inter, x.dtype)
-            ws = torch.empty(lib.FlashMoeFfnWorkspaceBytes(cfg, tokens, 1), dtype=torch.uint8, device=x.device)
-            _lib.check(lib.FlashMoeFfnBackward(cfg, dy.data_ptr(), x.data_ptr(), w13.data_ptr(), w2.data_ptr(),
-                                               gate_up.data_ptr(), *[None if g is None else g.data_ptr() for g in grads],
-                                               ws.data_ptr(), ws.numel(), tokens, _stream_ptr()), "FfnBackward")
+        nbytes = _lib.lib().FlashMoeFfnWorkspaceBytes(cfg, tokens, 1)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _lib.run(x.get_device(), "FlashMoeFfnBackward", cfg, dy.data_ptr(), x.data_ptr(), w13.data_ptr(), w2.data_ptr(),
+                 gate_up.data_ptr(), *[None if g is None else g.data_ptr() for g in grads], ws.data_ptr(), nbytes, tokens)
         return tuple(grads)
 
 
@@ -97,20 +97,18 @@ def gated_ffn(x: torch.Tensor, w13: Weight, w2: Weight) -> torch.Tensor:
     A training step may be captured into a CUDA graph.  As with every torch operator, capture it while no eager graph
     of the same leaves is alive (torch keeps the gradient accumulators of such a graph on its stream, which must not
     join the capture), or take the gradients with `torch.autograd.grad`."""
-    if not isinstance(x, torch.Tensor):
-        raise RuntimeError("x tensor is undefined")
-    _check(x, "x", x)
+    _check(x, "x")
     if x.dim() < 1:
         raise RuntimeError("x must be [..., hidden]")
     if isinstance(w13, Mx4Tensor) or isinstance(w2, Mx4Tensor):
         return _mx4_ffn(x, w13, w2)
     _check_weights(x, w13, w2)
     rows = _rows(x)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w13, w2)):
+    if (x.requires_grad or w13.requires_grad or w2.requires_grad) and torch.is_grad_enabled():
         y = _GatedFfn.apply(rows, w13, w2)
     else:
         y, _ = _forward(rows, w13, w2, save=False)
-    return y.reshape(x.shape)
+    return y if x.dim() == 2 else y.reshape(x.shape)
 
 
 def quantize_ffn_weights(w13: torch.Tensor, w2: torch.Tensor) -> Tuple[Mx4Tensor, Mx4Tensor]:
@@ -131,14 +129,13 @@ def _mx4_ffn(x: torch.Tensor, w13: Mx4Tensor, w2: Mx4Tensor) -> torch.Tensor:
         raise RuntimeError("x, w13 and w2 must be [..., hidden], [2, inter, hidden] and [hidden, inter]")
     if w2.shape[0] % 32:
         raise RuntimeError("hidden and inter must be multiples of 32")
-    rows, (hidden, inter), lib = _rows(x.detach()), w2.shape, _lib.lib()
+    rows, (hidden, inter) = _rows(x.detach()), w2.shape
+    cfg = _config(hidden, inter, x.dtype)
     y = torch.empty_like(rows)
-    with torch.cuda.device(x.device):
-        cfg = _config(hidden, inter, x.dtype)
-        ws = torch.empty(lib.FlashMoeMx4FfnWorkspaceBytes(cfg, rows.shape[0]), dtype=torch.uint8, device=x.device)
-        _lib.check(lib.FlashMoeMx4FfnForward(cfg, rows.data_ptr(), w13.values.data_ptr(), w13.scales.data_ptr(),
-                                             w2.values.data_ptr(), w2.scales.data_ptr(), y.data_ptr(), ws.data_ptr(),
-                                             ws.numel(), rows.shape[0], _stream_ptr()), "Mx4FfnForward")
+    nbytes = _lib.lib().FlashMoeMx4FfnWorkspaceBytes(cfg, rows.shape[0])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _lib.run(x.get_device(), "FlashMoeMx4FfnForward", cfg, rows.data_ptr(), w13.values.data_ptr(), w13.scales.data_ptr(),
+             w2.values.data_ptr(), w2.scales.data_ptr(), y.data_ptr(), ws.data_ptr(), nbytes, rows.shape[0])
     return y.reshape(x.shape)
 
 

@@ -14,7 +14,6 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .flashMoeLauncher import _stream_ptr
 
 DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 
@@ -29,6 +28,8 @@ class Mx4Tensor:
     """A 4-bit matrix [rows, cols] or batch of them [batch, rows, cols].  `values` uint8 [..., rows, cols / 2] with the
     even element in the low half of a byte; `scales` uint8, in blocks of 512 for 128 rows and 128 columns."""
 
+    __slots__ = ("values", "scales", "shape")
+
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
         for t, name in ((values, "values"), (scales, "scales")):
             if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or not t.is_contiguous() or t.data_ptr() % 16:
@@ -36,33 +37,36 @@ class Mx4Tensor:
         if values.dim() not in (2, 3) or values.shape[-1] == 0 or values.shape[-1] % 16 != 0:
             raise RuntimeError("values must be [rows, cols / 2] or [batch, rows, cols / 2] with cols a multiple of 32")
         batch = 1 if values.dim() == 2 else values.shape[0]
-        if scales.numel() != batch * -(-values.shape[-2] // 128) * -(-values.shape[-1] // 128) * 1024:
+        if scales.numel() != _scale_bytes(batch, values.shape[-2], 2 * values.shape[-1]):
             raise RuntimeError("scales must have 512 bytes per 128 rows and 128 columns, an even number of blocks per row")
         if values.device != scales.device:
             raise RuntimeError("values and scales must be on the same device")
-        self.values, self.scales = values, scales
+        self._set(values, scales)
 
-    @property
-    def shape(self) -> torch.Size:
-        return torch.Size((*self.values.shape[:-1], self.values.shape[-1] * 2))
+    def _set(self, values, scales):
+        self.values, self.scales = values, scales
+        self.shape = torch.Size((*values.shape[:-1], values.shape[-1] * 2))
+        return self
 
     @property
     def device(self) -> torch.device:
         return self.values.device
 
-    def _sizes(self):
-        return (1, *self.shape) if len(self.shape) == 2 else tuple(self.shape)
-
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values that the matrix stands for.  Exact in fp32; in bf16 and fp16 unless they leave the type's range."""
         code = _check_dtype(dtype)
-        if not self.values.is_cuda:
+        values, shape = self.values, self.shape
+        if not values.is_cuda:
             raise RuntimeError("values must be a CUDA tensor")
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.lib().FlashMoeMx4Dequantize(self.values.data_ptr(), self.scales.data_ptr(), *self._sizes(),
-                                                        code, out.data_ptr(), _stream_ptr()), "Mx4Dequantize")
+        out = torch.empty(shape, dtype=dtype, device=values.device)
+        _lib.run(values.get_device(), "FlashMoeMx4Dequantize", values.data_ptr(), self.scales.data_ptr(),
+                 shape[0] if len(shape) == 3 else 1, shape[-2], shape[-1], code, out.data_ptr())
         return out
+
+
+def _scale_bytes(batch: int, rows: int, cols: int) -> int:
+    """The size of the scales, as FlashMoeMx4ScaleBytes gives it."""
+    return batch * -(-rows // 128) * -(-cols // 256) * 1024
 
 
 def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
@@ -73,40 +77,40 @@ def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
     if not x.is_cuda:
         raise RuntimeError("x must be a CUDA tensor")
     code = _check_dtype(x.dtype)
-    if x.dim() not in (2, 3) or x.shape[-1] == 0 or x.shape[-1] % 32 != 0:
+    shape = x.shape
+    if len(shape) not in (2, 3) or shape[-1] == 0 or shape[-1] % 32 != 0:
         raise RuntimeError("x must be [rows, cols] or [batch, rows, cols] with cols a multiple of 32")
-    x3 = x.detach() if x.dim() == 3 else x.detach().unsqueeze(0)
-    batch, rows, cols = x3.shape
-    per16 = 16 // x.element_size()
-    strides = (x3.stride(0) if batch > 1 else 0, x3.stride(1) if rows > 1 else 0)
-    if x3.numel() and (x3.stride(2) != 1 or strides[0] % per16 or strides[1] % per16 or x.data_ptr() % 16):
+    batch, rows, cols = shape if len(shape) == 3 else (1, *shape)
+    ptr = x.data_ptr()
+    if x.is_contiguous():
+        strides = (rows * cols, cols)  # multiples of 32 elements
+        aligned = ptr % 16 == 0
+    else:
+        per16 = 16 // x.element_size()
+        strides = (x.stride(0) if batch > 1 else 0, x.stride(-2) if rows > 1 else 0)
+        aligned = ptr % 16 == 0 and x.stride(-1) == 1 and strides[0] % per16 == 0 and strides[1] % per16 == 0
+    if not aligned:
         raise RuntimeError("rows of x must be contiguous and start on 16 bytes")
-    lib = _lib.lib()
-    nbytes = lib.FlashMoeMx4ScaleBytes(batch, rows, cols)
-    if nbytes == 0 and x3.numel():
-        raise RuntimeError("x is too large")
-    values = torch.empty((*x.shape[:-1], cols // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(lib.FlashMoeMx4Quantize(x.data_ptr(), code, batch, rows, cols, *strides, values.data_ptr(),
-                                           scales.data_ptr(), _stream_ptr()), "Mx4Quantize")
-    return Mx4Tensor(values, scales)
+    values = torch.empty((*shape[:-1], cols // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(_scale_bytes(batch, rows, cols), dtype=torch.uint8, device=x.device)
+    _lib.run(x.get_device(), "FlashMoeMx4Quantize", ptr, code, batch, rows, cols, *strides, values.data_ptr(),
+             scales.data_ptr())
+    return Mx4Tensor.__new__(Mx4Tensor)._set(values, scales)
 
 
 def _product(a: Mx4Tensor, b: Mx4Tensor, out_dtype: torch.dtype, gated: bool) -> torch.Tensor:
     if not isinstance(a, Mx4Tensor) or not isinstance(b, Mx4Tensor):
         raise RuntimeError("operands must be Mx4Tensors")
     code = _check_dtype(out_dtype)
-    if a.device != b.device or not a.values.is_cuda:
+    av, bv, sa, sb = a.values, b.values, a.shape, b.shape
+    if av.device != bv.device or not av.is_cuda:
         raise RuntimeError("operands must be on the same CUDA device")
-    if len(a.shape) != 2 or len(b.shape) != (3 if gated else 2) or a.shape[-1] != b.shape[-1] or (gated and b.shape[0] != 2):
+    if len(sa) != 2 or len(sb) != (3 if gated else 2) or sa[-1] != sb[-1] or (gated and sb[0] != 2):
         raise RuntimeError("operands must be [M, K] and " + ("[2, N, K]" if gated else "[N, K]"))
-    (m, k), n = a.shape, b.shape[-2]
-    out = torch.empty((m, n), dtype=out_dtype, device=a.device)
-    with torch.cuda.device(a.device):
-        _lib.check(_lib.lib().FlashMoeMx4Matmul(a.values.data_ptr(), a.scales.data_ptr(), b.values.data_ptr(),
-                                                b.scales.data_ptr(), out.data_ptr(), code, m, n, k, int(gated),
-                                                _stream_ptr()), "Mx4Matmul")
+    m, n = sa[0], sb[-2]
+    out = torch.empty((m, n), dtype=out_dtype, device=av.device)
+    _lib.run(av.get_device(), "FlashMoeMx4Matmul", av.data_ptr(), a.scales.data_ptr(), bv.data_ptr(), b.scales.data_ptr(),
+             out.data_ptr(), code, m, n, sa[1], int(gated))
     return out
 
 

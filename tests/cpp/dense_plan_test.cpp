@@ -25,7 +25,10 @@ int main() {
         for (int gated = 0; gated < 2; ++gated)
           for (int mx4 = 0; mx4 < 2; ++mx4)
             for (int sms : {148, 132, 8}) {
-              const StreamPlan s = MakeStreamPlan(rows, tokens, kb, gated, mx4, sms);
+              DeviceSlots dev;
+              for (int n = 1; n <= FDMOE_STREAM_SPLIT; ++n) dev.stream_one[n] = sms / n, dev.stream_two[n] = 2 * sms / n;
+              for (int n = 1; n <= FDMOE_PAIR_SPLIT; ++n) dev.pair[n] = sms / (2 * n);
+              const StreamPlan s = MakeStreamPlan(rows, tokens, kb, gated, mx4, dev);
               const int parts = gated ? 2 : 1;
               const int stage = parts * 16384 + s.tile_tokens * 128 + (mx4 ? (parts + 1) * 1024 : 0);
               CHECK(s.tile_tokens % 16 == 0 && s.tile_tokens >= 16 && s.tile_tokens <= FDMOE_STREAM_TOKENS);
@@ -41,6 +44,12 @@ int main() {
               const int cols = parts * s.tile_tokens + (mx4 ? s.stages * (parts + 1) * 8 : 0);
               CHECK(s.tmem_cols >= cols && s.tmem_cols >= 32 && (s.tmem_cols & (s.tmem_cols - 1)) == 0);
               CHECK(s.tmem_cols * s.per_sm <= 512);
+              const PairPlan q = MakePairPlan(tokens, rows, kb, gated, mx4, dev);
+              const int cols_tile = gated ? q.tile_n / 2 : q.tile_n;
+              CHECK(q.tile_n == 256 || (q.tile_n == 128 && !mx4));
+              CHECK((q.split == 1 || q.split == 2 || q.split == 4) && q.split <= kb);
+              CHECK(q.tiles_m * 256 >= tokens && q.tiles_n * cols_tile >= rows && q.clusters >= 1);
+              CHECK(q.split == 1 ? q.clusters <= q.tiles_m * q.tiles_n : q.clusters == q.tiles_m * q.tiles_n);
             }
   {
     const int rows = 0, tokens = 0, kb = 0, gated = 0, mx4 = 0;
