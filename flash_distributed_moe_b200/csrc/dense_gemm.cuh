@@ -26,14 +26,21 @@ struct Waiter {
   uint64_t limit_ns;
 
   __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint32_t code) const {
-    if (ptx::mbar_try_wait_cluster(bar, parity)) return true;
+    if (ptx::mbar_try_wait(bar, parity)) return true;
     return slow(bar, parity, code);
+  }
+  // The same by a whole warp.  The warps that issue copies and MMAs run their loops together and let one elected lane
+  // issue: inside a branch on the lane the compiler cannot tell that one thread is active, and instructions whose
+  // operands have to be uniform cost several times as much (the pair kernel's k block took 684 cycles so, whatever the
+  // tile's width).
+  __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, uint32_t code) const {
+    return __all_sync(0xffffffffu, wait(bar, parity, code));
   }
   __device__ __noinline__ bool slow(uint64_t* bar, uint32_t parity, uint32_t code) const {
     const uint64_t t0 = ptx::globaltimer_ns();
     for (;;) {
       for (int i = 0; i < 64; ++i)
-        if (ptx::mbar_try_wait_cluster(bar, parity)) return true;
+        if (ptx::mbar_try_wait(bar, parity)) return true;
       if (*abort_flag) return false;
       if (ptx::globaltimer_ns() - t0 > limit_ns) {
         atomicCAS_system(status, 0u, code);
@@ -175,9 +182,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
 
   if (warp == 0) {
     // ---- loads: both CTAs fill their own stages; the bytes are counted on the even CTA's barriers
-    if (lane == 0) {
-      ptx::prefetch_tmap(&p.a);
-      ptx::prefetch_tmap(&p.b);
+    {
+      const bool elected = ptx::elect_one();
       uint32_t it = 0;
       bool ok = true;
       for (int tile = first; ok && tile < tiles; tile += step) {
@@ -187,11 +193,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % S::kStages;
           const uint32_t ph = (it / S::kStages) & 1;
-          if (!wt.wait(empty + s, ph ^ 1, FDMOE_DENSE_TIMEOUT_EMPTY)) {
+          if (!wt.wait_warp(empty + s, ph ^ 1, FDMOE_DENSE_TIMEOUT_EMPTY)) {
             ok = false;
             break;
           }
-          if (p.stall) continue;
+          if (p.stall || !elected) continue;
           if (rank == 0) ptx::mbar_expect_tx(full + s, 2 * (kStageOperand + half_n * 128 + S::kScales));
           const uint32_t bar = ptx::map_rank(ptx::smem_u32(full + s), leader);
           const uint32_t sa = ptx::smem_u32(stages + s * 2 * kStageOperand), sb = sa + kStageOperand;
@@ -224,7 +230,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     }
   } else if (warp == 1) {
     // ---- MMAs: one thread of the even CTA
-    if (rank == 0 && lane == 0) {
+    if (rank == 0) {
+      const bool elected = ptx::elect_one();
       const uint32_t idesc = ptx::make_idesc_f16(256, p.tile_n, p.bf16, p.a_mn, p.b_mn);
       // 16 k further: 32 bytes along a row, or 16 rows of 128 bytes
       const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
@@ -234,16 +241,17 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       for (int tile = first; ok && tile < tiles; tile += step, ++n) {
         const int acc = n % S::kAccs;
         const uint32_t aph = (n / S::kAccs) & 1;
-        if (!wt.wait(acc_empty + acc, aph ^ 1, FDMOE_DENSE_TIMEOUT_ACC)) break;
+        if (!wt.wait_warp(acc_empty + acc, aph ^ 1, FDMOE_DENSE_TIMEOUT_ACC)) break;
         ptx::tcgen05_fence_after();
         const uint32_t d = tmem + acc * kAccCols;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % S::kStages;
-          if (!wt.wait(full + s, (it / S::kStages) & 1, FDMOE_DENSE_TIMEOUT_FULL)) {
+          if (!wt.wait_warp(full + s, (it / S::kStages) & 1, FDMOE_DENSE_TIMEOUT_FULL)) {
             ok = false;
             break;
           }
           ptx::tcgen05_fence_after();
+          if (!elected) continue;
           const uint32_t sa = ptx::smem_u32(stages + s * 2 * kStageOperand), sb = sa + kStageOperand;
           if (MX4) {
             const uint32_t sf = ptx::smem_u32(scales + s * S::kScales);
@@ -268,7 +276,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
           }
           ptx::umma_commit_pair(empty + s, leader);
         }
-        if (ok) ptx::umma_commit_pair(acc_full + acc, leader);
+        if (ok && elected) ptx::umma_commit_pair(acc_full + acc, leader);
       }
     }
   } else if (warp >= 4) {
@@ -505,7 +513,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
   const uint32_t tmem = tmem_slot;
 
   if (warp == 4) {
-    if (lane == 0) {
+    {
+      const bool elected = ptx::elect_one();
       auto load_weights = [&](int s, int kb) {
         uint64_t* bar = full + s;
         uint8_t* sa = smem + s * stage_bytes;
@@ -522,16 +531,16 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
       // The weights of the first stages may be read while the launch before this one still writes the tokens.
       int ahead = 0;
       if (p.early_weights)
-        for (; ahead < p.stages && kb0 + ahead < kb1; ++ahead) load_weights(ahead, kb0 + ahead);
+        for (; ahead < p.stages && kb0 + ahead < kb1; ++ahead)
+          if (elected) load_weights(ahead, kb0 + ahead);
       ptx::grid_wait_dependency();
       // Only now may the next launch start: what it reads early was written before this launch's predecessor ended.
       ptx::grid_launch_dependents();
       for (int kb = kb0; kb < kb1; ++kb) {
         const int i = kb - kb0, s = i % p.stages;
-        if (i >= ahead) {
-          if (!wt.wait(empty + s, ((i / p.stages) & 1) ^ 1, FDMOE_DENSE_TIMEOUT_EMPTY)) break;
-          load_weights(s, kb);
-        }
+        if (i >= ahead && !wt.wait_warp(empty + s, ((i / p.stages) & 1) ^ 1, FDMOE_DENSE_TIMEOUT_EMPTY)) break;
+        if (!elected) continue;
+        if (i >= ahead) load_weights(s, kb);
         uint8_t* sb = smem + s * stage_bytes + kParts * kStageOperand;
         ptx::tma_load_2d(sb, &p.b, full + s, kb * (MX4 ? 128 : 64), tok0);
         if (MX4) ptx::tma_load_2d(sb + nt * 128 + kParts * 2 * kScaleBlock, &p.sfb, full + s, 0,
@@ -539,16 +548,18 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
       }
     }
   } else if (warp == 5) {
-    if (lane == 0) {
+    {
+      const bool elected = ptx::elect_one();
       const uint32_t idesc = ptx::make_idesc_f16(128, nt, p.bf16, false, false);
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
         const int i = kb - kb0, s = i % p.stages;
-        if (!wt.wait(full + s, (i / p.stages) & 1, FDMOE_DENSE_TIMEOUT_FULL)) {
+        if (!wt.wait_warp(full + s, (i / p.stages) & 1, FDMOE_DENSE_TIMEOUT_FULL)) {
           ok = false;
           break;
         }
         ptx::tcgen05_fence_after();
+        if (!elected) continue;
         const uint32_t sa = ptx::smem_u32(smem + s * stage_bytes), sb = sa + kParts * kStageOperand;
         const uint64_t db = ptx::smem_desc_sw128(sb, 16);
         if (MX4) {
@@ -577,7 +588,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
         }
         ptx::umma_commit(empty + s);
       }
-      if (ok) ptx::umma_commit(&acc_full);
+      if (ok && elected) ptx::umma_commit(&acc_full);
     }
   } else {
     // ---- partial sums to shared memory, [token][part][row]: all MMAs have read the stages, which make room for them
