@@ -17,8 +17,8 @@ EXPORTED_SYMBOLS = [
     "FlashMoeGetUniqueId", "FlashMoeCreate", "FlashMoeLaunch", "FlashMoeLaunchHost",
     "FlashMoeDestroy", "FlashMoeGetLastStatus", "FlashMoeDebugRead", "FlashMoeTestTaskSystem",
     "FlashMoeTestQueueGemm", "FlashMoeTestStall", "FlashMoeErrorString", "FlashMoeLaunchNoAlloc",
-    "FlashMoeFfnWorkspaceBytes", "FlashMoeFfnForward", "FlashMoeFfnBackward", "FlashMoeMx4ScaleBytes",
-    "FlashMoeMx4Quantize", "FlashMoeMx4Dequantize", "FlashMoeMx4Matmul", "FlashMoeMx4FfnWorkspaceBytes",
+    "FlashMoeFfnWorkspaceBytes", "FlashMoeFfnSavedBytes", "FlashMoeFfnForward", "FlashMoeFfnBackward",
+    "FlashMoeMx4ScaleBytes", "FlashMoeMx4Quantize", "FlashMoeMx4Dequantize", "FlashMoeMx4Matmul", "FlashMoeMx4FfnWorkspaceBytes",
     "FlashMoeMx4FfnForward", "FlashMoeDenseStatus", "FlashMoeTestFfnStall",
 ]
 
@@ -71,6 +71,7 @@ def lib() -> C.CDLL:
     i64, size, ffn = C.c_int64, C.c_size_t, C.POINTER(FlashMoeFfnConfig)
     for name, restype, args in (
             ("FlashMoeFfnWorkspaceBytes", size, [ffn, i64, C.c_int]),
+            ("FlashMoeFfnSavedBytes", size, [ffn, i64]),
             ("FlashMoeFfnForward", C.c_int, [ffn] + [vp] * 6 + [size, i64, vp]),
             ("FlashMoeFfnBackward", C.c_int, [ffn] + [vp] * 9 + [size, i64, vp]),
             ("FlashMoeMx4ScaleBytes", size, [i64] * 3),

@@ -77,8 +77,42 @@ __device__ __forceinline__ void unpack2(uint32_t v, bool bf16, float& lo, float&
         : "r"(v));
   }
 }
-__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
-__device__ __forceinline__ float gate(float g, float u) { return g * sigmoid(g) * u; }
+// Two values at a time: the epilogues are bound by instruction issue, and one instruction multiplies or adds both.
+struct F2 {
+  unsigned long long v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ void get(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+};
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack2(F2 a, bool bf16) {
+  float lo, hi;
+  a.get(lo, hi);
+  return pack2(lo, hi, bf16);
+}
+__device__ __forceinline__ F2 as_f2(uint32_t lo, uint32_t hi) { return F2(__uint_as_float(lo), __uint_as_float(hi)); }
+// 1 / (1 + 2^(-g log2 e)); an exponential that overflows gives 0.
+__device__ __forceinline__ F2 sigmoid(F2 g) {
+  float lo, hi;
+  (g * F2(-1.44269504f, -1.44269504f)).get(lo, hi);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(lo));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(hi));
+  lo += 1.0f;
+  hi += 1.0f;
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(lo));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(hi));
+  return F2(lo, hi);
+}
+__device__ __forceinline__ F2 gate(F2 g, F2 u) { return g * sigmoid(g) * u; }
 
 // -------------------------------------------------------------- pair kernel
 // A pair of CTAs works on D[256 x tile_n] tiles: CTA r holds rows [128 r, 128 r + 128) of A, of D, and half of the
@@ -93,11 +127,14 @@ constexpr int kScaleBlock = 512;      // scales of 128 rows and 128 k
 
 template <bool MX4, int EPI>
 struct PairShape {
-  static constexpr bool kThree = EPI == FDMOE_EPI_GATED || EPI == FDMOE_EPI_GATED_GRAD;
-  static constexpr int kStages = MX4 || kThree ? 5 : 6;
+  // Results leave through shared memory in boxes of 32 rows of 128 bytes (boxes of half the width took twice the
+  // time: the copy engine works by rows), two per epilogue warp.  Fewer stages for more boxes did not pay: with four
+  // stages the 4096 x 6144 x 2048 gated product took 162 us instead of 149.
+  static constexpr int kBoxes = MX4 ? 1 : 2;
+  static constexpr int kStaging = kBoxes * 4096;
+  static constexpr int kStages = 5;
   static constexpr int kAccs = MX4 ? 1 : 2;  // 256 columns each; 4-bit operands' scales need columns too
   static constexpr int kScales = MX4 ? 6 * kScaleBlock : 0;  // per stage: A 2 blocks, B 4
-  static constexpr int kStaging = kThree && !MX4 ? 6144 : 4096;  // per epilogue warp
   static constexpr int kBarriers = 256;
   static constexpr int kSmem =
       kStages * (2 * kStageOperand + kScales) + 8 * kStaging + kBarriers + 1024;  // 1024: alignment of the base
@@ -113,25 +150,16 @@ __device__ __forceinline__ PairTile pair_tile(int tile, int tiles_m, int tiles_n
   return {g * 8 + r % rows, r / rows};
 }
 
-// Writes 32 columns of a row of 16-bit results (16 words) to a 32 x 32 staging tile in the 64-byte swizzle.
-__device__ __forceinline__ void stage_half(uint8_t* buf, int lane, const uint32_t (&w)[16]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
-        make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-}
-// The same for fp32, 128-byte swizzle.
-__device__ __forceinline__ void stage_f32(uint8_t* buf, int lane, const float (&v)[32]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+// Writes 16 bytes (chunk `j` of eight) of a row of a box of 32 rows of 128 bytes, in the 128-byte swizzle.
+__device__ __forceinline__ void stage16(uint8_t* box, int lane, int j, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(a, b, c, d);
 }
 
 template <bool MX4, int EPI>
 __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_constant__ FdmoePairParams p) {
   using S = PairShape<MX4, EPI>;
-  constexpr bool kGated = EPI == FDMOE_EPI_GATED || EPI == FDMOE_EPI_GATED_F32;
+  constexpr bool kGated = EPI == FDMOE_EPI_GATED || EPI == FDMOE_EPI_GATED_SAVE || EPI == FDMOE_EPI_GATED_F32;
+  constexpr bool kF32 = EPI == FDMOE_EPI_F32 || EPI == FDMOE_EPI_GATED_F32;
   constexpr int kAccCols = 256;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
@@ -142,7 +170,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
   uint64_t* empty = full + S::kStages;
   uint64_t* acc_full = empty + S::kStages;
   uint64_t* acc_empty = acc_full + S::kAccs;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + S::kAccs);
+  uint64_t* gu_full = acc_empty + S::kAccs;  // gradient: one per epilogue warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gu_full + 8);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -162,6 +191,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       ptx::mbar_init(acc_full + a, 1);
       ptx::mbar_init(acc_empty + a, 16);  // eight epilogue warps of each CTA
     }
+    for (int w = 0; w < 8; ++w) ptx::mbar_init(gu_full + w, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
@@ -171,7 +201,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
   }
   ptx::tcgen05_fence_before();
   __syncthreads();
-  ptx::cluster_sync();  // both CTAs' barriers are set up
+  ptx::cluster_sync_relaxed();  // all CTAs' barriers are set up
   ptx::tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
   ptx::grid_wait_dependency();  // nothing of global memory is touched before this
@@ -184,6 +214,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     // ---- loads: both CTAs fill their own stages; the bytes are counted on the even CTA's barriers
     {
       const bool elected = ptx::elect_one();
+      // rows along N come in boxes of 64, the second of which may be used in part
+      const uint32_t b_bytes = p.b_mn && half_n > 64 ? kStageOperand : half_n * 128;
       uint32_t it = 0;
       bool ok = true;
       for (int tile = first; ok && tile < tiles; tile += step) {
@@ -198,7 +230,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
             break;
           }
           if (p.stall || !elected) continue;
-          if (rank == 0) ptx::mbar_expect_tx(full + s, 2 * (kStageOperand + half_n * 128 + S::kScales));
+          if (rank == 0) ptx::mbar_expect_tx(full + s, 2 * (kStageOperand + b_bytes + S::kScales));
           const uint32_t bar = ptx::map_rank(ptx::smem_u32(full + s), leader);
           const uint32_t sa = ptx::smem_u32(stages + s * 2 * kStageOperand), sb = sa + kStageOperand;
           if (MX4) {
@@ -281,14 +313,32 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     }
   } else if (warp >= 4) {
     // ---- epilogue: warps w and w + 4 read the same 32 lanes and take turns with the columns, 32 at a time
+    const bool elected = ptx::elect_one();
     const int w = warp - 4, quad = warp & 3, half = w >> 2;
     uint8_t* buf = staging + w * S::kStaging;
     const uint32_t sbuf = ptx::smem_u32(buf);
-    const int tile_cols = kGated ? half_n : p.tile_n, chunks = tile_cols >> 5;
+    const int tile_cols = kGated ? half_n : p.tile_n;
+    // This warp's groups of columns, a box wide: the first, and the distance to the next (of all pairs' and halves').
+    constexpr int kGroup = kF32 ? 32 : 64;
+    constexpr int kMost = (kGated ? 128 : 256) / kGroup / 2;  // groups of a warp
+    const int groups = tile_cols / kGroup, first_group = half * split + (int)part, group_step = 2 * split;
+    // Gradient: the boxes first take g and u of a group of columns, which dg and du then replace.
+    uint32_t gu_count = 0;
+    auto fetch_gu = [&](const PairTile& t, int c) {
+      if (elected) {
+        ptx::bulk_wait_group_read0();
+        ptx::mbar_expect_tx(gu_full + w, 8192);
+        const int x = t.n * tile_cols + c * 64, y = t.m * 256 + (int)rank * 128 + quad * 32;
+        ptx::tma_load_2d(buf, &p.gu[0], gu_full + w, x, y);
+        ptx::tma_load_2d(buf + 4096, &p.gu[1], gu_full + w, x, y);
+      }
+    };
     uint32_t n = 0;
     for (int tile = first; tile < tiles; tile += step, ++n) {
       const PairTile t = pair_tile(tile, p.tiles_m, p.tiles_n);
       const int acc = n % S::kAccs;
+      if constexpr (EPI == FDMOE_EPI_GATED_GRAD)
+        if (first_group < groups) fetch_gu(t, first_group);
       const bool done = wt.wait(acc_full + acc, (n / S::kAccs) & 1, FDMOE_DENSE_TIMEOUT_DONE);
       ptx::tcgen05_fence_after();
       const uint32_t d = tmem + acc * kAccCols + (uint32_t(quad * 32) << 16);
@@ -329,150 +379,218 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
           }
         }
       };
-      int used = 0;  // staging buffers written
-#pragma unroll 1
-      for (int c = half * split + (int)part; c < chunks; c += 2 * split, ++used) {
-        const int in = c * 32;                        // column in the tile
-        const int col = t.n * tile_cols + in;         // column of the result
-        uint32_t v[32];
-        load(in, v);
-        if constexpr (kGated) {
-          uint32_t u[32];
-          load(half_n + in, u);
+      auto release = [&]() {  // this warp has read its part of the accumulator
+        ptx::tcgen05_fence_before();
+        __syncwarp();
+        if (elected) ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(acc_empty + acc), leader));
+      };
+      // Waits until this warp's boxes may be written again (its last stores have read them).
+      auto boxes_free = [&]() {
+        if (elected) ptx::bulk_wait_group_read0();
+        __syncwarp();
+      };
+      auto boxes_written = [&]() {
+        ptx::fence_proxy_async_shared();
+        __syncwarp();
+      };
+      const int col0 = t.n * tile_cols;
+      // Sends box b, which all lanes have written, to columns from `col` on of result `map`.
+      auto send = [&](int map, int b, int col) {
+        if (elected && row0 < p.rows && col < p.cols) ptx::tma_store_2d(&p.out[map], sbuf + b * 4096, col, row0);
+      };
+      if constexpr (EPI == FDMOE_EPI_HALF) {
+        // All of the warp's columns are read, rounded and the accumulator given back before the first is stored.
+        uint32_t w[kMost][32];
+#pragma unroll
+        for (int j = 0; j < kMost; ++j) {
+          const int c = first_group + j * group_step;
+          if (c >= groups) break;
+          uint32_t v[2][32];
+          load(c * 64, v[0]);
+          load(c * 64 + 32, v[1]);
           ptx::tmem_ld_wait();
-          if constexpr (EPI == FDMOE_EPI_GATED_F32) {
-            float h[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) h[i] = gate(__uint_as_float(v[i]), __uint_as_float(u[i]));
-            if (lane == 0) ptx::bulk_wait_group_read0();
-            __syncwarp();
-            stage_f32(buf, lane, h);
-            ptx::fence_proxy_async_shared();
-            __syncwarp();
-            if (lane == 0 && row0 < p.rows && col < p.cols) ptx::tma_store_2d(&p.out[0], sbuf, col, row0);
-          } else {
-            uint32_t h[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              h[i] = pack2(gate(__uint_as_float(v[2 * i]), __uint_as_float(u[2 * i])),
-                           gate(__uint_as_float(v[2 * i + 1]), __uint_as_float(u[2 * i + 1])), p.bf16);
-            if (!MX4 && p.save_gu) {
-              // kept for the backward pass, rounded like every other activation
-              if (lane == 0) ptx::bulk_wait_group_read0();
-              __syncwarp();
-              stage_half(buf, lane, h);
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                h[i] = pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), p.bf16);
-              stage_half(buf + 2048, lane, h);
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                h[i] = pack2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]), p.bf16);
-              stage_half(buf + 4096, lane, h);
-              ptx::fence_proxy_async_shared();
-              __syncwarp();
-              if (lane == 0 && row0 < p.rows && col < p.cols) {
-                ptx::tma_store_2d(&p.out[0], sbuf, col, row0);
-                ptx::tma_store_2d(&p.out[1], sbuf + 2048, col, row0);
-                ptx::tma_store_2d(&p.out[2], sbuf + 4096, col, row0);
-              }
-            } else {
-              if (lane == 0) ptx::bulk_wait_group_read1();
-              __syncwarp();
-              stage_half(buf + (used & 1) * 2048, lane, h);
-              ptx::fence_proxy_async_shared();
-              __syncwarp();
-              if (lane == 0 && row0 < p.rows && col < p.cols)
-                ptx::tma_store_2d(&p.out[0], sbuf + (used & 1) * 2048, col, row0);
-            }
-          }
-        } else if constexpr (EPI == FDMOE_EPI_GATED_GRAD) {
-          // g and u of this row's 32 columns; columns come in eights because every row starts on 16 bytes
-          uint4 gw[4], uw[4];
-          const int row = row0 + lane;
-          const uint8_t* g0 = static_cast<const uint8_t*>(p.gu) + ((int64_t)row * 2 * p.cols + col) * 2;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const bool in_range = row < p.rows && col + 8 * j < p.cols;
-            gw[j] = in_range ? __ldg(reinterpret_cast<const uint4*>(g0) + j) : make_uint4(0, 0, 0, 0);
-            uw[j] = in_range ? __ldg(reinterpret_cast<const uint4*>(g0 + (int64_t)p.cols * 2) + j) : make_uint4(0, 0, 0, 0);
-          }
-          ptx::tmem_ld_wait();
-          uint32_t dg[16], du[16], h[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint32_t gp = reinterpret_cast<const uint32_t*>(gw)[i], up = reinterpret_cast<const uint32_t*>(uw)[i];
-            float g[2], u[2], a[2], b[2], e[2];
-            unpack2(gp, p.bf16, g[0], g[1]);
-            unpack2(up, p.bf16, u[0], u[1]);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const float dh = __uint_as_float(v[2 * i + q]), s = sigmoid(g[q]), silu = g[q] * s;
-              a[q] = dh * u[q] * s * (1.0f + g[q] * (1.0f - s));
-              b[q] = dh * silu;
-              e[q] = silu * u[q];
-            }
-            dg[i] = pack2(a[0], a[1], p.bf16);
-            du[i] = pack2(b[0], b[1], p.bf16);
-            h[i] = pack2(e[0], e[1], p.bf16);
-          }
-          if (lane == 0) ptx::bulk_wait_group_read0();
-          __syncwarp();
-          stage_half(buf, lane, dg);
-          stage_half(buf + 2048, lane, du);
-          stage_half(buf + 4096, lane, h);
-          ptx::fence_proxy_async_shared();
-          __syncwarp();
-          if (lane == 0 && row0 < p.rows && col < p.cols) {
-            ptx::tma_store_2d(&p.out[0], sbuf, col, row0);
-            ptx::tma_store_2d(&p.out[1], sbuf + 2048, col, row0);
-            ptx::tma_store_2d(&p.out[2], sbuf + 4096, col, row0);
-          }
-        } else if constexpr (EPI == FDMOE_EPI_F32) {
-          ptx::tmem_ld_wait();
-          float f[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
-          if (lane == 0) ptx::bulk_wait_group_read0();
-          __syncwarp();
-          stage_f32(buf, lane, f);
-          ptx::fence_proxy_async_shared();
-          __syncwarp();
-          if (lane == 0 && row0 < p.rows && col < p.cols) ptx::tma_store_2d(&p.out[0], sbuf, col, row0);
-        } else {
-          ptx::tmem_ld_wait();
-          uint32_t h[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) h[i] = pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), p.bf16);
-          if (lane == 0) ptx::bulk_wait_group_read1();
-          __syncwarp();
-          stage_half(buf + (used & 1) * 2048, lane, h);
-          ptx::fence_proxy_async_shared();
-          __syncwarp();
-          if (lane == 0 && row0 < p.rows && col < p.cols)
-            ptx::tma_store_2d(&p.out[0], sbuf + (used & 1) * 2048, col, row0);
+          for (int i = 0; i < 32; ++i) w[j][i] = pack2(as_f2(v[i >> 4][(2 * i) & 31], v[i >> 4][(2 * i + 1) & 31]), p.bf16);
         }
-        if (lane == 0) ptx::bulk_commit_group();
+        release();
+        if constexpr (S::kBoxes >= kMost) boxes_free();
+#pragma unroll
+        for (int j = 0; j < kMost; ++j) {
+          const int c = first_group + j * group_step, b = S::kBoxes >= kMost ? j : 0;
+          if (c >= groups) break;
+          if constexpr (S::kBoxes < kMost) boxes_free();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) stage16(buf + b * 4096, lane, i, w[j][4 * i], w[j][4 * i + 1], w[j][4 * i + 2], w[j][4 * i + 3]);
+          boxes_written();
+          send(0, b, col0 + c * 64);
+          if (elected) ptx::bulk_commit_group();
+        }
+      } else if constexpr (EPI == FDMOE_EPI_F32) {
+        uint32_t v[kMost][32];
+#pragma unroll
+        for (int j = 0; j < kMost; ++j)
+          if (first_group + j * group_step < groups) load((first_group + j * group_step) * 32, v[j]);
+        ptx::tmem_ld_wait();
+        release();
+#pragma unroll
+        for (int j = 0; j < kMost; ++j) {
+          const int c = first_group + j * group_step;
+          if (c >= groups) break;
+          boxes_free();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) stage16(buf, lane, i, v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3]);
+          boxes_written();
+          send(0, 0, col0 + c * 32);
+          if (elected) ptx::bulk_commit_group();
+        }
+      } else if constexpr (EPI == FDMOE_EPI_GATED_F32) {
+        uint32_t g[kMost][32], u[kMost][32];
+#pragma unroll
+        for (int j = 0; j < kMost; ++j)
+          if (first_group + j * group_step < groups) {
+            load((first_group + j * group_step) * 32, g[j]);
+            load(half_n + (first_group + j * group_step) * 32, u[j]);
+          }
+        ptx::tmem_ld_wait();
+        release();
+#pragma unroll
+        for (int j = 0; j < kMost; ++j) {
+          const int c = first_group + j * group_step;
+          if (c >= groups) break;
+          boxes_free();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float y[4];
+            gate(as_f2(g[j][4 * i], g[j][4 * i + 1]), as_f2(u[j][4 * i], u[j][4 * i + 1])).get(y[0], y[1]);
+            gate(as_f2(g[j][4 * i + 2], g[j][4 * i + 3]), as_f2(u[j][4 * i + 2], u[j][4 * i + 3])).get(y[2], y[3]);
+            stage16(buf, lane, i, __float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+          }
+          boxes_written();
+          send(0, 0, col0 + c * 32);
+          if (elected) ptx::bulk_commit_group();
+        }
+      } else if constexpr (kGated) {
+        // One group of 64 columns, 32 at a time; 4-bit operands have one accumulator, which is given back before the
+        // activation is computed.
+        const int c = first_group;
+        uint32_t g[MX4 ? 2 : 1][32], u[MX4 ? 2 : 1][32];
+        if (MX4 && c < groups) {
+#pragma unroll
+          for (int i = 0; i < (MX4 ? 2 : 1); ++i) {
+            load(c * 64 + i * 32, g[i]);
+            load(half_n + c * 64 + i * 32, u[i]);
+          }
+        }
+        if constexpr (MX4) {
+          ptx::tmem_ld_wait();
+          release();
+        }
+        if (c < groups) {
+          boxes_free();
+          uint32_t up[EPI == FDMOE_EPI_GATED_SAVE ? 32 : 1];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t(&gi)[32] = g[MX4 ? i : 0];
+            uint32_t(&ui)[32] = u[MX4 ? i : 0];
+            if constexpr (!MX4) {
+              load(c * 64 + i * 32, gi);
+              load(half_n + c * 64 + i * 32, ui);
+              ptx::tmem_ld_wait();
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // eight columns
+              uint32_t h[4], gw[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const int at = 8 * j + 2 * q;
+                h[q] = pack2(gate(as_f2(gi[at], gi[at + 1]), as_f2(ui[at], ui[at + 1])), p.bf16);
+                if constexpr (EPI == FDMOE_EPI_GATED_SAVE) {
+                  // kept for the backward pass, rounded like every other activation
+                  gw[q] = pack2(as_f2(gi[at], gi[at + 1]), p.bf16);
+                  up[16 * i + 4 * j + q] = pack2(as_f2(ui[at], ui[at + 1]), p.bf16);
+                }
+              }
+              stage16(buf, lane, i * 4 + j, h[0], h[1], h[2], h[3]);
+              if constexpr (EPI == FDMOE_EPI_GATED_SAVE) stage16(buf + 4096, lane, i * 4 + j, gw[0], gw[1], gw[2], gw[3]);
+            }
+          }
+          if constexpr (!MX4) release();
+          boxes_written();
+          send(0, 0, col0 + c * 64);
+          if constexpr (EPI == FDMOE_EPI_GATED_SAVE) {
+            if (elected) ptx::bulk_commit_group();
+            send(1, 1, col0 + c * 64);
+            if (elected) {
+              ptx::bulk_commit_group();
+              ptx::bulk_wait_group_read1();  // h has left
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) stage16(buf, lane, i, up[4 * i], up[4 * i + 1], up[4 * i + 2], up[4 * i + 3]);
+            boxes_written();
+            send(2, 0, col0 + c * 64);
+          }
+          if (elected) ptx::bulk_commit_group();
+        } else if constexpr (!MX4) {
+          release();
+        }
+      } else {
+#pragma unroll 1
+        for (int c = first_group; c < groups; c += group_step) {
+          if (c != first_group) fetch_gu(t, c);
+          wt.wait_warp(gu_full + w, gu_count++ & 1, FDMOE_DENSE_TIMEOUT_FULL);
+#pragma unroll 1
+          for (int i = 0; i < 2; ++i) {
+            uint32_t v[32];
+            load(c * 64 + i * 32, v);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // eight columns
+              uint4* const g_at = reinterpret_cast<uint4*>(buf + lane * 128 + (((i * 4 + j) ^ (lane & 7)) << 4));
+              uint4* const u_at = g_at + 4096 / 16;
+              const uint4 g4 = *g_at, u4 = *u_at;
+              const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
+              uint32_t dg[4], du[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                float a, b;
+                unpack2(gw[q], p.bf16, a, b);
+                const F2 g(a, b);
+                unpack2(uw[q], p.bf16, a, b);
+                const F2 u(a, b), dh = as_f2(v[8 * j + 2 * q], v[8 * j + 2 * q + 1]);
+                const F2 sg = sigmoid(g), silu = g * sg;
+                // silu' = s + g s (1 - s)
+                const F2 slope = fma2(silu, fma2(sg, F2(-1.0f, -1.0f), F2(1.0f, 1.0f)), sg);
+                dg[q] = pack2(dh * u * slope, p.bf16);
+                du[q] = pack2(dh * silu, p.bf16);
+              }
+              *g_at = make_uint4(dg[0], dg[1], dg[2], dg[3]);
+              *u_at = make_uint4(du[0], du[1], du[2], du[3]);
+            }
+          }
+          boxes_written();
+          send(0, 0, col0 + c * 64);
+          send(1, 1, col0 + c * 64);
+          if (elected) ptx::bulk_commit_group();
+        }
+        release();
       }
-      ptx::tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_rank(ptx::smem_u32(acc_empty + acc), leader));
     }
-    if (lane == 0) ptx::bulk_wait_group0();
+    if (elected) ptx::bulk_wait_group_read0();  // the boxes stay until they have been read
   }
   __syncwarp();
   if (warp < 4 && split > 1) ptx::cluster_sync();  // the epilogue warps' exchange of partial sums
   ptx::tcgen05_fence_before();
   __syncthreads();
   wt.drain();
-  ptx::cluster_sync();  // neither CTA leaves while the other may still read its operands or arrive on its barriers
+  ptx::cluster_sync_relaxed();  // neither CTA leaves while the other may still read its operands or arrive on its barriers
   ptx::tcgen05_fence_after();
   if (warp == 2) ptx::tmem_dealloc_pair(tmem, 512);
 }
 
 // ------------------------------------------------------------ stream kernel
 // One CTA: D[128 weight rows x tile_tokens] (gated: two such accumulators, gate and up) over its part of the k axis.
-// The cluster's partial sums meet in shared memory: CTA r adds those of tokens r, r + split, ... over all CTAs.
+// The cluster's partial sums meet in shared memory: CTA r adds those of every split-th group of four tokens.
 constexpr int kStreamThreads = 192;  // 4 epilogue warps, loads, MMAs
 
 template <bool MX4, int EPI>
@@ -591,60 +709,116 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
       if (ok && elected) ptx::umma_commit(&acc_full);
     }
   } else {
-    // ---- partial sums to shared memory, [token][part][row]: all MMAs have read the stages, which make room for them
-    if (wt.wait(&acc_full, 0, FDMOE_DENSE_TIMEOUT_DONE)) {
-      ptx::tcgen05_fence_after();
-      const int count = min(nt, p.tokens - tok0);
-      float* part = reinterpret_cast<float*>(smem);
-      const uint32_t d = tmem + (uint32_t(warp * 32) << 16);
+    const int count = min(nt, p.tokens - tok0);
+    const bool done = wt.wait(&acc_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
+    ptx::tcgen05_fence_after();
+    const uint32_t d = tmem + (uint32_t(warp * 32) << 16);
+    const int row = row0 + warp * 32 + lane;
+    // Four tokens' results of this row (of each part).  Neighbouring lanes exchange two, so that each stores two rows
+    // of two tokens.
+    constexpr bool kF32 = EPI == FDMOE_EPI_F32 || EPI == FDMOE_EPI_GATED_F32;
+    const bool even_ld = (p.ld & 1) == 0;
+    auto finish = [&](int t, const float(&v)[kParts][4]) {
+      float y[4];
 #pragma unroll
-      for (int q = 0; q < kParts; ++q)
+      for (int i = 0; i < 4; i += 2) {
+        if constexpr (kGated)
+          gate(F2(v[0][i], v[0][i + 1]), F2(v[1][i], v[1][i + 1])).get(y[i], y[i + 1]);
+        else
+          y[i] = v[0][i], y[i + 1] = v[0][i + 1];
+      }
+      const int64_t at = (int64_t)(tok0 + t) * p.ld;
+      if constexpr (kF32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (t + i < count && row < p.rows) static_cast<float*>(p.out)[at + i * p.ld + row] = y[i];
+      } else {
+        uint16_t* out = static_cast<uint16_t*>(p.out);
+        const bool odd = lane & 1;
+        const float a = __shfl_xor_sync(0xffffffffu, odd ? y[0] : y[2], 1), b = __shfl_xor_sync(0xffffffffu, odd ? y[1] : y[3], 1);
+        const uint32_t w0 = odd ? pack2(a, y[2], p.bf16) : pack2(y[0], a, p.bf16);
+        const uint32_t w1 = odd ? pack2(b, y[3], p.bf16) : pack2(y[1], b, p.bf16);
+        const int r = row & ~1, i0 = odd ? 2 : 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (t + i0 + i >= count) break;
+          const uint32_t w = i ? w1 : w0;
+          uint16_t* o = out + at + (i0 + i) * p.ld + r;
+          if (even_ld && r + 1 < p.rows) {
+            *reinterpret_cast<uint32_t*>(o) = w;
+          } else {
+            if (r < p.rows) o[0] = static_cast<uint16_t>(w);
+            if (r + 1 < p.rows) o[1] = static_cast<uint16_t>(w >> 16);
+          }
+        }
+      }
+    };
+    if (p.split == 1) {
+      if (done)
         for (int c = 0; c < count; c += 16) {
-          uint32_t v[16];
-          ptx::tmem_ld_32x16(d + q * nt + c, v);
+          uint32_t v[kParts][16];
+#pragma unroll
+          for (int q = 0; q < kParts; ++q) ptx::tmem_ld_32x16(d + q * nt + c, v[q]);
           ptx::tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (c + i < count) part[((c + i) * kParts + q) * 128 + warp * 32 + lane] = __uint_as_float(v[i]);
+          for (int i = 0; i < 16; i += 4) {
+            float f[kParts][4];
+#pragma unroll
+            for (int q = 0; q < kParts; ++q)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) f[q][j] = __uint_as_float(v[q][i + j]);
+            if (c + i < count) finish(c + i, f);
+          }
         }
+    } else {
+      // Groups of four tokens are dealt out to the CTAs of the cluster.  Each CTA stores its partial sums of a group
+      // into the owner's shared memory, [group of the owner][CTA][part][row][4 tokens], where the stages were: every
+      // CTA's MMAs have read theirs once all have arrived at the first barrier.
+      ptx::cluster_sync();
+      const uint32_t mine = ptx::smem_u32(smem) + (warp * 32 + lane) * 16;
+      if (done)
+        for (int c = 0; c < count; c += 16) {
+          uint32_t v[kParts][16];
+#pragma unroll
+          for (int q = 0; q < kParts; ++q) ptx::tmem_ld_32x16(d + q * nt + c, v[q]);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const int group = (c + i) >> 2, owner = group % p.split, slot = group / p.split;
+            if (c + i < count) {
+              const uint32_t to = ptx::map_rank(mine + (slot * p.split + rank) * kParts * 2048, owner);
+#pragma unroll
+              for (int q = 0; q < kParts; ++q)
+                ptx::st_cluster_u32x4(to + q * 2048, v[q][i], v[q][i + 1], v[q][i + 2], v[q][i + 3]);
+            }
+          }
+        }
+      ptx::cluster_sync();
+      const uint8_t* own = smem + (warp * 32 + lane) * 16;
+      for (int slot = 0, group = rank; group * 4 < count; ++slot, group += p.split) {
+        float f[kParts][4] = {};
+#pragma unroll 4
+        for (int r = 0; r < p.split; ++r)
+#pragma unroll
+          for (int q = 0; q < kParts; ++q) {
+            const float4 v = *reinterpret_cast<const float4*>(own + ((slot * p.split + r) * kParts + q) * 2048);
+            f[q][0] += v.x;
+            f[q][1] += v.y;
+            f[q][2] += v.z;
+            f[q][3] += v.w;
+          }
+        finish(group * 4, f);
+      }
     }
   }
   __syncwarp();
-  ptx::tcgen05_fence_before();
-  ptx::cluster_sync();
-  if (warp < 4 && !abort_flag) {
-    const int row = row0 + warp * 32 + lane;
-    const int count = min(nt, p.tokens - tok0);
-    const uint32_t base = ptx::smem_u32(smem) + (warp * 32 + lane) * 4;
-    for (int t = rank; t < count; t += p.split) {
-      float sum[kParts];
-#pragma unroll
-      for (int q = 0; q < kParts; ++q) {
-        float v[FDMOE_STREAM_SPLIT];
-#pragma unroll
-        for (int r = 0; r < FDMOE_STREAM_SPLIT; ++r)
-          if (r < p.split) v[r] = ptx::ld_cluster_f32(ptx::map_rank(base + (t * kParts + q) * 512, r));
-        sum[q] = v[0];
-#pragma unroll
-        for (int r = 1; r < FDMOE_STREAM_SPLIT; ++r)
-          if (r < p.split) sum[q] += v[r];
-      }
-      float y;
-      if constexpr (kGated)
-        y = gate(sum[0], sum[1]);
-      else
-        y = sum[0];
-      if (row < p.rows) {
-        const int64_t at = (int64_t)(tok0 + t) * p.ld + row;
-        if constexpr (EPI == FDMOE_EPI_F32 || EPI == FDMOE_EPI_GATED_F32)
-          static_cast<float*>(p.out)[at] = y;
-        else
-          static_cast<uint16_t*>(p.out)[at] = static_cast<uint16_t>(pack2(y, 0.0f, p.bf16));
-      }
-    }
+  if (warp >= 4 && p.split > 1) {
+    ptx::cluster_sync();
+    ptx::cluster_sync();
   }
+  ptx::tcgen05_fence_before();
+  __syncthreads();
   wt.drain();
-  ptx::cluster_sync();  // a CTA's partial sums stay until every other has read them
   ptx::tcgen05_fence_after();
   if (warp == 4) ptx::tmem_dealloc(tmem, p.tmem_cols);
 }

@@ -12,25 +12,32 @@ extern "C" int fdmoe_pair_launch(const FdmoePairParams* p, int epi, int mx4, int
   switch (epi) {
     case FDMOE_EPI_HALF: return launch_pair<false, FDMOE_EPI_HALF>(*p, clusters, s);
     case FDMOE_EPI_GATED: return launch_pair<false, FDMOE_EPI_GATED>(*p, clusters, s);
+    case FDMOE_EPI_GATED_SAVE: return launch_pair<false, FDMOE_EPI_GATED_SAVE>(*p, clusters, s);
     case FDMOE_EPI_GATED_GRAD: return launch_pair<false, FDMOE_EPI_GATED_GRAD>(*p, clusters, s);
   }
   return cudaErrorInvalidValue;
 }
 
-// All instances of a kernel have the same threads and nearly the same shared memory, so one stands for all.
-extern "C" int fdmoe_pair_clusters(int size, int* out) {
-  constexpr int smem = PairShape<false, FDMOE_EPI_HALF>::kSmem;
-  const cudaError_t e = cudaFuncSetAttribute(pair_gemm<false, FDMOE_EPI_HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+// What the device holds at once is asked for kernels that do nothing and have the shape of the real ones, whose use
+// of TMEM the occupancy calculator takes for all of an SM's.
+namespace {
+__global__ void __launch_bounds__(kPairThreads) pair_shape() {}
+__global__ void __launch_bounds__(kStreamThreads) stream_shape() { __shared__ volatile uint8_t barriers[256]; barriers[0] = 0; }
+
+template <typename F>
+int count_clusters(F kernel, int threads, int smem, int size, int* out) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const LaunchConfig l(dim3(size), kPairThreads, smem, size, nullptr);
-  return cudaOccupancyMaxActiveClusters(out, pair_gemm<false, FDMOE_EPI_HALF>, &l.cfg);
+  const LaunchConfig l(dim3(size), threads, smem, size, nullptr);
+  return cudaOccupancyMaxActiveClusters(out, kernel, &l.cfg);
+}
+}  // namespace
+
+extern "C" int fdmoe_pair_clusters(int size, int* out) {
+  return count_clusters(pair_shape, kPairThreads, PairShape<false, FDMOE_EPI_HALF>::kSmem, size, out);
 }
 extern "C" int fdmoe_stream_clusters(int size, int smem, int* out) {
-  const cudaError_t e = cudaFuncSetAttribute(stream_gemm<false, FDMOE_EPI_GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             kStreamSmemMax);
-  if (e != cudaSuccess) return e;
-  const LaunchConfig l(dim3(size), kStreamThreads, smem, size, nullptr);
-  return cudaOccupancyMaxActiveClusters(out, stream_gemm<false, FDMOE_EPI_GATED>, &l.cfg);
+  return count_clusters(stream_shape, kStreamThreads, smem, size, out);
 }
 
 extern "C" int fdmoe_stream_launch(const FdmoeStreamParams* p, int epi, int mx4, int smem, void* stream) {

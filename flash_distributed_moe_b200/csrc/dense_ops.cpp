@@ -169,7 +169,7 @@ int PairProduct(const Call& c, const Operand& a, const Operand& b, void* out, bo
   const int clusters = PairShape(p, c, rows, cols, k, false, false);
   DENSE_TRY(OperandMap(c, &p.a, a, 128));
   DENSE_TRY(OperandMap(c, &p.b, b, p.tile_n / 2));
-  DENSE_TRY(MakeMap(c, &p.out[0], out, 2, rows, cols, cols * 2, 32, 32));
+  DENSE_TRY(MakeMap(c, &p.out[0], out, 2, rows, cols, cols * 2, 64, 32));
   p.a_mn = a.mn;
   p.b_mn = b.mn;
   p.bf16 = bf16;
@@ -210,31 +210,30 @@ int GatedProduct(const Call& c, const void* x, const void* w13, void* h, void* g
   const int clusters = PairShape(p, c, T, I, H, true, false);
   DENSE_TRY(MakeMap(c, &p.a, x, 2, T, H, H * 2, 64, 128));
   DENSE_TRY(MakeMap(c, &p.b, w13, 2, 2 * I, H, H * 2, 64, p.tile_n / 2));
-  DENSE_TRY(MakeMap(c, &p.out[0], h, 2, T, I, I * 2, 32, 32));
+  DENSE_TRY(MakeMap(c, &p.out[0], h, 2, T, I, I * 2, 64, 32));
   if (gu) {
     // two matrices side by side: what a tile has beyond column I of the gate projection is not stored
-    DENSE_TRY(MakeMap(c, &p.out[1], gu, 2, T, I, I * 4, 32, 32));
-    DENSE_TRY(MakeMap(c, &p.out[2], static_cast<uint8_t*>(gu) + I * 2, 2, T, I, I * 4, 32, 32));
+    DENSE_TRY(MakeMap(c, &p.out[1], gu, 2, T, I, I * 4, 64, 32));
+    DENSE_TRY(MakeMap(c, &p.out[2], static_cast<uint8_t*>(gu) + I * 2, 2, T, I, I * 4, 64, 32));
   }
   p.up_row = (int32_t)I;
   p.bf16 = bf16;
-  p.save_gu = gu != nullptr;
   p.stall = stall;
-  return fdmoe_pair_launch(&p, FDMOE_EPI_GATED, 0, clusters, c.stream);
+  return fdmoe_pair_launch(&p, gu ? FDMOE_EPI_GATED_SAVE : FDMOE_EPI_GATED, 0, clusters, c.stream);
 }
 
-// From dy: dgu [T, 2I] and h [T, I].
-int GatedGradient(const Call& c, const void* dy, const void* w2, const void* gu, void* dgu, void* h, int64_t T, int64_t H,
-                  int64_t I, bool bf16) {
+// From dy: dgu [T, 2I].
+int GatedGradient(const Call& c, const void* dy, const void* w2, const void* gu, void* dgu, int64_t T, int64_t H, int64_t I,
+                  bool bf16) {
   FdmoePairParams p;
   memset(&p, 0, sizeof(p));
   const int clusters = PairShape(p, c, T, I, H, false, false);
   DENSE_TRY(MakeMap(c, &p.a, dy, 2, T, H, H * 2, 64, 128));
   DENSE_TRY(MakeMap(c, &p.b, w2, 2, H, I, I * 2, 64, 64));
-  DENSE_TRY(MakeMap(c, &p.out[0], dgu, 2, T, I, I * 4, 32, 32));
-  DENSE_TRY(MakeMap(c, &p.out[1], static_cast<uint8_t*>(dgu) + I * 2, 2, T, I, I * 4, 32, 32));
-  DENSE_TRY(MakeMap(c, &p.out[2], h, 2, T, I, I * 2, 32, 32));
-  p.gu = gu;
+  for (int i = 0; i < 2; ++i) {
+    DENSE_TRY(MakeMap(c, &p.gu[i], static_cast<const uint8_t*>(gu) + i * I * 2, 2, T, I, I * 4, 64, 32));
+    DENSE_TRY(MakeMap(c, &p.out[i], static_cast<uint8_t*>(dgu) + i * I * 2, 2, T, I, I * 4, 64, 32));
+  }
   p.b_mn = 1;
   p.bf16 = bf16;
   return fdmoe_pair_launch(&p, FDMOE_EPI_GATED_GRAD, 0, clusters, c.stream);
@@ -291,7 +290,7 @@ int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, 
   DENSE_TRY(Mx4Maps(c, &p.a, &p.sfa, a, k, 128));
   DENSE_TRY(Mx4Maps(c, &p.b, &p.sfb, b, k, 128));
   const int size = dtype == kF32 ? 4 : 2;
-  DENSE_TRY(MakeMap(c, &p.out[0], out, size, tokens, rows, rows * size, 32, 32));
+  DENSE_TRY(MakeMap(c, &p.out[0], out, size, tokens, rows, rows * size, 128 / size, 32));
   p.up_row = (int32_t)rows;
   p.sf_chunks = chunks;
   p.sf_up_block = up_block;
@@ -336,35 +335,45 @@ extern "C" int FlashMoeDenseStatus(uint32_t* code, int reset) {
   return 0;
 }
 
+// Scratch of a forward call: h, unless it is kept; of a backward call: the gradients of the projections.
 extern "C" size_t FlashMoeFfnWorkspaceBytes(const FlashMoeFfnConfig* cfg, int64_t tokensNum, int backward) {
   if (CheckFfn(cfg, tokensNum) != 0) return 0;
-  const size_t h = fdmoe::AlignBytes((size_t)tokensNum * cfg->intermediateSize * 2);
-  return backward ? h + fdmoe::AlignBytes((size_t)tokensNum * cfg->intermediateSize * 4) : h;
+  return fdmoe::AlignBytes((size_t)tokensNum * cfg->intermediateSize * (backward ? 4 : 2));
 }
 
-static int FfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y, void* gateUp,
+// What a forward call keeps for the backward pass: the projections [T, 2I], then h [T, I].
+static size_t SavedOffset(const FlashMoeFfnConfig* cfg, int64_t T) {
+  return fdmoe::AlignBytes((size_t)T * cfg->intermediateSize * 4);
+}
+extern "C" size_t FlashMoeFfnSavedBytes(const FlashMoeFfnConfig* cfg, int64_t tokensNum) {
+  if (CheckFfn(cfg, tokensNum) != 0) return 0;
+  return SavedOffset(cfg, tokensNum) + fdmoe::AlignBytes((size_t)tokensNum * cfg->intermediateSize * 2);
+}
+
+static int FfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y, void* saved,
                       void* workspace, size_t workspaceBytes, int64_t T, void* stream, bool stall) {
   DENSE_TRY(CheckFfn(cfg, T));
   if (T == 0) return 0;
-  if (!x || !w13 || !w2 || !y || !workspace || !Aligned(x) || !Aligned(w13) || !Aligned(w2) || !Aligned(y) ||
-      !Aligned(gateUp) || !Aligned(workspace) || workspaceBytes < FlashMoeFfnWorkspaceBytes(cfg, T, 0))
+  if (!x || !w13 || !w2 || !y || !Aligned(x) || !Aligned(w13) || !Aligned(w2) || !Aligned(y) || !Aligned(saved) ||
+      !Aligned(workspace) || (!saved && (!workspace || workspaceBytes < FlashMoeFfnWorkspaceBytes(cfg, T, 0))))
     return (int)cudaErrorInvalidValue;
   Call c;
   DENSE_TRY(BeginCall(&c, stream));
   const int64_t H = cfg->hiddenSize, I = cfg->intermediateSize;
   const bool bf16 = cfg->dtype == kBf16;
-  if (!gateUp && !stall && fdmoe::UseStream((int)T)) {
+  if (!saved && !stall && fdmoe::UseStream((int)T)) {
     DENSE_TRY(StreamProduct(c, x, w13, workspace, T, I, H, true, bf16, false));
     return StreamProduct(c, workspace, w2, y, T, H, I, false, bf16, true);
   }
-  DENSE_TRY(GatedProduct(c, x, w13, workspace, gateUp, T, H, I, bf16, stall));
+  void* h = saved ? static_cast<uint8_t*>(saved) + SavedOffset(cfg, T) : workspace;
+  DENSE_TRY(GatedProduct(c, x, w13, h, saved, T, H, I, bf16, stall));
   if (stall) return 0;
-  return PairProduct(c, {workspace, T, I, false}, {w2, H, I, false}, y, bf16);
+  return PairProduct(c, {h, T, I, false}, {w2, H, I, false}, y, bf16);
 }
 
 extern "C" int FlashMoeFfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y,
-                                  void* gateUp, void* workspace, size_t workspaceBytes, int64_t tokensNum, void* stream) {
-  return FfnForward(cfg, x, w13, w2, y, gateUp, workspace, workspaceBytes, tokensNum, stream, false);
+                                  void* saved, void* workspace, size_t workspaceBytes, int64_t tokensNum, void* stream) {
+  return FfnForward(cfg, x, w13, w2, y, saved, workspace, workspaceBytes, tokensNum, stream, false);
 }
 
 extern "C" int FlashMoeTestFfnStall(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y,
@@ -373,7 +382,7 @@ extern "C" int FlashMoeTestFfnStall(const FlashMoeFfnConfig* cfg, const void* x,
 }
 
 extern "C" int FlashMoeFfnBackward(const FlashMoeFfnConfig* cfg, const void* dy, const void* x, const void* w13,
-                                   const void* w2, const void* gateUp, void* dx, void* dw13, void* dw2, void* workspace,
+                                   const void* w2, const void* saved, void* dx, void* dw13, void* dw2, void* workspace,
                                    size_t workspaceBytes, int64_t T, void* stream) {
   DENSE_TRY(CheckFfn(cfg, T));
   const int64_t H = cfg->hiddenSize, I = cfg->intermediateSize;
@@ -383,16 +392,16 @@ extern "C" int FlashMoeFfnBackward(const FlashMoeFfnConfig* cfg, const void* dy,
     if (dw2) DENSE_CHECK(cudaMemsetAsync(dw2, 0, (size_t)(I * H) * 2, static_cast<cudaStream_t>(stream)));
     return 0;
   }
-  if (!dy || !x || !w13 || !w2 || !gateUp || !workspace || !Aligned(dy) || !Aligned(x) || !Aligned(w13) || !Aligned(w2) ||
-      !Aligned(gateUp) || !Aligned(workspace) || workspaceBytes < FlashMoeFfnWorkspaceBytes(cfg, T, 1))
+  if (!dy || !x || !w13 || !w2 || !saved || !workspace || !Aligned(dy) || !Aligned(x) || !Aligned(w13) || !Aligned(w2) ||
+      !Aligned(saved) || !Aligned(workspace) || workspaceBytes < FlashMoeFfnWorkspaceBytes(cfg, T, 1))
     return (int)cudaErrorInvalidValue;
   if (!dx && !dw13 && !dw2) return 0;
   Call c;
   DENSE_TRY(BeginCall(&c, stream));
   const bool bf16 = cfg->dtype == kBf16;
-  void* h = workspace;
-  void* dgu = static_cast<uint8_t*>(workspace) + fdmoe::AlignBytes((size_t)T * I * 2);
-  DENSE_TRY(GatedGradient(c, dy, w2, gateUp, dgu, h, T, H, I, bf16));
+  const void* h = static_cast<const uint8_t*>(saved) + SavedOffset(cfg, T);
+  void* dgu = workspace;
+  if (dx || dw13) DENSE_TRY(GatedGradient(c, dy, w2, saved, dgu, T, H, I, bf16));
   if (dx) DENSE_TRY(PairProduct(c, {dgu, T, 2 * I, false}, {w13, 2 * I, H, true}, dx, bf16));
   if (dw13) DENSE_TRY(PairProduct(c, {dgu, T, 2 * I, true}, {x, T, H, true}, dw13, bf16));
   if (dw2) DENSE_TRY(PairProduct(c, {dy, T, H, true}, {h, T, I, true}, dw2, bf16));

@@ -33,17 +33,24 @@ inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, 
   s.tile_tokens = s.token_tiles > 1 ? FDMOE_STREAM_TOKENS : RoundUp(tokens, 16);
   s.row_tiles = (rows + FDMOE_STREAM_ROWS - 1) / FDMOE_STREAM_ROWS;
   const int stage = parts * 16384 + s.tile_tokens * 128 + (mx4 ? (parts + 1) * 1024 : 0);
-  const int sums = std::min(tokens, s.tile_tokens) * parts * 512;  // partial sums, in the stages' place
+  // Partial sums, in the stages' place: groups of four tokens, the same number for every CTA of the cluster.
+  const int sums = (RoundUp(std::min(tokens, s.tile_tokens), 4) + 4 * (FDMOE_STREAM_SPLIT - 1)) * parts * 512;
   // Two CTAs per SM hide each other's beginning and end, if three stages each are left.
   s.per_sm = (kStreamSmemTwo - kStreamSlack) / stage >= 3 && sums <= kStreamSmemTwo - kStreamSlack ? 2 : 1;
   const int room = (s.per_sm == 2 ? kStreamSmemTwo : kStreamSmemOne) - kStreamSlack;
-  // Time in units of one k block on a full GPU: a CTA's k blocks and its beginning and end, times the waves.
+  // Time in cycles: a k block takes as long as its MMAs' issue or, with `active` CTAs reading weights at once, its share
+  // of the memory's 3500 bytes per cycle; a wave has a beginning and an end.
+  const double weights = parts * (mx4 ? 16384 + 1024 : 16384), issue = mx4 ? 400 + 250 * parts : 300 + 150 * parts;
   double best = 0;
   s.split = 1;
   for (int n = 1; n <= FDMOE_STREAM_SPLIT && n <= kblocks; ++n) {
-    const int64_t clusters = (int64_t)s.row_tiles * s.token_tiles;
     const int64_t slots = std::max(1, s.per_sm == 2 ? dev.stream_two[n] : dev.stream_one[n]);
-    const double t = (double)((clusters + slots - 1) / slots) * ((kblocks + n - 1) / n + 6);
+    double t = 0;
+    int64_t clusters = (int64_t)s.row_tiles * s.token_tiles;
+    for (int wave = 0; clusters > 0 && wave < 64; ++wave, clusters -= slots) {
+      const double active = (double)std::min(clusters, slots) * n;
+      t += (double)((kblocks + n - 1) / n) * std::max(issue, active * weights / 3500) + 5000;
+    }
     if (n == 1 || t < best) best = t, s.split = n;
   }
   s.stages = std::min(std::min(room / stage, (int)FDMOE_STREAM_STAGES), (kblocks + s.split - 1) / s.split);
@@ -66,7 +73,7 @@ struct PairPlan {
 inline PairPlan MakePairPlan(int64_t rows, int64_t cols, int kblocks, bool gated, bool mx4, const DeviceSlots& dev) {
   PairPlan best = {};
   double best_time = 0;
-  for (int tile_n = 256; tile_n >= (mx4 ? 256 : 128); tile_n /= 2)
+  for (int tile_n = 256; tile_n >= (mx4 ? 256 : 128); tile_n -= gated ? 128 : 64)  // whole groups of 64 result columns
     for (int split = 1; split <= FDMOE_PAIR_SPLIT && split <= kblocks; split *= 2) {
       PairPlan p;
       p.tile_n = tile_n;
@@ -76,7 +83,7 @@ inline PairPlan MakePairPlan(int64_t rows, int64_t cols, int kblocks, bool gated
       p.tiles_n = (int)((cols + tile_cols - 1) / tile_cols);
       const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, slots = std::max(1, dev.pair[split]);
       const double waves = (double)((tiles + slots - 1) / slots);
-      const double block = tile_n == 256 ? 512 : 330;
+      const double block = tile_n == 256 ? 512 : tile_n == 192 ? 435 : 360;
       const double k = (double)((kblocks + split - 1) / split) * block;
       const double t = split == 1 ? waves * k + 3000 : waves * (k + 6000);
       p.clusters = (int)(split == 1 ? std::min(tiles, slots) : tiles);

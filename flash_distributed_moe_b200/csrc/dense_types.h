@@ -27,7 +27,8 @@ enum {
   FDMOE_EPI_F32 = 1,         // as it is
   FDMOE_EPI_GATED = 2,       // silu(gate) * up, rounded to bf16 or fp16
   FDMOE_EPI_GATED_F32 = 3,   // silu(gate) * up
-  FDMOE_EPI_GATED_GRAD = 4,  // gradients of gate and up, and silu(gate) * up
+  FDMOE_EPI_GATED_GRAD = 4,  // gradients of gate and up
+  FDMOE_EPI_GATED_SAVE = 5,  // as FDMOE_EPI_GATED, and the gate and up projections
 };
 
 // Status codes of the dense kernels (first error wins).
@@ -41,13 +42,13 @@ enum {
 typedef struct {
   FdmoeTensorMap a, b;        // operands; `a` gives the rows of the result, `b` its columns
   FdmoeTensorMap sfa, sfb;    // their scales (4-bit operands)
-  FdmoeTensorMap out[3];      // results: the tile | h, gate, up | d gate, d up, h
-  const void* gu;             // gate and up projections [rows, 2 * cols] (FDMOE_EPI_GATED_GRAD)
+  FdmoeTensorMap out[3];      // results: the tile | h | h, gate, up | d gate, d up
+  FdmoeTensorMap gu[2];       // gate and up projections (FDMOE_EPI_GATED_GRAD)
   uint32_t* status;
   uint64_t timeout_ns;
   int32_t rows, cols;         // of the result
   int32_t tiles_m, tiles_n;
-  int32_t tile_n;             // 256 or 128 (4-bit operands: 256)
+  int32_t tile_n;             // 256, 192 or 128 (4-bit operands: 256)
   int32_t split;              // 1, 2 or 4 pairs per tile; above 1 a launch has a cluster per tile
   int32_t kblocks;
   int32_t a_mn, b_mn;         // operand stored with its rows along M (N) instead of along K
@@ -55,7 +56,6 @@ typedef struct {
   int32_t sf_chunks;          // 512-byte blocks of scales per 128 rows
   int32_t sf_up_block;        // block of 128 rows at which the up projection's scales start
   int32_t bf16;               // 16-bit operands and results are bf16, otherwise fp16
-  int32_t save_gu;            // gated: also write the gate and up projections
   int32_t stall;              // test hook: nothing is loaded, every wait runs out
 } FdmoePairParams;
 

@@ -16,19 +16,30 @@ namespace {
 
 constexpr int kQuantRows = 128, kQuantBlocks = 8;  // a CTA's tile: 128 rows x 256 columns, 1 KB of scales
 constexpr int kQuantThreads = 256;
+constexpr int kQuantBatch = 4;  // rows that a thread loads before it works on the first
 
 // Four lanes share a block of 32 elements, eight each.
 
-__device__ __forceinline__ void load_half8(const uint16_t* p, bool bf16, float (&v)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+// Eight elements as they are stored, and in 32 bits.
+template <bool F32>
+struct Eight {
+  uint4 w[F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* x, int64_t at) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + at * (F32 ? 4 : 2));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) unpack2(u[i], bf16, v[2 * i], v[2 * i + 1]);
-}
-__device__ __forceinline__ void load_f32x8(const float* p, float (&v)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
+    for (int i = 0; i < (F32 ? 2 : 1); ++i) w[i] = __ldg(p + i);
+  }
+  __device__ __forceinline__ void get(bool bf16, float (&v)[8]) const {
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
+#pragma unroll
+    for (int i = 0; i < 8; i += F32 ? 1 : 2) {
+      if constexpr (F32)
+        v[i] = __uint_as_float(u[i]);
+      else
+        unpack2(u[i / 2], bf16, v[i], v[i + 1]);
+    }
+  }
+};
 
 __device__ __forceinline__ uint32_t to_e2m1x8(const float (&v)[8]) {
   uint32_t r;
@@ -76,26 +87,32 @@ __global__ void __launch_bounds__(kQuantThreads) mx4_quantize_kernel(const Quant
   const bool in_cols = blk0 + b < blocks;
   const uint32_t group = 0xFu << (threadIdx.x & 28);
   if (in_cols) {
-#pragma unroll 4
-    for (int r = r0; r < rows; r += kQuantThreads / 32) {
-      const int64_t at = batch * p.batch_stride + (row0 + r) * p.row_stride + col;
-      float v[8];
-      if constexpr (F32)
-        load_f32x8(static_cast<const float*>(p.x) + at, v);
-      else
-        load_half8(static_cast<const uint16_t*>(p.x) + at, p.dtype == 0, v);
-      uint32_t top = 0;  // bits of the largest magnitude: infinities and NaN are above every number
+    for (int r1 = r0; r1 < rows; r1 += kQuantBatch * kQuantThreads / 32) {
+      Eight<F32> in[kQuantBatch];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-      top = max(top, __shfl_xor_sync(group, top, 1));
-      top = max(top, __shfl_xor_sync(group, top, 2));
-      const uint32_t field = top >> 23;
-      const uint32_t scale = field == 255 ? 255 : (field > 2 ? field - 2 : 0);
-      const float inv = __uint_as_float((254u - min(scale, 253u)) << 23);  // 2^-(scale - 127), exact
+      for (int i = 0; i < kQuantBatch; ++i) {
+        const int r = r1 + i * kQuantThreads / 32;
+        if (r < rows) in[i].load(p.x, batch * p.batch_stride + (row0 + r) * p.row_stride + col);
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= inv;
-      reinterpret_cast<uint32_t*>(p.values)[((batch * p.rows + row0 + r) * p.cols + col) >> 3] = to_e2m1x8(v);
-      if (part == 0) sc[(b >> 2) * kScaleBlock + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = (uint8_t)scale;
+      for (int i = 0; i < kQuantBatch; ++i) {
+        const int r = r1 + i * kQuantThreads / 32;
+        if (r >= rows) break;
+        float v[8];
+        in[i].get(p.dtype == 0, v);
+        uint32_t top = 0;  // bits of the largest magnitude: infinities and NaN are above every number
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+        top = max(top, __shfl_xor_sync(group, top, 1));
+        top = max(top, __shfl_xor_sync(group, top, 2));
+        const uint32_t field = top >> 23;
+        const uint32_t scale = field == 255 ? 255 : (field > 2 ? field - 2 : 0);
+        const float inv = __uint_as_float((254u - min(scale, 253u)) << 23);  // 2^-(scale - 127), exact
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= inv;
+        reinterpret_cast<uint32_t*>(p.values)[((batch * p.rows + row0 + r) * p.cols + col) >> 3] = to_e2m1x8(v);
+        if (part == 0) sc[(b >> 2) * kScaleBlock + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = (uint8_t)scale;
+      }
     }
   }
   __syncthreads();
@@ -131,23 +148,33 @@ __global__ void __launch_bounds__(kQuantThreads) mx4_dequantize_kernel(const Deq
   const int part = threadIdx.x & 3, b = (threadIdx.x >> 2) & 7, r0 = threadIdx.x >> 5;
   const int64_t col = (blk0 + b) * FDMOE_MX4_BLOCK + part * 8;
   if (blk0 + b >= blocks) return;
-#pragma unroll 4
-  for (int r = r0; r < rows; r += kQuantThreads / 32) {
-    const int64_t at = (batch * p.rows + row0 + r) * p.cols + col;
-    const uint32_t byte = sc[(b >> 2) * kScaleBlock + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)];
-    const float scale = __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : byte << 23);
-    float v[8];
-    from_e2m1x8(reinterpret_cast<const uint32_t*>(p.values)[at >> 3], v);
+  for (int r1 = r0; r1 < rows; r1 += kQuantBatch * kQuantThreads / 32) {
+    uint32_t in[kQuantBatch];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= scale;
-    if constexpr (F32) {
-      float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
-      o[0] = make_float4(v[0], v[1], v[2], v[3]);
-      o[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      const bool bf16 = p.dtype == 0;
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at) =
-          make_uint4(pack2(v[0], v[1], bf16), pack2(v[2], v[3], bf16), pack2(v[4], v[5], bf16), pack2(v[6], v[7], bf16));
+    for (int i = 0; i < kQuantBatch; ++i) {
+      const int r = r1 + i * kQuantThreads / 32;
+      if (r < rows) in[i] = __ldg(reinterpret_cast<const uint32_t*>(p.values) + (((batch * p.rows + row0 + r) * p.cols + col) >> 3));
+    }
+#pragma unroll
+    for (int i = 0; i < kQuantBatch; ++i) {
+      const int r = r1 + i * kQuantThreads / 32;
+      if (r >= rows) break;
+      const int64_t at = (batch * p.rows + row0 + r) * p.cols + col;
+      const uint32_t byte = sc[(b >> 2) * kScaleBlock + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)];
+      const float scale = __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : byte << 23);
+      float v[8];
+      from_e2m1x8(in[i], v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= scale;
+      if constexpr (F32) {
+        float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+        o[0] = make_float4(v[0], v[1], v[2], v[3]);
+        o[1] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        const bool bf16 = p.dtype == 0;
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at) =
+            make_uint4(pack2(v[0], v[1], bf16), pack2(v[2], v[3], bf16), pack2(v[4], v[5], bf16), pack2(v[6], v[7], bf16));
+      }
     }
   }
 }

@@ -56,28 +56,27 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _forward(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, save: bool):
-    (hidden, inter), tokens = w2.shape, x.shape[0]
+    (hidden, inter), tokens, lib = w2.shape, x.shape[0], _lib.lib()
     cfg = _config(hidden, inter, x.dtype)
     y = torch.empty_like(x)
-    gate_up = torch.empty((tokens, 2 * inter), dtype=x.dtype, device=x.device) if save else None
-    nbytes = _lib.lib().FlashMoeFfnWorkspaceBytes(cfg, tokens, 0)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    nbytes = lib.FlashMoeFfnSavedBytes(cfg, tokens) if save else lib.FlashMoeFfnWorkspaceBytes(cfg, tokens, 0)
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     _lib.run(x.get_device(), "FlashMoeFfnForward", cfg, x.data_ptr(), w13.data_ptr(), w2.data_ptr(), y.data_ptr(),
-             gate_up.data_ptr() if save else None, ws.data_ptr(), nbytes, tokens)
-    return y, gate_up
+             *((buf.data_ptr(), None, 0) if save else (None, buf.data_ptr(), nbytes)), tokens)
+    return y, buf
 
 
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w13, w2):
-        y, gate_up = _forward(x, w13, w2, save=True)
-        ctx.save_for_backward(x, w13, w2, gate_up)
+        y, saved = _forward(x, w13, w2, save=True)
+        ctx.save_for_backward(x, w13, w2, saved)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w13, w2, gate_up = ctx.saved_tensors
+        x, w13, w2, saved = ctx.saved_tensors
         (hidden, inter), tokens = w2.shape, x.shape[0]
         cfg = _config(hidden, inter, x.dtype)
         dy = _rows(dy)
@@ -85,13 +84,13 @@ class _GatedFfn(torch.autograd.Function):
         nbytes = _lib.lib().FlashMoeFfnWorkspaceBytes(cfg, tokens, 1)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         _lib.run(x.get_device(), "FlashMoeFfnBackward", cfg, dy.data_ptr(), x.data_ptr(), w13.data_ptr(), w2.data_ptr(),
-                 gate_up.data_ptr(), *[None if g is None else g.data_ptr() for g in grads], ws.data_ptr(), nbytes, tokens)
+                 saved.data_ptr(), *[None if g is None else g.data_ptr() for g in grads], ws.data_ptr(), nbytes, tokens)
         return tuple(grads)
 
 
 def gated_ffn(x: torch.Tensor, w13: Weight, w2: Weight) -> torch.Tensor:
     """x [..., H] -> [..., H].  Asynchronous on the current torch stream of x's device.  Differentiable in x, w13 and w2:
-    the gate and up projections of the tokens are kept for the backward pass, rounded to the dtype.  With Mx4Tensor
+    the gate and up projections of the tokens and silu(g) * u are kept for the backward pass, rounded to the dtype.  With Mx4Tensor
     weights (w13 [2, I, H], w2 [H, I]) x and the activations are quantised to 4 bits too, and there is no gradient.
 
     A training step may be captured into a CUDA graph.  As with every torch operator, capture it while no eager graph

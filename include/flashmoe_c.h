@@ -123,20 +123,23 @@ typedef struct {
   int32_t reserved[5];      /* zero */
 } FlashMoeFfnConfig;
 
-/* Bytes of scratch for a forward (backward == 0) or backward call; 0 for an unsupported config. */
+/* Bytes of scratch for a forward (backward == 0) or backward call, and of what a forward call keeps for
+ * the backward pass; 0 for an unsupported config. */
 size_t FlashMoeFfnWorkspaceBytes(const FlashMoeFfnConfig* config, int64_t tokensNum, int backward);
+size_t FlashMoeFfnSavedBytes(const FlashMoeFfnConfig* config, int64_t tokensNum);
 
-/* y[T,H] = (silu(x Wg^T) * (x Wu^T)) W2^T with w13 = [Wg; Wu] [2I,H], w2 [H,I].  `gateUp` [T,2I], if not
- * NULL, receives x Wg^T and x Wu^T for FlashMoeFfnBackward.  `y` may be `x`.  The projections, the
- * activation and both products are accumulated in fp32; h = silu(g) * u is rounded to the dtype. */
+/* y[T,H] = (silu(x Wg^T) * (x Wu^T)) W2^T with w13 = [Wg; Wu] [2I,H], w2 [H,I].  `saved`, if not NULL,
+ * receives what FlashMoeFfnBackward needs (the projections and h), and no workspace is needed then.  `y`
+ * may be `x`.  The projections, the activation and both products are accumulated in fp32; h = silu(g) * u
+ * is rounded to the dtype. */
 int FlashMoeFfnForward(const FlashMoeFfnConfig* config, const void* x, const void* w13, const void* w2,
-                       void* y, void* gateUp, void* workspace, size_t workspaceBytes, int64_t tokensNum,
+                       void* y, void* saved, void* workspace, size_t workspaceBytes, int64_t tokensNum,
                        void* stream);
 
 /* Gradients of x [T,H], w13 [2I,H] and w2 [H,I] from that of y; each of the three may be NULL.  With no
  * tokens the gradients of the weights are zero. */
 int FlashMoeFfnBackward(const FlashMoeFfnConfig* config, const void* dy, const void* x, const void* w13,
-                        const void* w2, const void* gateUp, void* dx, void* dw13, void* dw2,
+                        const void* w2, const void* saved, void* dx, void* dw13, void* dw2,
                         void* workspace, size_t workspaceBytes, int64_t tokensNum, void* stream);
 
 /* 4-bit microscaled matrices: E2M1 values, two to a byte (even element low), [batch, rows, cols / 2], and

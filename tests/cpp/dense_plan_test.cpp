@@ -39,14 +39,15 @@ int main() {
               CHECK(s.split >= 1 && s.split <= FDMOE_STREAM_SPLIT && s.split <= kb);
               CHECK(s.stages >= 1 && s.stages <= FDMOE_STREAM_STAGES);
               CHECK(s.stages * stage + kStreamSlack <= s.smem);
-              CHECK((tokens < s.tile_tokens ? tokens : s.tile_tokens) * parts * 512 + kStreamSlack <= s.smem);
+              const int in_tile = tokens < s.tile_tokens ? tokens : s.tile_tokens;  // partial sums, if the k axis is split
+              if (s.split > 1) CHECK(RoundUp(in_tile, 4 * s.split) * parts * 512 + kStreamSlack <= s.smem);
               CHECK(s.smem <= 226 * 1024 && (s.per_sm == 1 || s.smem <= 112 * 1024));
               const int cols = parts * s.tile_tokens + (mx4 ? s.stages * (parts + 1) * 8 : 0);
               CHECK(s.tmem_cols >= cols && s.tmem_cols >= 32 && (s.tmem_cols & (s.tmem_cols - 1)) == 0);
               CHECK(s.tmem_cols * s.per_sm <= 512);
               const PairPlan q = MakePairPlan(tokens, rows, kb, gated, mx4, dev);
               const int cols_tile = gated ? q.tile_n / 2 : q.tile_n;
-              CHECK(q.tile_n == 256 || (q.tile_n == 128 && !mx4));
+              CHECK(q.tile_n == 256 || ((q.tile_n == 128 || q.tile_n == 192) && !mx4));
               CHECK((q.split == 1 || q.split == 2 || q.split == 4) && q.split <= kb);
               CHECK(q.tiles_m * 256 >= tokens && q.tiles_n * cols_tile >= rows && q.clusters >= 1);
               CHECK(q.split == 1 ? q.clusters <= q.tiles_m * q.tiles_n : q.clusters == q.tiles_m * q.tiles_n);

@@ -156,7 +156,7 @@ def test_memory_around_the_results_is_left_alone(tokens):
         return buf, buf[pad:pad + n].view(*shape)
 
     ybuf, y = framed(tokens, hidden)
-    gbuf, gu = framed(tokens, 2 * inter)
+    gbuf, gu = framed(lib.FlashMoeFfnSavedBytes(cfg, tokens) // 2)
     dbuf = [framed(*t.shape) for t in (x, w13, w2)]
     sizes = [lib.FlashMoeFfnWorkspaceBytes(cfg, tokens, b) for b in (0, 1)]
     wbuf = [framed(s // 2) for s in sizes]
