@@ -38,25 +38,28 @@ inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, 
   // Two CTAs per SM hide each other's beginning and end, if three stages each are left.
   s.per_sm = (kStreamSmemTwo - kStreamSlack) / stage >= 3 && sums <= kStreamSmemTwo - kStreamSlack ? 2 : 1;
   const int room = (s.per_sm == 2 ? kStreamSmemTwo : kStreamSmemOne) - kStreamSlack;
-  // Time in cycles: a k block takes as long as its MMAs' issue or, with `active` CTAs reading weights at once, its share
-  // of the memory's 3500 bytes per cycle; a wave has a beginning and an end.
+  s.stages = std::min(room / stage, (int)FDMOE_STREAM_STAGES);
+  const int scales = mx4 ? (parts + 1) * 8 : 0;  // TMEM columns per stage
+  if (scales) s.stages = std::min(s.stages, ((s.per_sm == 2 ? 256 : 512) - parts * s.tile_tokens) / scales);
+  // Time in cycles.  A k block takes as long as its MMAs' issue, or as the weights of `active` CTAs do at the rate at
+  // which their stages in flight are filled, at most the memory's 3500 bytes per cycle; a wave has a beginning and an
+  // end.  Whole block, cold weights, CTAs per tile of the two products: 1 token of 2048 x 6144 22.7 us with 2 and 8,
+  // 21.3 with 4 and 8; 32 tokens of 4096 x 12288 63.5 with 1 and 6, 58.9 with 2 and 8, 63.6 with 2 and 4.
   const double weights = parts * (mx4 ? 16384 + 1024 : 16384), issue = mx4 ? 400 + 250 * parts : 300 + 150 * parts;
   double best = 0;
   s.split = 1;
   for (int n = 1; n <= FDMOE_STREAM_SPLIT && n <= kblocks; ++n) {
     const int64_t slots = std::max(1, s.per_sm == 2 ? dev.stream_two[n] : dev.stream_one[n]);
-    double t = 0;
+    double t = (n > 1 ? 1000 : 0) + s.tile_tokens * parts * 20.0 / n;  // the exchange of partial sums, and the epilogue
     int64_t clusters = (int64_t)s.row_tiles * s.token_tiles;
     for (int wave = 0; clusters > 0 && wave < 64; ++wave, clusters -= slots) {
       const double active = (double)std::min(clusters, slots) * n;
-      t += (double)((kblocks + n - 1) / n) * std::max(issue, active * weights / 3500) + 5000;
+      const double rate = std::min(3500.0, active * std::min(s.stages, (kblocks + n - 1) / n) * weights / 4000);
+      t += (double)((kblocks + n - 1) / n) * std::max(issue, active * weights / rate) + 5000;
     }
     if (n == 1 || t < best) best = t, s.split = n;
   }
-  s.stages = std::min(std::min(room / stage, (int)FDMOE_STREAM_STAGES), (kblocks + s.split - 1) / s.split);
-  const int scales = mx4 ? (parts + 1) * 8 : 0;  // TMEM columns per stage
-  const int cols_max = s.per_sm == 2 ? 256 : 512;
-  if (scales) s.stages = std::min(s.stages, (cols_max - parts * s.tile_tokens) / scales);
+  s.stages = std::min(s.stages, (kblocks + s.split - 1) / s.split);
   const int cols = parts * s.tile_tokens + s.stages * scales;
   s.tmem_cols = 32;
   while (s.tmem_cols < cols) s.tmem_cols *= 2;
@@ -92,8 +95,10 @@ inline PairPlan MakePairPlan(int64_t rows, int64_t cols, int kblocks, bool gated
   return best;
 }
 
-// Whether the streaming kernel takes a product instead of the pair kernel.
-inline bool UseStream(int tokens) { return tokens <= FDMOE_STREAM_TOKENS; }
+// Whether the streaming kernel takes a product instead of the pair kernel.  Whole block, streaming and pair kernels:
+// 64 tokens of 2048 x 768 14.8 and 20.9 us, of 1024 x 4096 18.8 and 21.0, of 2048 x 6144 29 and 32.6; 96 tokens 17.9
+// and 20.9, 22.2 and 21.2, 33.6 and 32.9; 128 tokens 21.0 and 21.0, 25.3 and 21.4, 38 and 33.
+inline bool UseStream(int64_t tokens) { return tokens <= 96; }
 
 
 inline size_t AlignBytes(size_t v) { return (v + 255) / 256 * 256; }

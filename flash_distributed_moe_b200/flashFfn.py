@@ -133,8 +133,8 @@ def _mx4_ffn(x: torch.Tensor, w13: Mx4Tensor, w2: Mx4Tensor) -> torch.Tensor:
     y = torch.empty_like(rows)
     nbytes = _lib.lib().FlashMoeMx4FfnWorkspaceBytes(cfg, rows.shape[0])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    _lib.run(x.get_device(), "FlashMoeMx4FfnForward", cfg, rows.data_ptr(), w13.values.data_ptr(), w13.scales.data_ptr(),
-             w2.values.data_ptr(), w2.scales.data_ptr(), y.data_ptr(), ws.data_ptr(), nbytes, rows.shape[0])
+    _lib.run(x.get_device(), "FlashMoeMx4FfnForward", cfg, rows.data_ptr(), *w13._pointers, *w2._pointers,
+             y.data_ptr(), ws.data_ptr(), nbytes, rows.shape[0])
     return y.reshape(x.shape)
 
 

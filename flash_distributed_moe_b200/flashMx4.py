@@ -24,11 +24,16 @@ def _check_dtype(dtype: torch.dtype) -> int:
     return DTYPES[dtype]
 
 
+def _scale_bytes(batch: int, rows: int, cols: int) -> int:
+    """The size of the scales, as FlashMoeMx4ScaleBytes gives it."""
+    return batch * -(-rows // 128) * -(-cols // 256) * 1024
+
+
 class Mx4Tensor:
     """A 4-bit matrix [rows, cols] or batch of them [batch, rows, cols].  `values` uint8 [..., rows, cols / 2] with the
     even element in the low half of a byte; `scales` uint8, in blocks of 512 for 128 rows and 128 columns."""
 
-    __slots__ = ("values", "scales", "shape")
+    __slots__ = ("shape", "device", "_tensors", "_buffer", "_pointers")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
         for t, name in ((values, "values"), (scales, "scales")):
@@ -41,32 +46,42 @@ class Mx4Tensor:
             raise RuntimeError("scales must have 512 bytes per 128 rows and 128 columns, an even number of blocks per row")
         if values.device != scales.device:
             raise RuntimeError("values and scales must be on the same device")
-        self._set(values, scales)
-
-    def _set(self, values, scales):
-        self.values, self.scales = values, scales
         self.shape = torch.Size((*values.shape[:-1], values.shape[-1] * 2))
+        self.device = values.device
+        self._tensors, self._buffer = (values, scales), None
+        self._pointers = values.data_ptr(), scales.data_ptr()
+
+    @classmethod
+    def _of_buffer(cls, buffer: torch.Tensor, shape: torch.Size, pointers) -> "Mx4Tensor":
+        """Values and scales one after the other in a buffer of the right size."""
+        self = cls.__new__(cls)
+        self.shape, self.device = shape, buffer.device
+        self._tensors, self._buffer, self._pointers = None, buffer, pointers
         return self
 
+    def _split(self):
+        if self._tensors is None:
+            n = self.shape.numel() // 2
+            self._tensors = self._buffer[:n].view(*self.shape[:-1], self.shape[-1] // 2), self._buffer[n:]
+        return self._tensors
+
     @property
-    def device(self) -> torch.device:
-        return self.values.device
+    def values(self) -> torch.Tensor:
+        return self._split()[0]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._split()[1]
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values that the matrix stands for.  Exact in fp32; in bf16 and fp16 unless they leave the type's range."""
-        code = _check_dtype(dtype)
-        values, shape = self.values, self.shape
-        if not values.is_cuda:
+        code, shape, device = _check_dtype(dtype), self.shape, self.device
+        if device.type != "cuda":
             raise RuntimeError("values must be a CUDA tensor")
-        out = torch.empty(shape, dtype=dtype, device=values.device)
-        _lib.run(values.get_device(), "FlashMoeMx4Dequantize", values.data_ptr(), self.scales.data_ptr(),
-                 shape[0] if len(shape) == 3 else 1, shape[-2], shape[-1], code, out.data_ptr())
+        out = torch.empty(shape, dtype=dtype, device=device)
+        _lib.run(device.index, "FlashMoeMx4Dequantize", *self._pointers, shape[0] if len(shape) == 3 else 1, shape[-2],
+                 shape[-1], code, out.data_ptr())
         return out
-
-
-def _scale_bytes(batch: int, rows: int, cols: int) -> int:
-    """The size of the scales, as FlashMoeMx4ScaleBytes gives it."""
-    return batch * -(-rows // 128) * -(-cols // 256) * 1024
 
 
 def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
@@ -76,41 +91,39 @@ def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
         raise RuntimeError("x tensor is undefined")
     if not x.is_cuda:
         raise RuntimeError("x must be a CUDA tensor")
-    code = _check_dtype(x.dtype)
-    shape = x.shape
+    code, shape, device = _check_dtype(x.dtype), x.shape, x.device
     if len(shape) not in (2, 3) or shape[-1] == 0 or shape[-1] % 32 != 0:
         raise RuntimeError("x must be [rows, cols] or [batch, rows, cols] with cols a multiple of 32")
     batch, rows, cols = shape if len(shape) == 3 else (1, *shape)
     ptr = x.data_ptr()
+    aligned = ptr % 16 == 0
     if x.is_contiguous():
-        strides = (rows * cols, cols)  # multiples of 32 elements
-        aligned = ptr % 16 == 0
+        batch_stride, row_stride = rows * cols, cols  # multiples of 32 elements
     else:
         per16 = 16 // x.element_size()
-        strides = (x.stride(0) if batch > 1 else 0, x.stride(-2) if rows > 1 else 0)
-        aligned = ptr % 16 == 0 and x.stride(-1) == 1 and strides[0] % per16 == 0 and strides[1] % per16 == 0
+        batch_stride, row_stride = x.stride(0) if batch > 1 else 0, x.stride(-2) if rows > 1 else 0
+        aligned = aligned and x.stride(-1) == 1 and batch_stride % per16 == 0 and row_stride % per16 == 0
     if not aligned:
         raise RuntimeError("rows of x must be contiguous and start on 16 bytes")
-    values = torch.empty((*shape[:-1], cols // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(_scale_bytes(batch, rows, cols), dtype=torch.uint8, device=x.device)
-    _lib.run(x.get_device(), "FlashMoeMx4Quantize", ptr, code, batch, rows, cols, *strides, values.data_ptr(),
-             scales.data_ptr())
-    return Mx4Tensor.__new__(Mx4Tensor)._set(values, scales)
+    n = batch * rows * cols // 2
+    buffer = torch.empty(n + _scale_bytes(batch, rows, cols), dtype=torch.uint8, device=device)
+    to = buffer.data_ptr()
+    _lib.run(device.index, "FlashMoeMx4Quantize", ptr, code, batch, rows, cols, batch_stride, row_stride, to, to + n)
+    return Mx4Tensor._of_buffer(buffer, shape, (to, to + n))
 
 
 def _product(a: Mx4Tensor, b: Mx4Tensor, out_dtype: torch.dtype, gated: bool) -> torch.Tensor:
     if not isinstance(a, Mx4Tensor) or not isinstance(b, Mx4Tensor):
         raise RuntimeError("operands must be Mx4Tensors")
     code = _check_dtype(out_dtype)
-    av, bv, sa, sb = a.values, b.values, a.shape, b.shape
-    if av.device != bv.device or not av.is_cuda:
+    device, sa, sb = a.device, a.shape, b.shape
+    if device != b.device or device.type != "cuda":
         raise RuntimeError("operands must be on the same CUDA device")
     if len(sa) != 2 or len(sb) != (3 if gated else 2) or sa[-1] != sb[-1] or (gated and sb[0] != 2):
         raise RuntimeError("operands must be [M, K] and " + ("[2, N, K]" if gated else "[N, K]"))
     m, n = sa[0], sb[-2]
-    out = torch.empty((m, n), dtype=out_dtype, device=av.device)
-    _lib.run(av.get_device(), "FlashMoeMx4Matmul", av.data_ptr(), a.scales.data_ptr(), bv.data_ptr(), b.scales.data_ptr(),
-             out.data_ptr(), code, m, n, sa[1], int(gated))
+    out = torch.empty((m, n), dtype=out_dtype, device=device)
+    _lib.run(device.index, "FlashMoeMx4Matmul", *a._pointers, *b._pointers, out.data_ptr(), code, m, n, sa[1], int(gated))
     return out
 
 
