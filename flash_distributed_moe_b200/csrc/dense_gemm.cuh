@@ -20,6 +20,11 @@ namespace dense {
 
 // ------------------------------------------------------------- bounded waits
 // Every wait ends: after `limit_ns` it records what it waited for, raises the CTA's abort flag, and all roles leave.
+// The warps that issue copies and MMAs run their loops with all lanes and let one elected lane issue: inside a branch
+// on the lane the compiler cannot tell that one thread is active, and instructions whose operands have to be uniform
+// cost several times as much (the pair kernel's k block took 684 cycles so, whatever the tile's width; it takes 365 at a
+// width of up to 192 and 520 at 256, where the tensor cores set the pace).  Their lanes wait each for itself: a vote
+// after every wait cost 40 cycles per k block.
 struct Waiter {
   volatile uint32_t* abort_flag;
   uint32_t* status;
@@ -29,10 +34,7 @@ struct Waiter {
     if (ptx::mbar_try_wait(bar, parity)) return true;
     return slow(bar, parity, code);
   }
-  // The same by a whole warp.  The warps that issue copies and MMAs run their loops together and let one elected lane
-  // issue: inside a branch on the lane the compiler cannot tell that one thread is active, and instructions whose
-  // operands have to be uniform cost several times as much (the pair kernel's k block took 684 cycles so, whatever the
-  // tile's width).
+  // The same by a whole warp that goes on together.
   __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, uint32_t code) const {
     return __all_sync(0xffffffffu, wait(bar, parity, code));
   }
@@ -114,6 +116,21 @@ __device__ __forceinline__ F2 sigmoid(F2 g) {
 }
 __device__ __forceinline__ F2 gate(F2 g, F2 u) { return g * sigmoid(g) * u; }
 
+// The projections g and u are kept for the backward pass in 24 bits, an fp32 number without its last eight (cut, so
+// that a NaN stays one): in the 16 bits of the operands their rounding would be as large an error of the gradients as the rounding of the
+// gradients themselves (relative error of dx and dw13 in bf16: 3.0e-3 instead of 2.4e-3).  The upper 16 bits of g and
+// u lie in [T, 2I], the eight that follow of both in one word of [T, I].
+__device__ __forceinline__ uint32_t upper16(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+__device__ __forceinline__ uint32_t next8(uint32_t g0, uint32_t u0, uint32_t g1, uint32_t u1) {
+  return __byte_perm(__byte_perm(g0, u0, 0x0051), __byte_perm(g1, u1, 0x0051), 0x5410);
+}
+// Two neighbouring values from a word of upper halves and a word of lower bytes (which = 0: g, 1: u); the last eight
+// bits are of no consequence.
+template <int which>
+__device__ __forceinline__ F2 from24(uint32_t upper, uint32_t lower) {
+  return as_f2(__byte_perm(upper, lower, which ? 0x1055 : 0x1044), __byte_perm(upper, lower, which ? 0x3277 : 0x3266));
+}
+
 // -------------------------------------------------------------- pair kernel
 // A pair of CTAs works on D[256 x tile_n] tiles: CTA r holds rows [128 r, 128 r + 128) of A, of D, and half of the
 // rows of B (gated: CTA 0 the gate projection's, CTA 1 the up projection's, so that D holds tile_n / 2 columns of
@@ -155,7 +172,7 @@ __device__ __forceinline__ void stage16(uint8_t* box, int lane, int j, uint32_t 
   *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(a, b, c, d);
 }
 
-template <bool MX4, int EPI>
+template <bool MX4, int EPI, bool BF16>
 __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_constant__ FdmoePairParams p) {
   using S = PairShape<MX4, EPI>;
   constexpr bool kGated = EPI == FDMOE_EPI_GATED || EPI == FDMOE_EPI_GATED_SAVE || EPI == FDMOE_EPI_GATED_F32;
@@ -225,7 +242,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % S::kStages;
           const uint32_t ph = (it / S::kStages) & 1;
-          if (!wt.wait_warp(empty + s, ph ^ 1, FDMOE_DENSE_TIMEOUT_EMPTY)) {
+          if (!wt.wait(empty + s, ph ^ 1, FDMOE_DENSE_TIMEOUT_EMPTY)) {
             ok = false;
             break;
           }
@@ -264,7 +281,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     // ---- MMAs: one thread of the even CTA
     if (rank == 0) {
       const bool elected = ptx::elect_one();
-      const uint32_t idesc = ptx::make_idesc_f16(256, p.tile_n, p.bf16, p.a_mn, p.b_mn);
+      const uint32_t idesc = ptx::make_idesc_f16(256, p.tile_n, BF16, p.a_mn, p.b_mn);
       // 16 k further: 32 bytes along a row, or 16 rows of 128 bytes
       const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
       const uint32_t a_lead = p.a_mn ? 8192 : 16, b_lead = p.b_mn ? 8192 : 16;
@@ -273,12 +290,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       for (int tile = first; ok && tile < tiles; tile += step, ++n) {
         const int acc = n % S::kAccs;
         const uint32_t aph = (n / S::kAccs) & 1;
-        if (!wt.wait_warp(acc_empty + acc, aph ^ 1, FDMOE_DENSE_TIMEOUT_ACC)) break;
+        if (!wt.wait(acc_empty + acc, aph ^ 1, FDMOE_DENSE_TIMEOUT_ACC)) break;
         ptx::tcgen05_fence_after();
         const uint32_t d = tmem + acc * kAccCols;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % S::kStages;
-          if (!wt.wait_warp(full + s, (it / S::kStages) & 1, FDMOE_DENSE_TIMEOUT_FULL)) {
+          if (!wt.wait(full + s, (it / S::kStages) & 1, FDMOE_DENSE_TIMEOUT_FULL)) {
             ok = false;
             break;
           }
@@ -322,9 +339,16 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     constexpr int kGroup = kF32 ? 32 : 64;
     constexpr int kMost = (kGated ? 128 : 256) / kGroup / 2;  // groups of a warp
     const int groups = tile_cols / kGroup, first_group = half * split + (int)part, group_step = 2 * split;
-    // Gradient: the boxes first take g and u of a group of columns, which dg and du then replace.
+    // Gradient: the boxes first take the upper halves of g and u of a group of columns, which dg and du then replace;
+    // the lower bytes of this lane's row come straight into registers.
     uint32_t gu_count = 0;
+    uint4 lower[8];
     auto fetch_gu = [&](const PairTile& t, int c) {
+      const int row = t.m * 256 + (int)rank * 128 + quad * 32 + lane, col = t.n * tile_cols + c * 64;
+      const uint16_t* at = static_cast<const uint16_t*>(p.lower) + (int64_t)row * p.cols + col;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        lower[j] = row < p.rows && col + 8 * j < p.cols ? __ldg(reinterpret_cast<const uint4*>(at) + j) : make_uint4(0, 0, 0, 0);
       if (elected) {
         ptx::bulk_wait_group_read0();
         ptx::mbar_expect_tx(gu_full + w, 8192);
@@ -339,7 +363,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       const int acc = n % S::kAccs;
       if constexpr (EPI == FDMOE_EPI_GATED_GRAD)
         if (first_group < groups) fetch_gu(t, first_group);
-      const bool done = wt.wait(acc_full + acc, (n / S::kAccs) & 1, FDMOE_DENSE_TIMEOUT_DONE);
+      const bool done = wt.wait_warp(acc_full + acc, (n / S::kAccs) & 1, FDMOE_DENSE_TIMEOUT_DONE);
       ptx::tcgen05_fence_after();
       const uint32_t d = tmem + acc * kAccCols + (uint32_t(quad * 32) << 16);
       const int row0 = t.m * 256 + (int)rank * 128 + quad * 32;
@@ -410,7 +434,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
           load(c * 64 + 32, v[1]);
           ptx::tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) w[j][i] = pack2(as_f2(v[i >> 4][(2 * i) & 31], v[i >> 4][(2 * i + 1) & 31]), p.bf16);
+          for (int i = 0; i < 32; ++i) w[j][i] = pack2(as_f2(v[i >> 4][(2 * i) & 31], v[i >> 4][(2 * i + 1) & 31]), BF16);
         }
         release();
         if constexpr (S::kBoxes >= kMost) boxes_free();
@@ -499,19 +523,25 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {  // eight columns
-              uint32_t h[4], gw[4];
+              uint32_t h[4], gw[4], lower[4];
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 const int at = 8 * j + 2 * q;
-                h[q] = pack2(gate(as_f2(gi[at], gi[at + 1]), as_f2(ui[at], ui[at + 1])), p.bf16);
+                h[q] = pack2(gate(as_f2(gi[at], gi[at + 1]), as_f2(ui[at], ui[at + 1])), BF16);
                 if constexpr (EPI == FDMOE_EPI_GATED_SAVE) {
-                  // kept for the backward pass, rounded like every other activation
-                  gw[q] = pack2(as_f2(gi[at], gi[at + 1]), p.bf16);
-                  up[16 * i + 4 * j + q] = pack2(as_f2(ui[at], ui[at + 1]), p.bf16);
+                  gw[q] = upper16(gi[at], gi[at + 1]);
+                  up[16 * i + 4 * j + q] = upper16(ui[at], ui[at + 1]);
+                  lower[q] = next8(gi[at], ui[at], gi[at + 1], ui[at + 1]);
                 }
               }
               stage16(buf, lane, i * 4 + j, h[0], h[1], h[2], h[3]);
-              if constexpr (EPI == FDMOE_EPI_GATED_SAVE) stage16(buf + 4096, lane, i * 4 + j, gw[0], gw[1], gw[2], gw[3]);
+              if constexpr (EPI == FDMOE_EPI_GATED_SAVE) {
+                stage16(buf + 4096, lane, i * 4 + j, gw[0], gw[1], gw[2], gw[3]);
+                const int row = row0 + lane, col = col0 + c * 64 + i * 32 + j * 8;  // columns come in eights
+                if (row < p.rows && col < p.cols)
+                  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.lower) + (int64_t)row * p.cols + col) =
+                      make_uint4(lower[0], lower[1], lower[2], lower[3]);
+              }
             }
           }
           if constexpr (!MX4) release();
@@ -539,7 +569,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
         for (int c = first_group; c < groups; c += group_step) {
           if (c != first_group) fetch_gu(t, c);
           wt.wait_warp(gu_full + w, gu_count++ & 1, FDMOE_DENSE_TIMEOUT_FULL);
-#pragma unroll 1
+#pragma unroll
           for (int i = 0; i < 2; ++i) {
             uint32_t v[32];
             load(c * 64 + i * 32, v);
@@ -548,21 +578,19 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
             for (int j = 0; j < 4; ++j) {  // eight columns
               uint4* const g_at = reinterpret_cast<uint4*>(buf + lane * 128 + (((i * 4 + j) ^ (lane & 7)) << 4));
               uint4* const u_at = g_at + 4096 / 16;
-              const uint4 g4 = *g_at, u4 = *u_at;
+              const uint4 g4 = *g_at, u4 = *u_at, l4 = lower[i * 4 + j];
               const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
+              const uint32_t lw[4] = {l4.x, l4.y, l4.z, l4.w};
               uint32_t dg[4], du[4];
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                float a, b;
-                unpack2(gw[q], p.bf16, a, b);
-                const F2 g(a, b);
-                unpack2(uw[q], p.bf16, a, b);
-                const F2 u(a, b), dh = as_f2(v[8 * j + 2 * q], v[8 * j + 2 * q + 1]);
+                const F2 g = from24<0>(gw[q], lw[q]), u = from24<1>(uw[q], lw[q]);
+                const F2 dh = as_f2(v[8 * j + 2 * q], v[8 * j + 2 * q + 1]);
                 const F2 sg = sigmoid(g), silu = g * sg;
                 // silu' = s + g s (1 - s)
                 const F2 slope = fma2(silu, fma2(sg, F2(-1.0f, -1.0f), F2(1.0f, 1.0f)), sg);
-                dg[q] = pack2(dh * u * slope, p.bf16);
-                du[q] = pack2(dh * silu, p.bf16);
+                dg[q] = pack2(dh * u * slope, BF16);
+                du[q] = pack2(dh * silu, BF16);
               }
               *g_at = make_uint4(dg[0], dg[1], dg[2], dg[3]);
               *u_at = make_uint4(du[0], du[1], du[2], du[3]);
@@ -656,7 +684,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
       ptx::grid_launch_dependents();
       for (int kb = kb0; kb < kb1; ++kb) {
         const int i = kb - kb0, s = i % p.stages;
-        if (i >= ahead && !wt.wait_warp(empty + s, ((i / p.stages) & 1) ^ 1, FDMOE_DENSE_TIMEOUT_EMPTY)) break;
+        if (i >= ahead && !wt.wait(empty + s, ((i / p.stages) & 1) ^ 1, FDMOE_DENSE_TIMEOUT_EMPTY)) break;
         if (!elected) continue;
         if (i >= ahead) load_weights(s, kb);
         uint8_t* sb = smem + s * stage_bytes + kParts * kStageOperand;
@@ -672,7 +700,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
         const int i = kb - kb0, s = i % p.stages;
-        if (!wt.wait_warp(full + s, (i / p.stages) & 1, FDMOE_DENSE_TIMEOUT_FULL)) {
+        if (!wt.wait(full + s, (i / p.stages) & 1, FDMOE_DENSE_TIMEOUT_FULL)) {
           ok = false;
           break;
         }
@@ -710,7 +738,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
     }
   } else {
     const int count = min(nt, p.tokens - tok0);
-    const bool done = wt.wait(&acc_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
+    const bool done = wt.wait_warp(&acc_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
     ptx::tcgen05_fence_after();
     const uint32_t d = tmem + (uint32_t(warp * 32) << 16);
     const int row = row0 + warp * 32 + lane;

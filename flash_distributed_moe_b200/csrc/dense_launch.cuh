@@ -40,14 +40,19 @@ struct LaunchConfig {
   }
 };
 
-template <bool MX4, int EPI>
-cudaError_t launch_pair(const FdmoePairParams& p, int clusters, cudaStream_t stream) {
+template <bool MX4, int EPI, bool BF16>
+cudaError_t launch_pair_of(const FdmoePairParams& p, int clusters, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
   constexpr int smem = PairShape<MX4, EPI>::kSmem;
-  cudaError_t e = prepare_kernel(pair_gemm<MX4, EPI>, smem, done);
+  cudaError_t e = prepare_kernel(pair_gemm<MX4, EPI, BF16>, smem, done);
   if (e != cudaSuccess) return e;
   const LaunchConfig l(dim3(clusters * 2 * p.split), kPairThreads, smem, 2 * p.split, stream);
-  return cudaLaunchKernelEx(&l.cfg, pair_gemm<MX4, EPI>, p);
+  return cudaLaunchKernelEx(&l.cfg, pair_gemm<MX4, EPI, BF16>, p);
+}
+template <bool MX4, int EPI>
+cudaError_t launch_pair(const FdmoePairParams& p, int clusters, cudaStream_t stream) {
+  if constexpr (EPI == FDMOE_EPI_F32 || EPI == FDMOE_EPI_GATED_F32) return launch_pair_of<MX4, EPI, true>(p, clusters, stream);
+  return p.bf16 ? launch_pair_of<MX4, EPI, true>(p, clusters, stream) : launch_pair_of<MX4, EPI, false>(p, clusters, stream);
 }
 
 constexpr int kStreamSmemMax = 227 * 1024 - 1024;  // beside the barriers in static shared memory

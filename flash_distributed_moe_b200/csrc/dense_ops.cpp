@@ -202,38 +202,53 @@ int StreamProduct(const Call& c, const void* x, const void* w, void* out, int64_
   return fdmoe_stream_launch(&p, gated ? FDMOE_EPI_GATED : FDMOE_EPI_HALF, 0, s.smem, c.stream);
 }
 
-// h[T, I] = silu(g) * u with [g, u] = x w13^T; also g and u to gu [T, 2I] where that is given.
-int GatedProduct(const Call& c, const void* x, const void* w13, void* h, void* gu, int64_t T, int64_t H, int64_t I,
-                 bool bf16, bool stall) {
+// What a forward call keeps for the backward pass: the upper halves of the projections [T, 2I], their lower bytes
+// [T, I], and h [T, I], 16 bits each.
+struct Saved {
+  uint8_t *gu = nullptr, *lower = nullptr, *h = nullptr;
+  static size_t Bytes(int64_t T, int64_t I) { return fdmoe::AlignBytes((size_t)T * I * 4) + 2 * fdmoe::AlignBytes((size_t)T * I * 2); }
+  Saved() = default;
+  Saved(const void* base, int64_t T, int64_t I) {
+    gu = static_cast<uint8_t*>(const_cast<void*>(base));
+    lower = gu + fdmoe::AlignBytes((size_t)T * I * 4);
+    h = lower + fdmoe::AlignBytes((size_t)T * I * 2);
+  }
+};
+
+// h[T, I] = silu(g) * u with [g, u] = x w13^T; also what is to be kept, where `saved` has room for it.
+int GatedProduct(const Call& c, const void* x, const void* w13, void* h, const Saved& saved, int64_t T, int64_t H,
+                 int64_t I, bool bf16, bool stall) {
   FdmoePairParams p;
   memset(&p, 0, sizeof(p));
   const int clusters = PairShape(p, c, T, I, H, true, false);
   DENSE_TRY(MakeMap(c, &p.a, x, 2, T, H, H * 2, 64, 128));
   DENSE_TRY(MakeMap(c, &p.b, w13, 2, 2 * I, H, H * 2, 64, p.tile_n / 2));
   DENSE_TRY(MakeMap(c, &p.out[0], h, 2, T, I, I * 2, 64, 32));
-  if (gu) {
+  if (saved.gu) {
     // two matrices side by side: what a tile has beyond column I of the gate projection is not stored
-    DENSE_TRY(MakeMap(c, &p.out[1], gu, 2, T, I, I * 4, 64, 32));
-    DENSE_TRY(MakeMap(c, &p.out[2], static_cast<uint8_t*>(gu) + I * 2, 2, T, I, I * 4, 64, 32));
+    DENSE_TRY(MakeMap(c, &p.out[1], saved.gu, 2, T, I, I * 4, 64, 32));
+    DENSE_TRY(MakeMap(c, &p.out[2], saved.gu + I * 2, 2, T, I, I * 4, 64, 32));
+    p.lower = saved.lower;
   }
   p.up_row = (int32_t)I;
   p.bf16 = bf16;
   p.stall = stall;
-  return fdmoe_pair_launch(&p, gu ? FDMOE_EPI_GATED_SAVE : FDMOE_EPI_GATED, 0, clusters, c.stream);
+  return fdmoe_pair_launch(&p, saved.gu ? FDMOE_EPI_GATED_SAVE : FDMOE_EPI_GATED, 0, clusters, c.stream);
 }
 
 // From dy: dgu [T, 2I].
-int GatedGradient(const Call& c, const void* dy, const void* w2, const void* gu, void* dgu, int64_t T, int64_t H, int64_t I,
-                  bool bf16) {
+int GatedGradient(const Call& c, const void* dy, const void* w2, const Saved& saved, void* dgu, int64_t T, int64_t H,
+                  int64_t I, bool bf16) {
   FdmoePairParams p;
   memset(&p, 0, sizeof(p));
   const int clusters = PairShape(p, c, T, I, H, false, false);
   DENSE_TRY(MakeMap(c, &p.a, dy, 2, T, H, H * 2, 64, 128));
   DENSE_TRY(MakeMap(c, &p.b, w2, 2, H, I, I * 2, 64, 64));
   for (int i = 0; i < 2; ++i) {
-    DENSE_TRY(MakeMap(c, &p.gu[i], static_cast<const uint8_t*>(gu) + i * I * 2, 2, T, I, I * 4, 64, 32));
+    DENSE_TRY(MakeMap(c, &p.gu[i], saved.gu + i * I * 2, 2, T, I, I * 4, 64, 32));
     DENSE_TRY(MakeMap(c, &p.out[i], static_cast<uint8_t*>(dgu) + i * I * 2, 2, T, I, I * 4, 64, 32));
   }
+  p.lower = saved.lower;
   p.b_mn = 1;
   p.bf16 = bf16;
   return fdmoe_pair_launch(&p, FDMOE_EPI_GATED_GRAD, 0, clusters, c.stream);
@@ -341,31 +356,28 @@ extern "C" size_t FlashMoeFfnWorkspaceBytes(const FlashMoeFfnConfig* cfg, int64_
   return fdmoe::AlignBytes((size_t)tokensNum * cfg->intermediateSize * (backward ? 4 : 2));
 }
 
-// What a forward call keeps for the backward pass: the projections [T, 2I], then h [T, I].
-static size_t SavedOffset(const FlashMoeFfnConfig* cfg, int64_t T) {
-  return fdmoe::AlignBytes((size_t)T * cfg->intermediateSize * 4);
-}
 extern "C" size_t FlashMoeFfnSavedBytes(const FlashMoeFfnConfig* cfg, int64_t tokensNum) {
   if (CheckFfn(cfg, tokensNum) != 0) return 0;
-  return SavedOffset(cfg, tokensNum) + fdmoe::AlignBytes((size_t)tokensNum * cfg->intermediateSize * 2);
+  return Saved::Bytes(tokensNum, cfg->intermediateSize);
 }
 
-static int FfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y, void* saved,
+static int FfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y, void* savedFor,
                       void* workspace, size_t workspaceBytes, int64_t T, void* stream, bool stall) {
   DENSE_TRY(CheckFfn(cfg, T));
   if (T == 0) return 0;
-  if (!x || !w13 || !w2 || !y || !Aligned(x) || !Aligned(w13) || !Aligned(w2) || !Aligned(y) || !Aligned(saved) ||
-      !Aligned(workspace) || (!saved && (!workspace || workspaceBytes < FlashMoeFfnWorkspaceBytes(cfg, T, 0))))
+  if (!x || !w13 || !w2 || !y || !Aligned(x) || !Aligned(w13) || !Aligned(w2) || !Aligned(y) || !Aligned(savedFor) ||
+      !Aligned(workspace) || (!savedFor && (!workspace || workspaceBytes < FlashMoeFfnWorkspaceBytes(cfg, T, 0))))
     return (int)cudaErrorInvalidValue;
   Call c;
   DENSE_TRY(BeginCall(&c, stream));
   const int64_t H = cfg->hiddenSize, I = cfg->intermediateSize;
   const bool bf16 = cfg->dtype == kBf16;
-  if (!saved && !stall && fdmoe::UseStream(T)) {
+  if (!savedFor && !stall && fdmoe::UseStream(T)) {
     DENSE_TRY(StreamProduct(c, x, w13, workspace, T, I, H, true, bf16, false));
     return StreamProduct(c, workspace, w2, y, T, H, I, false, bf16, true);
   }
-  void* h = saved ? static_cast<uint8_t*>(saved) + SavedOffset(cfg, T) : workspace;
+  const Saved saved = savedFor ? Saved(savedFor, T, I) : Saved();
+  void* h = savedFor ? saved.h : workspace;
   DENSE_TRY(GatedProduct(c, x, w13, h, saved, T, H, I, bf16, stall));
   if (stall) return 0;
   return PairProduct(c, {h, T, I, false}, {w2, H, I, false}, y, bf16);
@@ -382,7 +394,7 @@ extern "C" int FlashMoeTestFfnStall(const FlashMoeFfnConfig* cfg, const void* x,
 }
 
 extern "C" int FlashMoeFfnBackward(const FlashMoeFfnConfig* cfg, const void* dy, const void* x, const void* w13,
-                                   const void* w2, const void* saved, void* dx, void* dw13, void* dw2, void* workspace,
+                                   const void* w2, const void* savedBy, void* dx, void* dw13, void* dw2, void* workspace,
                                    size_t workspaceBytes, int64_t T, void* stream) {
   DENSE_TRY(CheckFfn(cfg, T));
   const int64_t H = cfg->hiddenSize, I = cfg->intermediateSize;
@@ -392,19 +404,19 @@ extern "C" int FlashMoeFfnBackward(const FlashMoeFfnConfig* cfg, const void* dy,
     if (dw2) DENSE_CHECK(cudaMemsetAsync(dw2, 0, (size_t)(I * H) * 2, static_cast<cudaStream_t>(stream)));
     return 0;
   }
-  if (!dy || !x || !w13 || !w2 || !saved || !workspace || !Aligned(dy) || !Aligned(x) || !Aligned(w13) || !Aligned(w2) ||
-      !Aligned(saved) || !Aligned(workspace) || workspaceBytes < FlashMoeFfnWorkspaceBytes(cfg, T, 1))
+  if (!dy || !x || !w13 || !w2 || !savedBy || !workspace || !Aligned(dy) || !Aligned(x) || !Aligned(w13) || !Aligned(w2) ||
+      !Aligned(savedBy) || !Aligned(workspace) || workspaceBytes < FlashMoeFfnWorkspaceBytes(cfg, T, 1))
     return (int)cudaErrorInvalidValue;
   if (!dx && !dw13 && !dw2) return 0;
   Call c;
   DENSE_TRY(BeginCall(&c, stream));
   const bool bf16 = cfg->dtype == kBf16;
-  const void* h = static_cast<const uint8_t*>(saved) + SavedOffset(cfg, T);
+  const Saved saved(savedBy, T, I);
   void* dgu = workspace;
   if (dx || dw13) DENSE_TRY(GatedGradient(c, dy, w2, saved, dgu, T, H, I, bf16));
   if (dx) DENSE_TRY(PairProduct(c, {dgu, T, 2 * I, false}, {w13, 2 * I, H, true}, dx, bf16));
   if (dw13) DENSE_TRY(PairProduct(c, {dgu, T, 2 * I, true}, {x, T, H, true}, dw13, bf16));
-  if (dw2) DENSE_TRY(PairProduct(c, {dy, T, H, true}, {h, T, I, true}, dw2, bf16));
+  if (dw2) DENSE_TRY(PairProduct(c, {dy, T, H, true}, {saved.h, T, I, true}, dw2, bf16));
   return 0;
 }
 

@@ -71,8 +71,11 @@ struct PairPlan {
   int tile_n, split, tiles_m, tiles_n, clusters;
 };
 
-// `cols`: of the result; `kblocks` stages of k.  Time in cycles: the waves of tiles, each its k blocks' MMAs, and once
-// per launch (per cluster where pairs share a tile) its beginning and end.
+// `cols`: of the result; `kblocks` stages of k.  Time in cycles: the waves of tiles, each its k blocks (about 520,
+// 455 and 365 cycles at widths of 256, 192 and 128) and once per launch, or per cluster where pairs share a tile, its
+// beginning and end; sharing also takes the partial sums' way through the cluster's shared memory, at 14 bytes a cycle.
+// In us, for width / pairs per tile: 4096 x 2048 x 6144 (rows, columns, k) 69 with 256/1, 80 with 192/1, 95 with
+// 128/1, 90 with 256/2; 777 x 1000 x 5488 36, 32, 28 and 24, 19 with 128/2, 36 with 128/4.
 inline PairPlan MakePairPlan(int64_t rows, int64_t cols, int kblocks, bool gated, bool mx4, const DeviceSlots& dev) {
   PairPlan best = {};
   double best_time = 0;
@@ -86,9 +89,10 @@ inline PairPlan MakePairPlan(int64_t rows, int64_t cols, int kblocks, bool gated
       p.tiles_n = (int)((cols + tile_cols - 1) / tile_cols);
       const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, slots = std::max(1, dev.pair[split]);
       const double waves = (double)((tiles + slots - 1) / slots);
-      const double block = tile_n == 256 ? 512 : tile_n == 192 ? 435 : 360;
+      const double block = tile_n == 256 ? 520 : tile_n == 192 ? 455 : 365;
       const double k = (double)((kblocks + split - 1) / split) * block;
-      const double t = split == 1 ? waves * k + 3000 : waves * (k + 6000);
+      const double exchange = (double)tile_n * 512 * (split - 1) / split / 14;
+      const double t = split == 1 ? waves * k + 3000 : waves * (k + 3500 + exchange);
       p.clusters = (int)(split == 1 ? std::min(tiles, slots) : tiles);
       if (best_time == 0 || t < best_time) best = p, best_time = t;
     }

@@ -42,8 +42,9 @@ enum {
 typedef struct {
   FdmoeTensorMap a, b;        // operands; `a` gives the rows of the result, `b` its columns
   FdmoeTensorMap sfa, sfb;    // their scales (4-bit operands)
-  FdmoeTensorMap out[3];      // results: the tile | h | h, gate, up | d gate, d up
-  FdmoeTensorMap gu[2];       // gate and up projections (FDMOE_EPI_GATED_GRAD)
+  FdmoeTensorMap out[3];      // results: the tile | h | h, upper halves of gate, up | d gate, d up
+  FdmoeTensorMap gu[2];       // upper halves of gate and up projections (FDMOE_EPI_GATED_GRAD)
+  void* lower;                // [rows, cols] lower bytes of both (FDMOE_EPI_GATED_SAVE and FDMOE_EPI_GATED_GRAD)
   uint32_t* status;
   uint64_t timeout_ns;
   int32_t rows, cols;         // of the result

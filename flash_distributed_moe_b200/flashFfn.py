@@ -90,7 +90,7 @@ class _GatedFfn(torch.autograd.Function):
 
 def gated_ffn(x: torch.Tensor, w13: Weight, w2: Weight) -> torch.Tensor:
     """x [..., H] -> [..., H].  Asynchronous on the current torch stream of x's device.  Differentiable in x, w13 and w2:
-    the gate and up projections of the tokens and silu(g) * u are kept for the backward pass, rounded to the dtype.  With Mx4Tensor
+    the gate and up projections of the tokens and silu(g) * u are kept for the backward pass, in 24 bits and in the dtype.  With Mx4Tensor
     weights (w13 [2, I, H], w2 [H, I]) x and the activations are quantised to 4 bits too, and there is no gradient.
 
     A training step may be captured into a CUDA graph.  As with every torch operator, capture it while no eager graph

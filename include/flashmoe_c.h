@@ -129,7 +129,7 @@ size_t FlashMoeFfnWorkspaceBytes(const FlashMoeFfnConfig* config, int64_t tokens
 size_t FlashMoeFfnSavedBytes(const FlashMoeFfnConfig* config, int64_t tokensNum);
 
 /* y[T,H] = (silu(x Wg^T) * (x Wu^T)) W2^T with w13 = [Wg; Wu] [2I,H], w2 [H,I].  `saved`, if not NULL,
- * receives what FlashMoeFfnBackward needs (the projections and h), and no workspace is needed then.  `y`
+ * receives what FlashMoeFfnBackward needs (the projections in 24 bits, and h), and no workspace is needed then.  `y`
  * may be `x`.  The projections, the activation and both products are accumulated in fp32; h = silu(g) * u
  * is rounded to the dtype. */
 int FlashMoeFfnForward(const FlashMoeFfnConfig* config, const void* x, const void* w13, const void* w2,

@@ -284,3 +284,13 @@ def test_refusals():
     (dx,) = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
     with pytest.raises(RuntimeError):  # no second derivative
         dx.sum().backward()
+
+
+def test_a_nan_token_reaches_the_gradients():
+    x, w13, w2, dy = dl.make(20, 64, 72, BF16, seed=11)
+    x[5, 7] = float("nan")
+    leaves = [t.requires_grad_() for t in (x, w13, w2)]
+    dx, dw13, dw2 = torch.autograd.grad(gated_ffn(*leaves), leaves, dy)
+    keep = torch.arange(20, device="cuda") != 5
+    assert torch.isnan(dx[5]).all() and torch.isfinite(dx[keep]).all()
+    assert torch.isnan(dw13).all() and torch.isnan(dw2).all()
