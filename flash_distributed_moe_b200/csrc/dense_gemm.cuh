@@ -152,7 +152,7 @@ struct PairShape {
   static constexpr int kStages = 5;
   static constexpr int kAccs = MX4 ? 1 : 2;  // 256 columns each; 4-bit operands' scales need columns too
   static constexpr int kScales = MX4 ? 6 * kScaleBlock : 0;  // per stage: A 2 blocks, B 4
-  static constexpr int kBarriers = 256;
+  static constexpr int kBarriers = 256 + FDMOE_PAIR_LIST * 4;  // and the list of tiles
   static constexpr int kSmem =
       kStages * (2 * kStageOperand + kScales) + 8 * kStaging + kBarriers + 1024;  // 1024: alignment of the base
 };
@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
   using S = PairShape<MX4, EPI>;
   constexpr bool kGated = EPI == FDMOE_EPI_GATED || EPI == FDMOE_EPI_GATED_SAVE || EPI == FDMOE_EPI_GATED_F32;
   constexpr bool kF32 = EPI == FDMOE_EPI_F32 || EPI == FDMOE_EPI_GATED_F32;
+  constexpr bool kMany = !MX4 && EPI == FDMOE_EPI_HALF;  // launches may have several products
   constexpr int kAccCols = 256;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
@@ -190,13 +191,13 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
   uint64_t* gu_full = acc_empty + S::kAccs;  // gradient: one per epilogue warp
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gu_full + 8);
   volatile uint32_t* abort_flag = tmem_slot + 1;
+  uint32_t* list = tmem_slot + 2;  // [0]: how many; product << 28 | tile
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // A cluster is `split` pairs, which share the k axis of a tile.
   const uint32_t cta = ptx::cluster_rank(), rank = cta & 1, leader = cta & ~1u, part = cta >> 1;
   const int split = p.split;
-  const int kb0 = p.kblocks * (int)part / split, kb1 = p.kblocks * ((int)part + 1) / split;
-  const int half_n = p.tile_n >> 1;  // rows of B per CTA; gated: columns of each projection
+  const int first = blockIdx.x / (2 * split), step = gridDim.x / (2 * split);
   const Waiter wt{abort_flag, p.status, p.timeout_ns};
 
   if (threadIdx.x == 0) {
@@ -216,6 +217,31 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     ptx::tmem_alloc_pair(tmem_slot, 512);
     ptx::tmem_relinquish_pair();
   }
+  if constexpr (kMany) {
+    // The tiles of several products in this pair's order: rounds over the pairs, each taking part as long as it has
+    // tiles of the product left, so that the tiles in work at a time are neighbours.
+    if (warp == 3 && p.products > 1) {
+      uint32_t n = 0;
+      for (int g = 0; g < p.products; ++g) {
+        uint32_t have[FDMOE_PAIR_MOST / 32], tile = 0;
+#pragma unroll
+        for (int i = 0; i < FDMOE_PAIR_MOST / 32; ++i) have[i] = i * 32 + lane < step ? p.count[g][i * 32 + lane] : 0;
+        for (uint32_t r = 0; r < p.count[g][first]; ++r) {
+          uint32_t before = 0, all = 0;
+#pragma unroll
+          for (int i = 0; i < FDMOE_PAIR_MOST / 32; ++i) {
+            const uint32_t in = __ballot_sync(0xffffffffu, have[i] > r);
+            all += __popc(in);
+            if (first >= i * 32) before += __popc(first >= i * 32 + 32 ? in : in & ((1u << (first - i * 32)) - 1u));
+          }
+          if (lane == 0 && n < FDMOE_PAIR_LIST - 3) list[1 + n] = (uint32_t)g << 28 | (tile + before);
+          tile += all;
+          ++n;
+        }
+      }
+      if (lane == 0) list[0] = min(n, (uint32_t)FDMOE_PAIR_LIST - 3);
+    }
+  }
   ptx::tcgen05_fence_before();
   __syncthreads();
   ptx::cluster_sync_relaxed();  // all CTAs' barriers are set up
@@ -224,21 +250,37 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
   ptx::grid_wait_dependency();  // nothing of global memory is touched before this
   ptx::grid_launch_dependents();
 
-  const int tiles = p.tiles_m * p.tiles_n;
-  const int first = blockIdx.x / (2 * split), step = gridDim.x / (2 * split);
+  // The i-th tile of this pair (cluster) and its product.
+  const auto tile_at = [&](int i, int& g, PairTile& t) {
+    g = 0;
+    int tile = first + i * step;
+    if (kMany && p.products > 1) {
+      if (i >= (int)list[0]) return false;
+      g = list[1 + i] >> 28;
+      tile = list[1 + i] & 0x0FFFFFFF;
+    } else if (tile >= p.product[0].tiles_m * p.product[0].tiles_n) {
+      return false;
+    }
+    t = pair_tile(tile, p.product[g].tiles_m, p.product[g].tiles_n);
+    return true;
+  };
 
   if (warp == 0) {
     // ---- loads: both CTAs fill their own stages; the bytes are counted on the even CTA's barriers
     {
       const bool elected = ptx::elect_one();
-      // rows along N come in boxes of 64, the second of which may be used in part
-      const uint32_t b_bytes = p.b_mn && half_n > 64 ? kStageOperand : half_n * 128;
       uint32_t it = 0;
       bool ok = true;
-      for (int tile = first; ok && tile < tiles; tile += step) {
-        const PairTile t = pair_tile(tile, p.tiles_m, p.tiles_n);
+      int g;
+      PairTile t;
+      for (int i = 0; ok && tile_at(i, g, t); ++i) {
+        const FdmoePairProduct& pr = p.product[g];
+        const int half_n = pr.tile_n >> 1;  // rows of B per CTA; gated: columns of each projection
+        const int kb0 = pr.kblocks * (int)part / split, kb1 = pr.kblocks * ((int)part + 1) / split;
+        // rows along N come in boxes of 64, the second of which may be used in part
+        const uint32_t b_bytes = pr.b_mn && half_n > 64 ? kStageOperand : half_n * 128;
         const int ax = t.m * 256 + (int)rank * 128;
-        const int bx = kGated ? t.n * half_n + (int)rank * p.up_row : t.n * p.tile_n + (int)rank * half_n;
+        const int bx = kGated ? t.n * half_n + (int)rank * p.up_row : t.n * pr.tile_n + (int)rank * half_n;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % S::kStages;
           const uint32_t ph = (it / S::kStages) & 1;
@@ -252,8 +294,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
           const uint32_t sa = ptx::smem_u32(stages + s * 2 * kStageOperand), sb = sa + kStageOperand;
           if (MX4) {
             // 128 bytes of a row are 256 elements
-            ptx::tma_load_2d_pair(sa, &p.a, bar, kb * 128, ax);
-            ptx::tma_load_2d_pair(sb, &p.b, bar, kb * 128, bx);
+            ptx::tma_load_2d_pair(sa, &pr.a, bar, kb * 128, ax);
+            ptx::tma_load_2d_pair(sb, &pr.b, bar, kb * 128, bx);
             const uint32_t sf = ptx::smem_u32(scales + s * S::kScales);
             ptx::tma_load_2d_pair(sf, &p.sfa, bar, 0, (t.m * 2 + (int)rank) * p.sf_chunks + kb * 2);
             // both CTAs need the scales of all 256 rows of B
@@ -261,17 +303,17 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
             ptx::tma_load_2d_pair(sf + 2 * kScaleBlock, &p.sfb, bar, 0, b0 * p.sf_chunks + kb * 2);
             ptx::tma_load_2d_pair(sf + 4 * kScaleBlock, &p.sfb, bar, 0, b1 * p.sf_chunks + kb * 2);
           } else {
-            if (p.a_mn) {
-              ptx::tma_load_2d_pair(sa, &p.a, bar, ax, kb * 64);
-              ptx::tma_load_2d_pair(sa + 8192, &p.a, bar, ax + 64, kb * 64);
+            if (pr.a_mn) {
+              ptx::tma_load_2d_pair(sa, &pr.a, bar, ax, kb * 64);
+              ptx::tma_load_2d_pair(sa + 8192, &pr.a, bar, ax + 64, kb * 64);
             } else {
-              ptx::tma_load_2d_pair(sa, &p.a, bar, kb * 64, ax);
+              ptx::tma_load_2d_pair(sa, &pr.a, bar, kb * 64, ax);
             }
-            if (p.b_mn) {
-              ptx::tma_load_2d_pair(sb, &p.b, bar, bx, kb * 64);
-              if (half_n > 64) ptx::tma_load_2d_pair(sb + 8192, &p.b, bar, bx + 64, kb * 64);
+            if (pr.b_mn) {
+              ptx::tma_load_2d_pair(sb, &pr.b, bar, bx, kb * 64);
+              if (half_n > 64) ptx::tma_load_2d_pair(sb + 8192, &pr.b, bar, bx + 64, kb * 64);
             } else {
-              ptx::tma_load_2d_pair(sb, &p.b, bar, kb * 64, bx);
+              ptx::tma_load_2d_pair(sb, &pr.b, bar, kb * 64, bx);
             }
           }
         }
@@ -281,13 +323,17 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     // ---- MMAs: one thread of the even CTA
     if (rank == 0) {
       const bool elected = ptx::elect_one();
-      const uint32_t idesc = ptx::make_idesc_f16(256, p.tile_n, BF16, p.a_mn, p.b_mn);
-      // 16 k further: 32 bytes along a row, or 16 rows of 128 bytes
-      const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
-      const uint32_t a_lead = p.a_mn ? 8192 : 16, b_lead = p.b_mn ? 8192 : 16;
-      uint32_t it = 0, n = 0;
+      uint32_t it = 0;
       bool ok = true;
-      for (int tile = first; ok && tile < tiles; tile += step, ++n) {
+      int g;
+      PairTile t;
+      for (int n = 0; ok && tile_at(n, g, t); ++n) {
+        const FdmoePairProduct& pr = p.product[g];
+        const int kb0 = pr.kblocks * (int)part / split, kb1 = pr.kblocks * ((int)part + 1) / split;
+        const uint32_t idesc = ptx::make_idesc_f16(256, pr.tile_n, BF16, pr.a_mn, pr.b_mn);
+        // 16 k further: 32 bytes along a row, or 16 rows of 128 bytes
+        const uint32_t a_step = pr.a_mn ? 2048 >> 4 : 32 >> 4, b_step = pr.b_mn ? 2048 >> 4 : 32 >> 4;
+        const uint32_t a_lead = pr.a_mn ? 8192 : 16, b_lead = pr.b_mn ? 8192 : 16;
         const int acc = n % S::kAccs;
         const uint32_t aph = (n / S::kAccs) & 1;
         if (!wt.wait(acc_empty + acc, aph ^ 1, FDMOE_DENSE_TIMEOUT_ACC)) break;
@@ -334,32 +380,34 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     const int w = warp - 4, quad = warp & 3, half = w >> 2;
     uint8_t* buf = staging + w * S::kStaging;
     const uint32_t sbuf = ptx::smem_u32(buf);
-    const int tile_cols = kGated ? half_n : p.tile_n;
     // This warp's groups of columns, a box wide: the first, and the distance to the next (of all pairs' and halves').
     constexpr int kGroup = kF32 ? 32 : 64;
     constexpr int kMost = (kGated ? 128 : 256) / kGroup / 2;  // groups of a warp
-    const int groups = tile_cols / kGroup, first_group = half * split + (int)part, group_step = 2 * split;
+    const int first_group = half * split + (int)part, group_step = 2 * split;
     // Gradient: the boxes first take the upper halves of g and u of a group of columns, which dg and du then replace;
     // the lower bytes of this lane's row come straight into registers.
     uint32_t gu_count = 0;
     uint4 lower[8];
     auto fetch_gu = [&](const PairTile& t, int c) {
-      const int row = t.m * 256 + (int)rank * 128 + quad * 32 + lane, col = t.n * tile_cols + c * 64;
-      const uint16_t* at = static_cast<const uint16_t*>(p.lower) + (int64_t)row * p.cols + col;
+      const FdmoePairProduct& pr = p.product[0];
+      const int row = t.m * 256 + (int)rank * 128 + quad * 32 + lane, col = t.n * pr.tile_n + c * 64;
+      const uint16_t* at = static_cast<const uint16_t*>(p.lower) + (int64_t)row * pr.cols + col;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        lower[j] = row < p.rows && col + 8 * j < p.cols ? __ldg(reinterpret_cast<const uint4*>(at) + j) : make_uint4(0, 0, 0, 0);
+        lower[j] = row < pr.rows && col + 8 * j < pr.cols ? __ldg(reinterpret_cast<const uint4*>(at) + j) : make_uint4(0, 0, 0, 0);
       if (elected) {
         ptx::bulk_wait_group_read0();
         ptx::mbar_expect_tx(gu_full + w, 8192);
-        const int x = t.n * tile_cols + c * 64, y = t.m * 256 + (int)rank * 128 + quad * 32;
+        const int x = t.n * pr.tile_n + c * 64, y = t.m * 256 + (int)rank * 128 + quad * 32;
         ptx::tma_load_2d(buf, &p.gu[0], gu_full + w, x, y);
         ptx::tma_load_2d(buf + 4096, &p.gu[1], gu_full + w, x, y);
       }
     };
-    uint32_t n = 0;
-    for (int tile = first; tile < tiles; tile += step, ++n) {
-      const PairTile t = pair_tile(tile, p.tiles_m, p.tiles_n);
+    int g;
+    PairTile t;
+    for (int n = 0; tile_at(n, g, t); ++n) {
+      const FdmoePairProduct& pr = p.product[g];
+      const int half_n = pr.tile_n >> 1, tile_cols = kGated ? half_n : pr.tile_n, groups = tile_cols / kGroup;
       const int acc = n % S::kAccs;
       if constexpr (EPI == FDMOE_EPI_GATED_GRAD)
         if (first_group < groups) fetch_gu(t, first_group);
@@ -370,7 +418,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       if (split > 1) {
         // the cluster's only tile: the partial sums go where the stages were, [column / 4][row][4]
         if (done)
-          for (int c = half; c < p.tile_n >> 5; c += 2) {
+          for (int c = half; c < pr.tile_n >> 5; c += 2) {
             uint32_t v[32];
             ptx::tmem_ld_32x32(d + c * 32, v);
             ptx::tmem_ld_wait();
@@ -420,7 +468,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       const int col0 = t.n * tile_cols;
       // Sends box b, which all lanes have written, to columns from `col` on of result `map`.
       auto send = [&](int map, int b, int col) {
-        if (elected && row0 < p.rows && col < p.cols) ptx::tma_store_2d(&p.out[map], sbuf + b * 4096, col, row0);
+        if (elected && row0 < pr.rows && col < pr.cols) ptx::tma_store_2d(&pr.out[map], sbuf + b * 4096, col, row0);
       };
       if constexpr (EPI == FDMOE_EPI_HALF) {
         // All of the warp's columns are read, rounded and the accumulator given back before the first is stored.
@@ -538,8 +586,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
               if constexpr (EPI == FDMOE_EPI_GATED_SAVE) {
                 stage16(buf + 4096, lane, i * 4 + j, gw[0], gw[1], gw[2], gw[3]);
                 const int row = row0 + lane, col = col0 + c * 64 + i * 32 + j * 8;  // columns come in eights
-                if (row < p.rows && col < p.cols)
-                  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.lower) + (int64_t)row * p.cols + col) =
+                if (row < pr.rows && col < pr.cols)
+                  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.lower) + (int64_t)row * pr.cols + col) =
                       make_uint4(lower[0], lower[1], lower[2], lower[3]);
               }
             }

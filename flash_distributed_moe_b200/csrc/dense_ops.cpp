@@ -145,35 +145,80 @@ int OperandMap(const Call& c, FdmoeTensorMap* out, const Operand& o, int box_row
   return MakeMap(c, out, o.base, 2, o.rows, o.cols, o.cols * 2, 64, o.mn ? 64 : box_rows);
 }
 
-// The shape of a launch of the pair kernel; returns its number of clusters.
+int KBlocks(int64_t k, bool mx4) { return (int)((k + (mx4 ? FDMOE_MX4_STAGE_K : 64) - 1) / (mx4 ? FDMOE_MX4_STAGE_K : 64)); }
+
+// A launch of the pair kernel with one product of this shape; returns its number of clusters.
 int PairShape(FdmoePairParams& p, const Call& c, int64_t rows, int64_t cols, int64_t k, bool gated, bool mx4) {
-  const int stage_k = mx4 ? FDMOE_MX4_STAGE_K : 64;
+  FdmoePairProduct& q = p.product[0];
   p.status = c.status;
   p.timeout_ns = c.timeout_ns;
-  p.rows = (int32_t)rows;
-  p.cols = (int32_t)cols;
-  p.kblocks = (int32_t)((k + stage_k - 1) / stage_k);
-  const fdmoe::PairPlan plan = fdmoe::MakePairPlan(rows, cols, p.kblocks, gated, mx4, *c.slots);
-  p.tile_n = plan.tile_n;
+  p.products = 1;
+  q.rows = (int32_t)rows;
+  q.cols = (int32_t)cols;
+  q.kblocks = KBlocks(k, mx4);
+  const fdmoe::PairPlan plan = fdmoe::MakePairPlan(rows, cols, q.kblocks, gated, mx4, *c.slots);
   p.split = plan.split;
-  p.tiles_m = plan.tiles_m;
-  p.tiles_n = plan.tiles_n;
+  q.tile_n = plan.tile_n;
+  q.tiles_m = plan.tiles_m;
+  q.tiles_n = plan.tiles_n;
   return plan.clusters;
 }
 
-// out[rows, cols] = A B^T, both given as stored.
-int PairProduct(const Call& c, const Operand& a, const Operand& b, void* out, bool bf16) {
+// out = A B^T, both operands given as stored.
+struct Product {
+  Operand a, b;
+  void* out;
+  int64_t rows() const { return a.mn ? a.cols : a.rows; }
+  int64_t cols() const { return b.mn ? b.cols : b.rows; }
+  int64_t k() const { return a.mn ? a.rows : a.cols; }
+};
+
+int ProductMaps(const Call& c, FdmoePairProduct& q, const Product& w) {
+  q.a_mn = w.a.mn;
+  q.b_mn = w.b.mn;
+  DENSE_TRY(OperandMap(c, &q.a, w.a, 128));
+  DENSE_TRY(OperandMap(c, &q.b, w.b, q.tile_n / 2));
+  return MakeMap(c, &q.out[0], w.out, 2, w.rows(), w.cols(), w.cols() * 2, 64, 32);
+}
+
+int PairProduct(const Call& c, const Product& w, bool bf16) {
   FdmoePairParams p;
   memset(&p, 0, sizeof(p));
-  const int64_t rows = a.mn ? a.cols : a.rows, cols = b.mn ? b.cols : b.rows, k = a.mn ? a.rows : a.cols;
-  const int clusters = PairShape(p, c, rows, cols, k, false, false);
-  DENSE_TRY(OperandMap(c, &p.a, a, 128));
-  DENSE_TRY(OperandMap(c, &p.b, b, p.tile_n / 2));
-  DENSE_TRY(MakeMap(c, &p.out[0], out, 2, rows, cols, cols * 2, 64, 32));
-  p.a_mn = a.mn;
-  p.b_mn = b.mn;
+  const int clusters = PairShape(p, c, w.rows(), w.cols(), w.k(), false, false);
+  DENSE_TRY(ProductMaps(c, p.product[0], w));
   p.bf16 = bf16;
   return fdmoe_pair_launch(&p, FDMOE_EPI_HALF, 0, clusters, c.stream);
+}
+
+// Up to three products that do not depend on each other, in one launch if that is faster.
+int PairProducts(const Call& c, const Product* w, int n, bool bf16) {
+  fdmoe::ManyShape shape[FDMOE_PAIR_PRODUCTS];
+  for (int i = 0; i < n; ++i) shape[i] = {w[i].rows(), w[i].cols(), KBlocks(w[i].k(), false)};
+  const fdmoe::ManyPlan m = fdmoe::MakeManyPlan(shape, n, *c.slots);
+  if (!m.use) {
+    for (int i = 0; i < n; ++i) DENSE_TRY(PairProduct(c, w[i], bf16));
+    return 0;
+  }
+  FdmoePairParams p;
+  memset(&p, 0, sizeof(p));
+  p.status = c.status;
+  p.timeout_ns = c.timeout_ns;
+  p.products = n;
+  p.split = 1;
+  p.bf16 = bf16;
+  for (int i = 0; i < n; ++i) {
+    const int x = m.order[i];
+    FdmoePairProduct& q = p.product[i];
+    q.rows = (int32_t)shape[x].rows;
+    q.cols = (int32_t)shape[x].cols;
+    q.kblocks = shape[x].kblocks;
+    q.tile_n = m.tile_n[x];
+    q.tiles_m = (int32_t)((shape[x].rows + FDMOE_PAIR_TILE - 1) / FDMOE_PAIR_TILE);
+    q.tiles_n = (int32_t)((shape[x].cols + q.tile_n - 1) / q.tile_n);
+    DENSE_TRY(ProductMaps(c, q, w[x]));
+  }
+  memcpy(p.count, m.count, sizeof(p.count));
+  return fdmoe_pair_launch(&p, FDMOE_EPI_HALF, 0, m.pairs, c.stream);
 }
 
 // out[tokens, rows] = x w^T (gated: silu(x w[:rows]^T) * (x w[rows:]^T)) for few tokens.
@@ -221,13 +266,14 @@ int GatedProduct(const Call& c, const void* x, const void* w13, void* h, const S
   FdmoePairParams p;
   memset(&p, 0, sizeof(p));
   const int clusters = PairShape(p, c, T, I, H, true, false);
-  DENSE_TRY(MakeMap(c, &p.a, x, 2, T, H, H * 2, 64, 128));
-  DENSE_TRY(MakeMap(c, &p.b, w13, 2, 2 * I, H, H * 2, 64, p.tile_n / 2));
-  DENSE_TRY(MakeMap(c, &p.out[0], h, 2, T, I, I * 2, 64, 32));
+  FdmoePairProduct& q = p.product[0];
+  DENSE_TRY(MakeMap(c, &q.a, x, 2, T, H, H * 2, 64, 128));
+  DENSE_TRY(MakeMap(c, &q.b, w13, 2, 2 * I, H, H * 2, 64, q.tile_n / 2));
+  DENSE_TRY(MakeMap(c, &q.out[0], h, 2, T, I, I * 2, 64, 32));
   if (saved.gu) {
     // two matrices side by side: what a tile has beyond column I of the gate projection is not stored
-    DENSE_TRY(MakeMap(c, &p.out[1], saved.gu, 2, T, I, I * 4, 64, 32));
-    DENSE_TRY(MakeMap(c, &p.out[2], saved.gu + I * 2, 2, T, I, I * 4, 64, 32));
+    DENSE_TRY(MakeMap(c, &q.out[1], saved.gu, 2, T, I, I * 4, 64, 32));
+    DENSE_TRY(MakeMap(c, &q.out[2], saved.gu + I * 2, 2, T, I, I * 4, 64, 32));
     p.lower = saved.lower;
   }
   p.up_row = (int32_t)I;
@@ -242,14 +288,15 @@ int GatedGradient(const Call& c, const void* dy, const void* w2, const Saved& sa
   FdmoePairParams p;
   memset(&p, 0, sizeof(p));
   const int clusters = PairShape(p, c, T, I, H, false, false);
-  DENSE_TRY(MakeMap(c, &p.a, dy, 2, T, H, H * 2, 64, 128));
-  DENSE_TRY(MakeMap(c, &p.b, w2, 2, H, I, I * 2, 64, 64));
+  FdmoePairProduct& q = p.product[0];
+  DENSE_TRY(MakeMap(c, &q.a, dy, 2, T, H, H * 2, 64, 128));
+  DENSE_TRY(MakeMap(c, &q.b, w2, 2, H, I, I * 2, 64, 64));
   for (int i = 0; i < 2; ++i) {
     DENSE_TRY(MakeMap(c, &p.gu[i], saved.gu + i * I * 2, 2, T, I, I * 4, 64, 32));
-    DENSE_TRY(MakeMap(c, &p.out[i], static_cast<uint8_t*>(dgu) + i * I * 2, 2, T, I, I * 4, 64, 32));
+    DENSE_TRY(MakeMap(c, &q.out[i], static_cast<uint8_t*>(dgu) + i * I * 2, 2, T, I, I * 4, 64, 32));
   }
   p.lower = saved.lower;
-  p.b_mn = 1;
+  q.b_mn = 1;
   p.bf16 = bf16;
   return fdmoe_pair_launch(&p, FDMOE_EPI_GATED_GRAD, 0, clusters, c.stream);
 }
@@ -302,10 +349,10 @@ int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, 
   FdmoePairParams p;
   memset(&p, 0, sizeof(p));
   const int clusters = PairShape(p, c, tokens, rows, k, gated, true);
-  DENSE_TRY(Mx4Maps(c, &p.a, &p.sfa, a, k, 128));
-  DENSE_TRY(Mx4Maps(c, &p.b, &p.sfb, b, k, 128));
+  DENSE_TRY(Mx4Maps(c, &p.product[0].a, &p.sfa, a, k, 128));
+  DENSE_TRY(Mx4Maps(c, &p.product[0].b, &p.sfb, b, k, 128));
   const int size = dtype == kF32 ? 4 : 2;
-  DENSE_TRY(MakeMap(c, &p.out[0], out, size, tokens, rows, rows * size, 128 / size, 32));
+  DENSE_TRY(MakeMap(c, &p.product[0].out[0], out, size, tokens, rows, rows * size, 128 / size, 32));
   p.up_row = (int32_t)rows;
   p.sf_chunks = chunks;
   p.sf_up_block = up_block;
@@ -380,7 +427,7 @@ static int FfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w
   void* h = savedFor ? saved.h : workspace;
   DENSE_TRY(GatedProduct(c, x, w13, h, saved, T, H, I, bf16, stall));
   if (stall) return 0;
-  return PairProduct(c, {h, T, I, false}, {w2, H, I, false}, y, bf16);
+  return PairProduct(c, {{h, T, I, false}, {w2, H, I, false}, y}, bf16);
 }
 
 extern "C" int FlashMoeFfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y,
@@ -414,10 +461,12 @@ extern "C" int FlashMoeFfnBackward(const FlashMoeFfnConfig* cfg, const void* dy,
   const Saved saved(savedBy, T, I);
   void* dgu = workspace;
   if (dx || dw13) DENSE_TRY(GatedGradient(c, dy, w2, saved, dgu, T, H, I, bf16));
-  if (dx) DENSE_TRY(PairProduct(c, {dgu, T, 2 * I, false}, {w13, 2 * I, H, true}, dx, bf16));
-  if (dw13) DENSE_TRY(PairProduct(c, {dgu, T, 2 * I, true}, {x, T, H, true}, dw13, bf16));
-  if (dw2) DENSE_TRY(PairProduct(c, {dy, T, H, true}, {saved.h, T, I, true}, dw2, bf16));
-  return 0;
+  Product work[FDMOE_PAIR_PRODUCTS];
+  int n = 0;
+  if (dx) work[n++] = {{dgu, T, 2 * I, false}, {w13, 2 * I, H, true}, dx};
+  if (dw13) work[n++] = {{dgu, T, 2 * I, true}, {x, T, H, true}, dw13};
+  if (dw2) work[n++] = {{dy, T, H, true}, {saved.h, T, I, true}, dw2};
+  return PairProducts(c, work, n, bf16);
 }
 
 extern "C" size_t FlashMoeMx4ScaleBytes(int64_t batch, int64_t rows, int64_t cols) {

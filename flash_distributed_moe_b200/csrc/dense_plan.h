@@ -69,7 +69,10 @@ inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, 
 
 struct PairPlan {
   int tile_n, split, tiles_m, tiles_n, clusters;
+  double cycles;  // estimated
 };
+
+inline double BlockCycles(int tile_n) { return tile_n == 256 ? 520 : tile_n == 192 ? 455 : 365; }
 
 // `cols`: of the result; `kblocks` stages of k.  Time in cycles: the waves of tiles, each its k blocks (about 520,
 // 455 and 365 cycles at widths of 256, 192 and 128) and once per launch, or per cluster where pairs share a tile, its
@@ -89,14 +92,98 @@ inline PairPlan MakePairPlan(int64_t rows, int64_t cols, int kblocks, bool gated
       p.tiles_n = (int)((cols + tile_cols - 1) / tile_cols);
       const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, slots = std::max(1, dev.pair[split]);
       const double waves = (double)((tiles + slots - 1) / slots);
-      const double block = tile_n == 256 ? 520 : tile_n == 192 ? 455 : 365;
-      const double k = (double)((kblocks + split - 1) / split) * block;
+      const double k = (double)((kblocks + split - 1) / split) * BlockCycles(tile_n);
       const double exchange = (double)tile_n * 512 * (split - 1) / split / 14;
       const double t = split == 1 ? waves * k + 3000 : waves * (k + 3500 + exchange);
       p.clusters = (int)(split == 1 ? std::min(tiles, slots) : tiles);
+      p.cycles = t;
       if (best_time == 0 || t < best_time) best = p, best_time = t;
     }
   return best;
+}
+
+// Several products in one launch of the pair kernel: their tiles, the longest first, fill the pairs evenly, where
+// launches of their own would each end with a wave that is partly empty.
+struct ManyShape {
+  int64_t rows, cols;
+  int kblocks;
+};
+struct ManyPlan {
+  bool use;              // better than a launch for each
+  int pairs;
+  int order[FDMOE_PAIR_PRODUCTS];   // the products by the length of their tiles
+  int tile_n[FDMOE_PAIR_PRODUCTS];  // of each product
+  uint8_t count[FDMOE_PAIR_PRODUCTS][FDMOE_PAIR_MOST];  // tiles of order[i] for each pair
+};
+
+inline ManyPlan MakeManyPlan(const ManyShape* shape, int n, const DeviceSlots& dev) {
+  ManyPlan m = {};
+  m.pairs = std::min(dev.pair[1], (int)FDMOE_PAIR_MOST);
+  if (n < 2 || m.pairs < 1) return m;
+  double apart = 0;  // launches of their own
+  for (int i = 0; i < n; ++i) {
+    const PairPlan p = MakePairPlan(shape[i].rows, shape[i].cols, shape[i].kblocks, false, false, dev);
+    apart += p.cycles + 4000;
+  }
+  auto tiles = [&](int i, int tile_n) {
+    return (double)((shape[i].rows + FDMOE_PAIR_TILE - 1) / FDMOE_PAIR_TILE) * ((shape[i].cols + tile_n - 1) / tile_n);
+  };
+  auto length = [&](int i, int tile_n) { return shape[i].kblocks * BlockCycles(tile_n) + 600; };
+  // Widths: every choice, by the even share and the longest tile.
+  const int widths[3] = {256, 192, 128};
+  int choices = 1;
+  for (int i = 0; i < n; ++i) choices *= 3;
+  double best = 0;
+  for (int c = 0; c < choices; ++c) {
+    double total = 0, most = 0, least = 0;
+    for (int i = 0, d = c; i < n; ++i, d /= 3) {
+      const double l = length(i, widths[d % 3]);
+      total += l * tiles(i, widths[d % 3]);
+      most = std::max(most, l);
+      least = least == 0 ? l : std::min(least, l);
+    }
+    const double t = std::max(total / m.pairs + least / 2, most);
+    if (c == 0 || t < best) {
+      best = t;
+      for (int i = 0, d = c; i < n; ++i, d /= 3) m.tile_n[i] = widths[d % 3];
+    }
+  }
+  for (int i = 0; i < n; ++i) m.order[i] = i;
+  std::sort(m.order, m.order + n, [&](int x, int y) { return length(x, m.tile_n[x]) > length(y, m.tile_n[y]); });
+  // Deal out: raise a level under which every pair is filled with whole tiles, until all tiles have a place.
+  double load[FDMOE_PAIR_MOST] = {};
+  int held[FDMOE_PAIR_MOST] = {};
+  for (int i = 0; i < n; ++i) {
+    const int x = m.order[i];
+    const double l = length(x, m.tile_n[x]), want = tiles(x, m.tile_n[x]);
+    if (want > (double)m.pairs * (FDMOE_PAIR_LIST - 3)) return m;
+    double low = 0, high = want * l;
+    for (int p = 0; p < m.pairs; ++p) high = std::max(high, load[p] + (want / m.pairs + 1) * l);
+    auto fits = [&](double level) {
+      double f = 0;
+      for (int p = 0; p < m.pairs; ++p)
+        if (level > load[p]) f += (int)((level - load[p]) / l);
+      return f;
+    };
+    for (int k = 0; k < 24; ++k) {
+      const double mid = 0.5 * (low + high);
+      (fits(mid) >= want ? high : low) = mid;
+    }
+    int64_t over = -(int64_t)want;
+    int got[FDMOE_PAIR_MOST];
+    for (int p = 0; p < m.pairs; ++p) over += got[p] = high > load[p] ? (int)((high - load[p]) / l) : 0;
+    for (int p = m.pairs - 1; p >= 0 && over > 0; --p)  // those that reach the level itself give one back
+      if (got[p] > 0 && load[p] + got[p] * l > high - l) --got[p], --over;
+    if (over != 0) return m;
+    for (int p = 0; p < m.pairs; ++p) {
+      load[p] += got[p] * l;
+      held[p] += got[p];
+      if (got[p] > 255 || held[p] > FDMOE_PAIR_LIST - 3) return m;
+      m.count[i][p] = (uint8_t)got[p];
+    }
+  }
+  m.use = *std::max_element(load, load + m.pairs) + 3000 < apart;
+  return m;
 }
 
 // Whether the streaming kernel takes a product instead of the pair kernel.  Whole block, streaming and pair kernels:

@@ -13,6 +13,9 @@ extern "C" {
 enum {
   FDMOE_PAIR_TILE = 256,      // rows of a tile of the pair kernel, and most columns
   FDMOE_PAIR_SPLIT = 4,       // most pairs that share the k axis of a tile of the pair kernel
+  FDMOE_PAIR_PRODUCTS = 3,    // most products that a launch of the pair kernel works on
+  FDMOE_PAIR_MOST = 96,       // most pairs of such a launch
+  FDMOE_PAIR_LIST = 64,       // most tiles of a pair in it
   FDMOE_STREAM_ROWS = 128,    // weight rows of a tile of the streaming kernel
   FDMOE_STREAM_TOKENS = 128,  // most tokens of a tile of the streaming kernel
   FDMOE_STREAM_SPLIT = 8,     // most CTAs that share the k axis of a tile of the streaming kernel
@@ -39,25 +42,32 @@ enum {
   FDMOE_DENSE_TIMEOUT_DONE = 24,   // an accumulator was not completed
 };
 
+// One product of a launch of the pair kernel.
 typedef struct {
   FdmoeTensorMap a, b;        // operands; `a` gives the rows of the result, `b` its columns
-  FdmoeTensorMap sfa, sfb;    // their scales (4-bit operands)
   FdmoeTensorMap out[3];      // results: the tile | h | h, upper halves of gate, up | d gate, d up
+  int32_t rows, cols;         // of the result
+  int32_t tiles_m, tiles_n;
+  int32_t tile_n;             // 256, 192 or 128 (4-bit operands: 256)
+  int32_t kblocks;
+  int32_t a_mn, b_mn;         // operand stored with its rows along M (N) instead of along K
+} FdmoePairProduct;
+
+typedef struct {
+  FdmoePairProduct product[FDMOE_PAIR_PRODUCTS];
+  FdmoeTensorMap sfa, sfb;    // scales of 4-bit operands
   FdmoeTensorMap gu[2];       // upper halves of gate and up projections (FDMOE_EPI_GATED_GRAD)
   void* lower;                // [rows, cols] lower bytes of both (FDMOE_EPI_GATED_SAVE and FDMOE_EPI_GATED_GRAD)
   uint32_t* status;
   uint64_t timeout_ns;
-  int32_t rows, cols;         // of the result
-  int32_t tiles_m, tiles_n;
-  int32_t tile_n;             // 256, 192 or 128 (4-bit operands: 256)
+  int32_t products;           // above 1: FDMOE_EPI_HALF, `split` 1, tiles dealt out by `count`
   int32_t split;              // 1, 2 or 4 pairs per tile; above 1 a launch has a cluster per tile
-  int32_t kblocks;
-  int32_t a_mn, b_mn;         // operand stored with its rows along M (N) instead of along K
   int32_t up_row;             // row of `b` at which the up projection starts (gated)
   int32_t sf_chunks;          // 512-byte blocks of scales per 128 rows
   int32_t sf_up_block;        // block of 128 rows at which the up projection's scales start
   int32_t bf16;               // 16-bit operands and results are bf16, otherwise fp16
   int32_t stall;              // test hook: nothing is loaded, every wait runs out
+  uint8_t count[FDMOE_PAIR_PRODUCTS][FDMOE_PAIR_MOST];  // tiles of each product for each pair
 } FdmoePairParams;
 
 typedef struct {

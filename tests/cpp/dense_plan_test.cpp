@@ -2,6 +2,7 @@
 // split of the k axis stay within what the kernel and the hardware allow.
 #include <cstdio>
 #include <cstdlib>
+#include <vector>
 
 #include "../../flash_distributed_moe_b200/csrc/dense_plan.h"
 
@@ -52,6 +53,41 @@ int main() {
               CHECK(q.tiles_m * 256 >= tokens && q.tiles_n * cols_tile >= rows && q.clusters >= 1);
               CHECK(q.split == 1 ? q.clusters <= q.tiles_m * q.tiles_n : q.clusters == q.tiles_m * q.tiles_n);
             }
+  // Several products in one launch: every tile is dealt out once, in the order in which the kernel lists them.
+  const int dims[] = {8, 72, 256, 777, 1000, 2048, 4096, 12288};
+  for (int tokens : dims)
+    for (int rows : dims)
+      for (int kb : dims)
+        for (int n = 2; n <= 3; ++n) {
+          const int gated = n, mx4 = 0;  // for the message
+          DeviceSlots dev = {};
+          dev.pair[1] = 74, dev.pair[2] = 33, dev.pair[4] = 15;
+          const int T = tokens, H = rows, I = kb;
+          const ManyShape shape[3] = {{T, H, (2 * I + 63) / 64}, {2 * I, H, (T + 63) / 64}, {H, I, (T + 63) / 64}};
+          const ManyPlan m = MakeManyPlan(shape, n, dev);
+          if (!m.use) continue;
+          CHECK(m.pairs == 74);
+          std::vector<int> held(m.pairs, 0);
+          for (int i = 0; i < n; ++i) {
+            const int x = m.order[i];
+            CHECK(m.tile_n[x] == 256 || m.tile_n[x] == 192 || m.tile_n[x] == 128);
+            const long tiles = ((shape[x].rows + 255) / 256) * ((shape[x].cols + m.tile_n[x] - 1) / m.tile_n[x]);
+            std::vector<char> seen(tiles, 0);
+            long base = 0;
+            for (int r = 0; r < 256; ++r) {
+              long all = 0;
+              for (int p = 0; p < m.pairs; ++p)
+                if (m.count[i][p] > r) {
+                  CHECK(base + all < tiles && !seen[base + all]);
+                  seen[base + all] = 1;
+                  ++all, ++held[p];
+                }
+              base += all;
+            }
+            CHECK(base == tiles);
+          }
+          for (int p = 0; p < m.pairs; ++p) CHECK(held[p] <= FDMOE_PAIR_LIST - 3);
+        }
   {
     const int rows = 0, tokens = 0, kb = 0, gated = 0, mx4 = 0;
     CHECK(ScaleChunks(32) == 2 && ScaleChunks(256) == 2 && ScaleChunks(288) == 4);
