@@ -26,45 +26,53 @@ struct DeviceSlots {
 };
 
 // `rows` weight rows (gated: of each projection), `tokens` >= 1, `kblocks` stages of k in all.
+//
+// Time in cycles.  A k block takes as long as its MMAs' issue, or as the weights of `active` CTAs do at the rate at which
+// their stages in flight are filled, at most the memory's 3500 bytes per cycle; a wave has a beginning and an end.  Two
+// CTAs per SM hide each other's beginning and end and issue at the same time, but have half the stages each.  Cold
+// weights, CTAs per tile of the two products of a block: 1 token of 2048 x 6144 22.7 us with 2 and 8, 21.3 with 4 and 8;
+// 32 tokens of 4096 x 12288 63.5 with 1 and 6, 58.9 with 2 and 8, 63.6 with 2 and 4.
 inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, bool mx4, const DeviceSlots& dev) {
-  StreamPlan s;
+  StreamPlan best = {};
+  double best_time = 0;
   const int parts = gated ? 2 : 1;
-  s.token_tiles = (tokens + FDMOE_STREAM_TOKENS - 1) / FDMOE_STREAM_TOKENS;
-  s.tile_tokens = s.token_tiles > 1 ? FDMOE_STREAM_TOKENS : RoundUp(tokens, 16);
-  s.row_tiles = (rows + FDMOE_STREAM_ROWS - 1) / FDMOE_STREAM_ROWS;
-  const int stage = parts * 16384 + s.tile_tokens * 128 + (mx4 ? (parts + 1) * 1024 : 0);
-  // Partial sums, in the stages' place: groups of four tokens, the same number for every CTA of the cluster.
-  const int sums = (RoundUp(std::min(tokens, s.tile_tokens), 4) + 4 * (FDMOE_STREAM_SPLIT - 1)) * parts * 512;
-  // Two CTAs per SM hide each other's beginning and end, if three stages each are left.
-  s.per_sm = (kStreamSmemTwo - kStreamSlack) / stage >= 3 && sums <= kStreamSmemTwo - kStreamSlack ? 2 : 1;
-  const int room = (s.per_sm == 2 ? kStreamSmemTwo : kStreamSmemOne) - kStreamSlack;
-  s.stages = std::min(room / stage, (int)FDMOE_STREAM_STAGES);
-  const int scales = mx4 ? (parts + 1) * 8 : 0;  // TMEM columns per stage
-  if (scales) s.stages = std::min(s.stages, ((s.per_sm == 2 ? 256 : 512) - parts * s.tile_tokens) / scales);
-  // Time in cycles.  A k block takes as long as its MMAs' issue, or as the weights of `active` CTAs do at the rate at
-  // which their stages in flight are filled, at most the memory's 3500 bytes per cycle; a wave has a beginning and an
-  // end.  Whole block, cold weights, CTAs per tile of the two products: 1 token of 2048 x 6144 22.7 us with 2 and 8,
-  // 21.3 with 4 and 8; 32 tokens of 4096 x 12288 63.5 with 1 and 6, 58.9 with 2 and 8, 63.6 with 2 and 4.
-  const double weights = parts * (mx4 ? 16384 + 1024 : 16384), issue = mx4 ? 400 + 250 * parts : 300 + 150 * parts;
-  double best = 0;
-  s.split = 1;
-  for (int n = 1; n <= FDMOE_STREAM_SPLIT && n <= kblocks; ++n) {
-    const int64_t slots = std::max(1, s.per_sm == 2 ? dev.stream_two[n] : dev.stream_one[n]);
-    double t = (n > 1 ? 1000 : 0) + s.tile_tokens * parts * 20.0 / n;  // the exchange of partial sums, and the epilogue
-    int64_t clusters = (int64_t)s.row_tiles * s.token_tiles;
-    for (int wave = 0; clusters > 0 && wave < 64; ++wave, clusters -= slots) {
-      const double active = (double)std::min(clusters, slots) * n;
-      const double rate = std::min(3500.0, active * std::min(s.stages, (kblocks + n - 1) / n) * weights / 4000);
-      t += (double)((kblocks + n - 1) / n) * std::max(issue, active * weights / rate) + 5000;
+  for (int per_sm = 2; per_sm >= 1; --per_sm) {
+    StreamPlan s = {};
+    s.per_sm = per_sm;
+    s.token_tiles = (tokens + FDMOE_STREAM_TOKENS - 1) / FDMOE_STREAM_TOKENS;
+    s.tile_tokens = s.token_tiles > 1 ? FDMOE_STREAM_TOKENS : RoundUp(tokens, 16);
+    s.row_tiles = (rows + FDMOE_STREAM_ROWS - 1) / FDMOE_STREAM_ROWS;
+    const int stage = parts * 16384 + s.tile_tokens * 128 + (mx4 ? (parts + 1) * 1024 : 0);
+    const int room = (per_sm == 2 ? kStreamSmemTwo : kStreamSmemOne) - kStreamSlack;
+    // Partial sums, in the stages' place: groups of four tokens, the same number for every CTA of the cluster.
+    const int sums = (RoundUp(std::min(tokens, s.tile_tokens), 4) + 4 * (FDMOE_STREAM_SPLIT - 1)) * parts * 512;
+    const int scales = mx4 ? (parts + 1) * 8 : 0;  // TMEM columns per stage
+    int most = std::min(room / stage, (int)FDMOE_STREAM_STAGES);
+    if (scales) most = std::min(most, ((per_sm == 2 ? 256 : 512) - parts * s.tile_tokens) / scales);
+    if (per_sm == 2 && (most < 2 || sums > room || parts * s.tile_tokens > 256)) continue;
+    const double weights = parts * (mx4 ? 16384 + 1024 : 16384), issue = mx4 ? 400 + 250 * parts : 300 + 150 * parts;
+    for (int n = 1; n <= FDMOE_STREAM_SPLIT && n <= kblocks; ++n) {
+      const int64_t slots = std::max(1, per_sm == 2 ? dev.stream_two[n] : dev.stream_one[n]);
+      const int blocks = (kblocks + n - 1) / n;
+      double t = (n > 1 ? 600 + 200 * n : 0) + s.tile_tokens * parts * 20.0 / n;  // the exchange of partial sums, and the epilogue
+      int64_t clusters = (int64_t)s.row_tiles * s.token_tiles;
+      for (int wave = 0; clusters > 0 && wave < 64; ++wave, clusters -= slots) {
+        const double active = (double)std::min(clusters, slots) * n;
+        const double rate = std::min(3500.0, active * std::min(most, blocks) * weights / 4000);
+        t += blocks * std::max(issue, active * weights / rate) + 5000;
+      }
+      if (best_time != 0 && t >= best_time) continue;
+      best_time = t;
+      best = s;
+      best.split = n;
+      best.stages = std::min(most, blocks);
+      const int cols = parts * s.tile_tokens + best.stages * scales;
+      best.tmem_cols = 32;
+      while (best.tmem_cols < cols) best.tmem_cols *= 2;
+      best.smem = std::max(best.stages * stage, n > 1 ? sums : 0) + kStreamSlack;
     }
-    if (n == 1 || t < best) best = t, s.split = n;
   }
-  s.stages = std::min(s.stages, (kblocks + s.split - 1) / s.split);
-  const int cols = parts * s.tile_tokens + s.stages * scales;
-  s.tmem_cols = 32;
-  while (s.tmem_cols < cols) s.tmem_cols *= 2;
-  s.smem = std::max(s.stages * stage, sums) + kStreamSlack;
-  return s;
+  return best;
 }
 
 struct PairPlan {
