@@ -190,11 +190,40 @@ int PairProduct(const Call& c, const Product& w, bool bf16) {
   return fdmoe_pair_launch(&p, FDMOE_EPI_HALF, 0, clusters, c.stream);
 }
 
+// MakeManyPlan takes some ten microseconds; the plans of the last shapes are kept.
+void CachedManyPlan(const fdmoe::ManyShape* shape, int n, const fdmoe::DeviceSlots* slots, fdmoe::ManyPlan* out) {
+  struct Entry {
+    const fdmoe::DeviceSlots* slots = nullptr;  // of the device
+    int n = 0;
+    int64_t key[3 * FDMOE_PAIR_PRODUCTS];
+    fdmoe::ManyPlan plan;
+  };
+  static std::mutex mutex;
+  static Entry cache[32];
+  static int next = 0;
+  int64_t key[3 * FDMOE_PAIR_PRODUCTS] = {};
+  for (int i = 0; i < n; ++i) key[3 * i] = shape[i].rows, key[3 * i + 1] = shape[i].cols, key[3 * i + 2] = shape[i].kblocks;
+  std::lock_guard<std::mutex> lock(mutex);
+  for (const Entry& e : cache)
+    if (e.slots == slots && e.n == n && memcmp(e.key, key, sizeof(key)) == 0) {
+      *out = e.plan;
+      return;
+    }
+  Entry& e = cache[next];
+  next = (next + 1) % 32;
+  e.plan = fdmoe::MakeManyPlan(shape, n, *slots);
+  e.slots = slots;
+  e.n = n;
+  memcpy(e.key, key, sizeof(key));
+  *out = e.plan;
+}
+
 // Up to three products that do not depend on each other, in one launch if that is faster.
 int PairProducts(const Call& c, const Product* w, int n, bool bf16) {
   fdmoe::ManyShape shape[FDMOE_PAIR_PRODUCTS];
   for (int i = 0; i < n; ++i) shape[i] = {w[i].rows(), w[i].cols(), KBlocks(w[i].k(), false)};
-  const fdmoe::ManyPlan m = fdmoe::MakeManyPlan(shape, n, *c.slots);
+  fdmoe::ManyPlan m;
+  CachedManyPlan(shape, n, c.slots, &m);
   if (!m.use) {
     for (int i = 0; i < n; ++i) DENSE_TRY(PairProduct(c, w[i], bf16));
     return 0;

@@ -31,7 +31,7 @@ struct DeviceSlots {
 // their stages in flight are filled, at most the memory's 3500 bytes per cycle; a wave has a beginning and an end.  Two
 // CTAs per SM hide each other's beginning and end and issue at the same time, but have half the stages each.  Cold
 // weights, CTAs per tile of the two products of a block: 1 token of 2048 x 6144 22.7 us with 2 and 8, 21.3 with 4 and 8;
-// 32 tokens of 4096 x 12288 63.5 with 1 and 6, 58.9 with 2 and 8, 63.6 with 2 and 4.
+// 32 tokens of 4096 x 12288 63.5 with 1 and 6, 56.3 with 2 and 8, and 59.6 with one CTA per SM, 1 and 4.
 inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, bool mx4, const DeviceSlots& dev) {
   StreamPlan best = {};
   double best_time = 0;
@@ -50,15 +50,18 @@ inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, 
     int most = std::min(room / stage, (int)FDMOE_STREAM_STAGES);
     if (scales) most = std::min(most, ((per_sm == 2 ? 256 : 512) - parts * s.tile_tokens) / scales);
     if (per_sm == 2 && (most < 2 || sums > room || parts * s.tile_tokens > 256)) continue;
-    const double weights = parts * (mx4 ? 16384 + 1024 : 16384), issue = mx4 ? 400 + 250 * parts : 300 + 150 * parts;
+    const double weights = parts * (mx4 ? 16384 + 1024 : 16384), issue = mx4 ? 430 + 210 * parts : 380 + 160 * parts;
     for (int n = 1; n <= FDMOE_STREAM_SPLIT && n <= kblocks; ++n) {
-      const int64_t slots = std::max(1, per_sm == 2 ? dev.stream_two[n] : dev.stream_one[n]);
+      const int64_t slots = per_sm == 2 ? dev.stream_two[n] : dev.stream_one[n];
+      if (slots < 1) continue;  // the device cannot hold such a cluster
       const int blocks = (kblocks + n - 1) / n;
-      double t = (n > 1 ? 600 + 200 * n : 0) + s.tile_tokens * parts * 20.0 / n;  // the exchange of partial sums, and the epilogue
+      double t = per_sm == 1 ? 2000 : 0;  // the launches before and after it cannot overlap with it
+      // the partial sums' way through the cluster's shared memory at 14 bytes per cycle, and the epilogue
+      t += (n > 1 ? 600 + 200 * n : 0) + s.tile_tokens * parts * (36.0 * (n - 1) + 20.0) / n;
       int64_t clusters = (int64_t)s.row_tiles * s.token_tiles;
       for (int wave = 0; clusters > 0 && wave < 64; ++wave, clusters -= slots) {
         const double active = (double)std::min(clusters, slots) * n;
-        const double rate = std::min(3500.0, active * std::min(most, blocks) * weights / 4000);
+        const double rate = std::min(3500.0, active * most * weights / 4000);
         t += blocks * std::max(issue, active * weights / rate) + 5000;
       }
       if (best_time != 0 && t >= best_time) continue;
@@ -98,7 +101,8 @@ inline PairPlan MakePairPlan(int64_t rows, int64_t cols, int kblocks, bool gated
       p.tiles_m = (int)((rows + FDMOE_PAIR_TILE - 1) / FDMOE_PAIR_TILE);
       const int tile_cols = gated ? tile_n / 2 : tile_n;
       p.tiles_n = (int)((cols + tile_cols - 1) / tile_cols);
-      const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, slots = std::max(1, dev.pair[split]);
+      const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, slots = dev.pair[split];
+      if (slots < 1) continue;  // the device cannot hold such a cluster
       const double waves = (double)((tiles + slots - 1) / slots);
       const double k = (double)((kblocks + split - 1) / split) * BlockCycles(tile_n);
       const double exchange = (double)tile_n * 512 * (split - 1) / split / 14;

@@ -93,9 +93,9 @@ def gated_ffn(x: torch.Tensor, w13: Weight, w2: Weight) -> torch.Tensor:
     the gate and up projections of the tokens and silu(g) * u are kept for the backward pass, in 24 bits and in the dtype.  With Mx4Tensor
     weights (w13 [2, I, H], w2 [H, I]) x and the activations are quantised to 4 bits too, and there is no gradient.
 
-    A training step may be captured into a CUDA graph.  As with every torch operator, capture it while no eager graph
-    of the same leaves is alive (torch keeps the gradient accumulators of such a graph on its stream, which must not
-    join the capture), or take the gradients with `torch.autograd.grad`."""
+    A training step may be captured into a CUDA graph while no eager graph of the same leaves is alive: torch keeps the
+    gradient accumulators of such a graph on its stream, which a captured backward pass of any operator, this one
+    included, cannot join, and raises an error."""
     _check(x, "x")
     if x.dim() < 1:
         raise RuntimeError("x must be [..., hidden]")
