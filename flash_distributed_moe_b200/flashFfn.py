@@ -35,9 +35,10 @@ def _check(t: torch.Tensor, name: str) -> None:
 
 
 def _check_weights(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> None:
+    dtype, device = x.dtype, x.get_device()
     for t, name in ((w13, "w13"), (w2, "w2")):
         _check(t, name)
-        if t.dtype != x.dtype or t.device != x.device:
+        if t.dtype != dtype or t.get_device() != device:
             raise RuntimeError(f"{name} must have the dtype and device of x")
         if not t.is_contiguous() or t.data_ptr() % 16:
             raise RuntimeError(f"{name} must be contiguous and start on 16 bytes")
@@ -55,14 +56,20 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _aligned(nbytes: int) -> int:
+    return (nbytes + 255) & -256
+
+
 def _forward(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, save: bool):
-    (hidden, inter), tokens, lib = w2.shape, x.shape[0], _lib.lib()
-    cfg = _config(hidden, inter, x.dtype)
+    (hidden, inter), tokens = w2.shape, x.shape[0]
+    part = tokens * inter
+    # as FlashMoeFfnSavedBytes and FlashMoeFfnWorkspaceBytes give them
+    nbytes = _aligned(4 * part) + 2 * _aligned(2 * part) if save else _aligned(2 * part)
     y = torch.empty_like(x)
-    nbytes = lib.FlashMoeFfnSavedBytes(cfg, tokens) if save else lib.FlashMoeFfnWorkspaceBytes(cfg, tokens, 0)
     buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    _lib.run(x.get_device(), "FlashMoeFfnForward", cfg, x.data_ptr(), w13.data_ptr(), w2.data_ptr(), y.data_ptr(),
-             *((buf.data_ptr(), None, 0) if save else (None, buf.data_ptr(), nbytes)), tokens)
+    to = buf.data_ptr()
+    _lib.run(x.get_device(), "FlashMoeFfnForward", _config(hidden, inter, x.dtype), x.data_ptr(), w13.data_ptr(),
+             w2.data_ptr(), y.data_ptr(), to if save else None, None if save else to, nbytes, tokens)
     return y, buf
 
 
@@ -78,14 +85,17 @@ class _GatedFfn(torch.autograd.Function):
     def backward(ctx, dy):
         x, w13, w2, saved = ctx.saved_tensors
         (hidden, inter), tokens = w2.shape, x.shape[0]
-        cfg = _config(hidden, inter, x.dtype)
         dy = _rows(dy)
-        grads = [torch.empty_like(t) if need else None for t, need in zip((x, w13, w2), ctx.needs_input_grad)]
-        nbytes = _lib.lib().FlashMoeFfnWorkspaceBytes(cfg, tokens, 1)
+        need = ctx.needs_input_grad
+        dx = torch.empty_like(x) if need[0] else None
+        dw13 = torch.empty_like(w13) if need[1] else None
+        dw2 = torch.empty_like(w2) if need[2] else None
+        nbytes = _aligned(4 * tokens * inter)  # FlashMoeFfnWorkspaceBytes
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        _lib.run(x.get_device(), "FlashMoeFfnBackward", cfg, dy.data_ptr(), x.data_ptr(), w13.data_ptr(), w2.data_ptr(),
-                 saved.data_ptr(), *[None if g is None else g.data_ptr() for g in grads], ws.data_ptr(), nbytes, tokens)
-        return tuple(grads)
+        _lib.run(x.get_device(), "FlashMoeFfnBackward", _config(hidden, inter, x.dtype), dy.data_ptr(), x.data_ptr(),
+                 w13.data_ptr(), w2.data_ptr(), saved.data_ptr(), dx.data_ptr() if need[0] else None,
+                 dw13.data_ptr() if need[1] else None, dw2.data_ptr() if need[2] else None, ws.data_ptr(), nbytes, tokens)
+        return dx, dw13, dw2
 
 
 def gated_ffn(x: torch.Tensor, w13: Weight, w2: Weight) -> torch.Tensor:
