@@ -1,7 +1,7 @@
 // Matrix products of the dense operators on tcgen05, for 16-bit operands (bf16, fp16) and for 4-bit ones with a
 // scale per 32 elements.  Two kernels:
 //
-//   pair_gemm    D[256 x 256] or D[256 x 128] tiles on pairs of CTAs.
+//   pair_gemm    D[256 x 256], D[256 x 192] or D[256 x 128] tiles on pairs of CTAs.
 //   stream_gemm  the weights are the M operand (128 rows a tile), up to 128 tokens the N operand, and a cluster of
 //                up to eight CTAs shares the k axis of a tile: for few tokens, where every byte of the weights is
 //                read once and that read has to be spread over all SMs.
@@ -117,9 +117,9 @@ __device__ __forceinline__ F2 sigmoid(F2 g) {
 __device__ __forceinline__ F2 gate(F2 g, F2 u) { return g * sigmoid(g) * u; }
 
 // The projections g and u are kept for the backward pass in 24 bits, an fp32 number without its last eight (cut, so
-// that a NaN stays one): in the 16 bits of the operands their rounding would be as large an error of the gradients as the rounding of the
-// gradients themselves (relative error of dx and dw13 in bf16: 3.0e-3 instead of 2.4e-3).  The upper 16 bits of g and
-// u lie in [T, 2I], the eight that follow of both in one word of [T, I].
+// that a NaN stays one): in the 16 bits of the operands their rounding would be as large an error of dx and dw13 as the
+// rounding of dg and du (relative error in bf16: 3.0e-3 instead of 2.4e-3).  The upper 16 bits of g and u lie in
+// [T, 2I], the eight that follow of both in one word of [T, I].
 __device__ __forceinline__ uint32_t upper16(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
 __device__ __forceinline__ uint32_t next8(uint32_t g0, uint32_t u0, uint32_t g1, uint32_t u1) {
   return __byte_perm(__byte_perm(g0, u0, 0x0051), __byte_perm(g1, u1, 0x0051), 0x5410);
@@ -136,7 +136,7 @@ __device__ __forceinline__ F2 from24(uint32_t upper, uint32_t lower) {
 // rows of B (gated: CTA 0 the gate projection's, CTA 1 the up projection's, so that D holds tile_n / 2 columns of
 // each), and the even CTA issues MMAs of 256 x tile_n x 16 (64 for 4-bit operands) that read both.  With tile_n = 256
 // 32 KB per stage and CTA (64 k of 16-bit operands, 256 k of 4-bit ones) serve 512 cycles of MMA, which is what one
-// CTA's tile of 128 x 256 needs 48 KB for.  Two rules make it fit few tiles (MakePairPlan): tile_n = 128, and a
+// CTA's tile of 128 x 256 needs 48 KB for.  Two rules make it fit few tiles (MakePairPlan): a smaller tile_n, and a
 // cluster of two or four pairs that share the k axis of a tile and add their partial sums through shared memory.
 constexpr int kPairThreads = 384;
 constexpr int kStageOperand = 16384;  // 128 rows of 128 bytes
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       }
     }
   } else if (warp >= 4) {
-    // ---- epilogue: warps w and w + 4 read the same 32 lanes and take turns with the columns, 32 at a time
+    // ---- epilogue: warps w and w + 4 read the same 32 lanes and take turns with the groups of columns
     const bool elected = ptx::elect_one();
     const int w = warp - 4, quad = warp & 3, half = w >> 2;
     uint8_t* buf = staging + w * S::kStaging;

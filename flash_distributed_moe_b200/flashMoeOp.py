@@ -43,11 +43,14 @@ class FlashMoeBlockWrapper(torch.nn.Module):
 
 class FlashFfnBlockWrapper(torch.nn.Module):
     """The same for a dense block: any module exposing `gate_up_proj.weight` [2I,H] (gate rows first) and
-    `down_proj.weight` [H,I], e.g. the dense layers and shared experts of the same models.  With `fourBit` the
+    `down_proj.weight` [H,I], without biases and with SiLU between them, e.g. the dense layers and shared experts of the same models.  With `fourBit` the
     weights are quantised once, here, and the forward pass reads them at half a byte per value."""
 
     def __init__(self, mlpModule: torch.nn.Module, fourBit: bool = False):
         super().__init__()
+        for projection in (mlpModule.gate_up_proj, mlpModule.down_proj):
+            if getattr(projection, "bias", None) is not None:
+                raise RuntimeError("projections with a bias are not supported")
         self.mlpModule = mlpModule
         self.fourBitWeights = None
         if fourBit:

@@ -31,7 +31,8 @@ def _scale_bytes(batch: int, rows: int, cols: int) -> int:
 
 class Mx4Tensor:
     """A 4-bit matrix [rows, cols] or batch of them [batch, rows, cols].  `values` uint8 [..., rows, cols / 2] with the
-    even element in the low half of a byte; `scales` uint8, in blocks of 512 for 128 rows and 128 columns."""
+    even element in the low half of a byte; `scales` uint8, in blocks of 512 for 128 rows and 128 columns, where those of
+    columns that do not exist are not 255 (which stands for NaN; mx4_quantize writes 0)."""
 
     __slots__ = ("shape", "device", "_tensors", "_buffer", "_pointers")
 

@@ -248,6 +248,9 @@ def test_wrapper_runs_a_dense_block():
     assert m.gate_up_proj.weight.grad is not None and m.down_proj.weight.grad is not None
     with torch.no_grad():
         assert FlashFfnBlockWrapper(m, fourBit=True)(x).shape == y.shape
+    m.down_proj.bias = torch.nn.Parameter(torch.zeros(256, dtype=BF16, device="cuda"))
+    with pytest.raises(RuntimeError):
+        FlashFfnBlockWrapper(m)
 
 
 def test_a_wait_that_runs_out(monkeypatch):
@@ -294,3 +297,24 @@ def test_a_nan_token_reaches_the_gradients():
     keep = torch.arange(20, device="cuda") != 5
     assert torch.isnan(dx[5]).all() and torch.isfinite(dx[keep]).all()
     assert torch.isnan(dw13).all() and torch.isnan(dw2).all()
+
+
+def test_offsets_beyond_32_bits():
+    # [T, 2I] has 2.3e9 elements: the last tokens' results, and the weights' gradients from those tokens alone
+    tokens, hidden, inter, last = 70000, 64, 16384, 300
+    g = torch.Generator(device="cuda").manual_seed(12)
+    r = lambda *s, std: torch.empty(*s, device="cuda").normal_(0, std, generator=g).to(BF16)  # noqa: E731
+    x, w13, w2 = r(tokens, hidden, std=1.0), r(2 * inter, hidden, std=0.2), r(hidden, inter, std=inter ** -0.5)
+    dy = torch.zeros(tokens, hidden, dtype=BF16, device="cuda")
+    dy[-last:] = r(last, hidden, std=1.0)
+    leaves = [t.requires_grad_() for t in (x, w13, w2)]
+    y = gated_ffn(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy)
+    tail = [t.detach() for t in (x[-last:], w13, w2)]
+    dl.assert_within(y[-last:].detach(), *dl.ffn(*tail))
+    want = dl.ffn_grads(*tail, dy[-last:])
+    assert not grads[0][:-last].any()
+    dl.assert_within(grads[0][-last:], *want[0])
+    for got, (value, bound) in zip(grads[1:], want[1:]):
+        # the zeros of the other tokens add nothing, but the sums have more terms
+        dl.assert_within(got, value, bound * (tokens / last))

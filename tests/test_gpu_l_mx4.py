@@ -185,3 +185,17 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         quantize_ffn_weights(w13[:64], w2)
     assert isinstance(q13, Mx4Tensor)
+
+
+def test_offsets_beyond_32_bits():
+    rows, cols, last = 70000, 32768, 200  # 2.3e9 elements
+    x = torch.empty(rows, cols, dtype=BF16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(5))
+    q = mx4_quantize(x)
+    small = mx4_quantize(x[-last:].clone())
+    assert torch.equal(q.values[-last:], small.values)
+    assert torch.equal(q.dequantize()[-last:], dl.mx4(x[-last:]).to(BF16))
+    w = mx4_quantize(values(64, cols, seed=1))
+    y, part = mx4_matmul(q, w), mx4_matmul(small, w)
+    want, e = dl.product(small.dequantize(FP32).double(), w.dequantize(FP32).double())
+    for got in (y[-last:], part):
+        dl.assert_within(got, want, dl.rounded(want, e, BF16))
