@@ -213,6 +213,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
+  if (warp == 0 && ptx::elect_one()) {
+    ptx::prefetch_tmap(&p.product[0].a);
+    ptx::prefetch_tmap(&p.product[0].b);
+  }
   if (warp == 2) {
     ptx::tmem_alloc_pair(tmem_slot, 512);
     ptx::tmem_relinquish_pair();
@@ -678,7 +682,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
   uint8_t* smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
   const int nt = p.tile_tokens;
   const uint32_t stage_bytes = kParts * kStageOperand + nt * 128 + kScales;  // a multiple of 1024: nt of 16
-  __shared__ uint64_t full[FDMOE_STREAM_STAGES], empty[FDMOE_STREAM_STAGES], acc_full;
+  __shared__ uint64_t full[FDMOE_STREAM_STAGES], empty[FDMOE_STREAM_STAGES], acc_full, sums_full;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile uint32_t abort_flag;
 
@@ -694,10 +698,20 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
       ptx::mbar_init(empty + s, 1);
     }
     ptx::mbar_init(&acc_full, 1);
+    ptx::mbar_init(&sums_full, 1);
     abort_flag = 0;
     ptx::fence_mbar_init();
+    // the partial sums of this CTA's groups of four tokens, from every CTA of the cluster
+    const int groups = (min(nt, p.tokens - tok0) + 3) >> 2;
+    if (rank < groups)
+      ptx::mbar_expect_tx(&sums_full, (uint32_t)((groups - rank + p.split - 1) / p.split * p.split * kParts * 2048));
   }
   if (warp == 4) {
+    if (ptx::elect_one()) {
+      ptx::prefetch_tmap(&p.a);
+      ptx::prefetch_tmap(&p.b);
+    }
+    __syncwarp();
     ptx::tmem_alloc(&tmem_slot, p.tmem_cols);
     ptx::tmem_relinquish();
   }
@@ -849,8 +863,9 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
     } else {
       // Groups of four tokens are dealt out to the CTAs of the cluster.  Each CTA stores its partial sums of a group
       // into the owner's shared memory, [group of the owner][CTA][part][row][4 tokens], where the stages were: every
-      // CTA's MMAs have read theirs once all have arrived at the first barrier.
-      ptx::cluster_sync();
+      // CTA's MMAs have read theirs once all have arrived at the cluster's barrier.  The bytes are counted on a barrier
+      // of the owner, which a releasing and acquiring barrier of the cluster would take 900 cycles longer than.
+      ptx::cluster_sync_relaxed();
       const uint32_t mine = ptx::smem_u32(smem) + (warp * 32 + lane) * 16;
       if (done)
         for (int c = 0; c < count; c += 16) {
@@ -863,15 +878,16 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
             const int group = (c + i) >> 2, owner = group % p.split, slot = group / p.split;
             if (c + i < count) {
               const uint32_t to = ptx::map_rank(mine + (slot * p.split + rank) * kParts * 2048, owner);
+              const uint32_t bar = ptx::map_rank(ptx::smem_u32(&sums_full), owner);
 #pragma unroll
               for (int q = 0; q < kParts; ++q)
-                ptx::st_cluster_u32x4(to + q * 2048, v[q][i], v[q][i + 1], v[q][i + 2], v[q][i + 3]);
+                ptx::st_async_u32x4(to + q * 2048, v[q][i], v[q][i + 1], v[q][i + 2], v[q][i + 3], bar);
             }
           }
         }
-      ptx::cluster_sync();
       const uint8_t* own = smem + (warp * 32 + lane) * 16;
-      for (int slot = 0, group = rank; group * 4 < count; ++slot, group += p.split) {
+      const bool have = rank * 4 < count && wt.wait_warp(&sums_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
+      for (int slot = 0, group = rank; have && group * 4 < count; ++slot, group += p.split) {
         float f[kParts][4] = {};
 #pragma unroll 4
         for (int r = 0; r < p.split; ++r)
@@ -888,10 +904,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
     }
   }
   __syncwarp();
-  if (warp >= 4 && p.split > 1) {
-    ptx::cluster_sync();
-    ptx::cluster_sync();
-  }
+  if (warp >= 4 && p.split > 1) ptx::cluster_sync_relaxed();
   ptx::tcgen05_fence_before();
   __syncthreads();
   wt.drain();
