@@ -44,6 +44,7 @@ struct Shared {
   std::mutex mutex;
   uint32_t* status = nullptr;
   EncodeTiledFn encode = nullptr;
+  CUresult (*context)(CUcontext*) = nullptr;  // cuCtxGetCurrent
   bool known[64] = {};
   fdmoe::DeviceSlots slots[64];
 } g_shared;
@@ -60,9 +61,18 @@ int BeginCall(Call* c, void* stream) {
   int dev = 0;
   DENSE_CHECK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
-  // a thread that has made no CUDA call yet (autograd's) has no context, which the descriptors need
-  DENSE_CHECK(cudaSetDevice(dev));
   std::lock_guard<std::mutex> lock(g_shared.mutex);
+  if (!g_shared.context) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    DENSE_CHECK(cudaGetDriverEntryPoint("cuCtxGetCurrent", &fn, cudaEnableDefault, &found));
+    if (found != cudaDriverEntryPointSuccess) return (int)cudaErrorUnknown;
+    g_shared.context = reinterpret_cast<CUresult (*)(CUcontext*)>(fn);
+  }
+  // A thread that has made no CUDA call yet (autograd's) has no context, which the descriptors need; one that has keeps
+  // its own.
+  CUcontext context = nullptr;
+  if (g_shared.context(&context) != CUDA_SUCCESS || !context) DENSE_CHECK(cudaSetDevice(dev));
   if (!g_shared.status) {
     // the first call of the process may be inside a stream capture, which this allocation is no part of
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;

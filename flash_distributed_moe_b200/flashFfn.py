@@ -102,6 +102,7 @@ def gated_ffn(x: torch.Tensor, w13: Weight, w2: Weight) -> torch.Tensor:
     """x [..., H] -> [..., H].  Asynchronous on the current torch stream of x's device.  Differentiable in x, w13 and w2:
     the gate and up projections of the tokens and silu(g) * u are kept for the backward pass, in 24 bits and in the dtype.  With Mx4Tensor
     weights (w13 [2, I, H], w2 [H, I]) x and the activations are quantised to 4 bits too, and there is no gradient.
+    h = silu(g) * u is rounded to the dtype: in fp16 it is infinite beyond 65504, as in a program of torch operators.
 
     A training step may be captured into a CUDA graph while no eager graph of the same leaves is alive: torch keeps the
     gradient accumulators of such a graph on its stream, which a captured backward pass of any operator, this one
