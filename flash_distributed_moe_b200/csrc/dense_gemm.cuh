@@ -155,6 +155,7 @@ struct PairShape {
   static constexpr int kBarriers = 256 + FDMOE_PAIR_LIST * 4;  // and the list of tiles
   static constexpr int kSmem =
       kStages * (2 * kStageOperand + kScales) + 8 * kStaging + kBarriers + 1024;  // 1024: alignment of the base
+  static_assert(kSmem > 196 * 1024, "takes all columns of an SM's TMEM: no other kernel that takes some may fit beside it");
 };
 
 struct PairTile {

@@ -72,7 +72,9 @@ inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, 
       const int cols = parts * s.tile_tokens + best.stages * scales;
       best.tmem_cols = 32;
       while (best.tmem_cols < cols) best.tmem_cols *= 2;
-      best.smem = std::max(best.stages * stage, n > 1 ? sums : 0) + kStreamSlack;
+      // The whole share, used or not: then CTAs that fit on an SM together find their columns there too.  One that had to
+      // wait for columns could wait for a CTA whose cluster waits for columns that this one's cluster holds elsewhere.
+      best.smem = per_sm == 2 ? kStreamSmemTwo : kStreamSmemOne;
     }
   }
   return best;

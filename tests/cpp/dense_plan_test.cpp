@@ -46,6 +46,11 @@ int main() {
               const int cols = parts * s.tile_tokens + (mx4 ? s.stages * (parts + 1) * 8 : 0);
               CHECK(s.tmem_cols >= cols && s.tmem_cols >= 32 && (s.tmem_cols & (s.tmem_cols - 1)) == 0);
               CHECK(s.tmem_cols * s.per_sm <= 512);
+              // No CTA may wait for another's columns while a CTA of its cluster on another SM already holds some:
+              // wherever the shared memory of several has room, their columns have too.
+              const int taken = s.smem + 1024, sm = 228 * 1024;
+              CHECK(taken / 1024 * 544 > sm / 1024 * s.tmem_cols);  // the sum of columns is a multiple of 32
+              CHECK(taken + 196 * 1024 > sm);                       // kernels that take all 512 columns
               const PairPlan q = MakePairPlan(tokens, rows, kb, gated, mx4, dev);
               const int cols_tile = gated ? q.tile_n / 2 : q.tile_n;
               CHECK(q.tile_n == 256 || ((q.tile_n == 128 || q.tile_n == 192) && !mx4));

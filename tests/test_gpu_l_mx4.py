@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import dense_testlib as dl
-from flash_distributed_moe_b200 import (Mx4Tensor, gated_ffn, mx4_gated_matmul, mx4_matmul, mx4_quantize,
+from flash_distributed_moe_b200 import (Mx4Tensor, dense_status, gated_ffn, mx4_gated_matmul, mx4_matmul, mx4_quantize,
                                         quantize_ffn_weights)
 
 pytestmark = pytest.mark.gpu
@@ -161,6 +161,26 @@ def test_another_stream():
         got = mx4_matmul(mx4_quantize(x), w)
     s.synchronize()
     assert torch.equal(got, want)
+
+
+def test_different_products_at_once():
+    """On streams of their own: products that need from 32 columns of an SM's tensor memory to all of them."""
+    calls = []
+    for i, tokens in enumerate((1, 33, 64, 120, 300)):
+        x = values(tokens, 512, seed=i)
+        q, w, w13 = mx4_quantize(x), *(mx4_quantize(values(*s, 512, seed=9)) for s in ((520,), (2, 384)))
+        dense = dl.make(tokens, 512, 768, BF16, seed=i)[:3]
+        calls += [lambda q=q, w=w: mx4_matmul(q, w), lambda q=q, w13=w13: mx4_gated_matmul(q, w13), lambda d=dense: gated_ffn(*d)]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in calls], [[] for _ in calls]
+    for _ in range(8):
+        for c, s, g in zip(calls, streams, got):
+            with torch.cuda.stream(s):
+                g.append(c())
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for gs, w in zip(got, want) for g in gs)
+    assert dense_status() == 0
 
 
 def test_refusals():
