@@ -2,7 +2,7 @@
 // scale per 32 elements.  Two kernels:
 //
 //   pair_gemm    D[256 x 256], D[256 x 192] or D[256 x 128] tiles on pairs of CTAs.
-//   stream_gemm  the weights are the M operand (128 rows a tile), up to 128 tokens the N operand, and a cluster of
+//   stream_gemm  the weights are the M operand (128 rows a tile), up to 160 tokens the N operand, and a cluster of
 //                up to eight CTAs shares the k axis of a tile: for few tokens, where every byte of the weights is
 //                read once and that read has to be spread over all SMs.
 //
@@ -672,7 +672,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
 // ------------------------------------------------------------ stream kernel
 // One CTA: D[128 weight rows x tile_tokens] (gated: two such accumulators, gate and up) over its part of the k axis.
 // The cluster's partial sums meet in shared memory: CTA r adds those of every split-th group of four tokens.
-constexpr int kStreamThreads = 192;  // 4 epilogue warps, loads, MMAs
+constexpr int kStreamThreads = 320;  // 8 epilogue warps (4 took 10 % longer at 96 tokens of 2048 x 6144), loads, MMAs
+constexpr int kStreamLoads = 8, kStreamMmas = 9;  // their warps
 
 template <bool MX4, int EPI>
 __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_constant__ FdmoeStreamParams p) {
@@ -707,7 +708,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
     if (rank < groups)
       ptx::mbar_expect_tx(&sums_full, (uint32_t)((groups - rank + p.split - 1) / p.split * p.split * kParts * 2048));
   }
-  if (warp == 4) {
+  if (warp == kStreamLoads) {
     if (ptx::elect_one()) {
       ptx::prefetch_tmap(&p.a);
       ptx::prefetch_tmap(&p.b);
@@ -721,7 +722,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
   ptx::tcgen05_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  if (warp == 4) {
+  if (warp == kStreamLoads) {
     {
       const bool elected = ptx::elect_one();
       auto load_weights = [&](int s, int kb) {
@@ -756,7 +757,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
                                   (tok0 >> 7) * p.sf_chunks + kb * 2);
       }
     }
-  } else if (warp == 5) {
+  } else if (warp == kStreamMmas) {
     {
       const bool elected = ptx::elect_one();
       const uint32_t idesc = ptx::make_idesc_f16(128, nt, p.bf16, false, false);
@@ -803,8 +804,10 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
     const int count = min(nt, p.tokens - tok0);
     const bool done = wt.wait_warp(&acc_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
     ptx::tcgen05_fence_after();
-    const uint32_t d = tmem + (uint32_t(warp * 32) << 16);
-    const int row = row0 + warp * 32 + lane;
+    // warps w and w + 4 read the same 32 lanes (rows) and take turns with the tokens
+    const int quad = warp & 3, half = warp >> 2;
+    const uint32_t d = tmem + (uint32_t(quad * 32) << 16);
+    const int row = row0 + quad * 32 + lane;
     // Four tokens' results of this row (of each part).  Neighbouring lanes exchange two, so that each stores two rows
     // of two tokens.
     constexpr bool kF32 = EPI == FDMOE_EPI_F32 || EPI == FDMOE_EPI_GATED_F32;
@@ -846,7 +849,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
     };
     if (p.split == 1) {
       if (done)
-        for (int c = 0; c < count; c += 16) {
+        for (int c = half * 16; c < count; c += 32) {
           uint32_t v[kParts][16];
 #pragma unroll
           for (int q = 0; q < kParts; ++q) ptx::tmem_ld_32x16(d + q * nt + c, v[q]);
@@ -867,9 +870,9 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
       // CTA's MMAs have read theirs once all have arrived at the cluster's barrier.  The bytes are counted on a barrier
       // of the owner, which a releasing and acquiring barrier of the cluster would take 900 cycles longer than.
       ptx::cluster_sync_relaxed();
-      const uint32_t mine = ptx::smem_u32(smem) + (warp * 32 + lane) * 16;
+      const uint32_t mine = ptx::smem_u32(smem) + (quad * 32 + lane) * 16;
       if (done)
-        for (int c = 0; c < count; c += 16) {
+        for (int c = half * 16; c < count; c += 32) {
           uint32_t v[kParts][16];
 #pragma unroll
           for (int q = 0; q < kParts; ++q) ptx::tmem_ld_32x16(d + q * nt + c, v[q]);
@@ -886,9 +889,9 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
             }
           }
         }
-      const uint8_t* own = smem + (warp * 32 + lane) * 16;
+      const uint8_t* own = smem + (quad * 32 + lane) * 16;
       const bool have = rank * 4 < count && wt.wait_warp(&sums_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
-      for (int slot = 0, group = rank; have && group * 4 < count; ++slot, group += p.split) {
+      for (int slot = half, group = rank + half * p.split; have && group * 4 < count; slot += 2, group += 2 * p.split) {
         float f[kParts][4] = {};
 #pragma unroll 4
         for (int r = 0; r < p.split; ++r)
@@ -905,12 +908,12 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
     }
   }
   __syncwarp();
-  if (warp >= 4 && p.split > 1) ptx::cluster_sync_relaxed();
+  if (warp >= kStreamLoads && p.split > 1) ptx::cluster_sync_relaxed();
   ptx::tcgen05_fence_before();
   __syncthreads();
   wt.drain();
   ptx::tcgen05_fence_after();
-  if (warp == 4) ptx::tmem_dealloc(tmem, p.tmem_cols);
+  if (warp == kStreamLoads) ptx::tmem_dealloc(tmem, p.tmem_cols);
 }
 
 }  // namespace dense

@@ -361,7 +361,7 @@ int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, 
   const int chunks = (int)fdmoe::ScaleChunks(k), up_block = (int)((rows + 127) / 128);
   const int epi = gated ? (dtype == kF32 ? FDMOE_EPI_GATED_F32 : FDMOE_EPI_GATED)
                         : (dtype == kF32 ? FDMOE_EPI_F32 : FDMOE_EPI_HALF);
-  if (fdmoe::UseStream(tokens) || (dtype == kF32 ? rows % 4 : rows % 8) != 0) {
+  if (fdmoe::UseStreamMx4(tokens) || (dtype == kF32 ? rows % 4 : rows % 8) != 0) {
     FdmoeStreamParams p;
     memset(&p, 0, sizeof(p));
     const fdmoe::StreamPlan s = fdmoe::MakeStreamPlan((int)rows, (int)tokens, kblocks, gated, true, *c.slots);
@@ -458,7 +458,7 @@ static int FfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w
   DENSE_TRY(BeginCall(&c, stream));
   const int64_t H = cfg->hiddenSize, I = cfg->intermediateSize;
   const bool bf16 = cfg->dtype == kBf16;
-  if (!savedFor && !stall && fdmoe::UseStream(T)) {
+  if (!savedFor && !stall && fdmoe::UseStream(T, 6 * H * I)) {
     DENSE_TRY(StreamProduct(c, x, w13, workspace, T, I, H, true, bf16, false));
     return StreamProduct(c, workspace, w2, y, T, H, I, false, bf16, true);
   }

@@ -15,6 +15,7 @@ constexpr int kStreamSlack = 1024;            // for the alignment of the stages
 
 struct StreamPlan {
   int tile_tokens, token_tiles, row_tiles, split, stages, smem, tmem_cols, per_sm;
+  double cycles;  // estimated
 };
 
 inline int RoundUp(int v, int m) { return (v + m - 1) / m * m; }
@@ -39,8 +40,9 @@ inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, 
   for (int per_sm = 2; per_sm >= 1; --per_sm) {
     StreamPlan s = {};
     s.per_sm = per_sm;
-    s.token_tiles = (tokens + FDMOE_STREAM_TOKENS - 1) / FDMOE_STREAM_TOKENS;
-    s.tile_tokens = s.token_tiles > 1 ? FDMOE_STREAM_TOKENS : RoundUp(tokens, 16);
+    const int most_tokens = mx4 ? FDMOE_STREAM_TOKENS_MX4 : FDMOE_STREAM_TOKENS;
+    s.token_tiles = (tokens + most_tokens - 1) / most_tokens;
+    s.tile_tokens = s.token_tiles > 1 ? most_tokens : RoundUp(tokens, 16);
     s.row_tiles = (rows + FDMOE_STREAM_ROWS - 1) / FDMOE_STREAM_ROWS;
     const int stage = parts * 16384 + s.tile_tokens * 128 + (mx4 ? (parts + 1) * 1024 : 0);
     const int room = (per_sm == 2 ? kStreamSmemTwo : kStreamSmemOne) - kStreamSlack;
@@ -49,11 +51,11 @@ inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, 
     const int scales = mx4 ? (parts + 1) * 8 : 0;  // TMEM columns per stage
     int most = std::min(room / stage, (int)FDMOE_STREAM_STAGES);
     if (scales) most = std::min(most, ((per_sm == 2 ? 256 : 512) - parts * s.tile_tokens) / scales);
-    if (per_sm == 2 && (most < 2 || sums > room || parts * s.tile_tokens > 256)) continue;
+    if (per_sm == 2 && (most < 2 || parts * s.tile_tokens > 256)) continue;
     const double weights = parts * (mx4 ? 16384 + 1024 : 16384), issue = mx4 ? 430 + 210 * parts : 380 + 160 * parts;
     for (int n = 1; n <= FDMOE_STREAM_SPLIT && n <= kblocks; ++n) {
       const int64_t slots = per_sm == 2 ? dev.stream_two[n] : dev.stream_one[n];
-      if (slots < 1) continue;  // the device cannot hold such a cluster
+      if (slots < 1 || (n > 1 && sums > room)) continue;  // the device cannot hold such a cluster, or a CTA the sums
       const int blocks = (kblocks + n - 1) / n;
       double t = per_sm == 1 ? 2000 : 0;  // the launches before and after it cannot overlap with it
       // the partial sums' way through the cluster's shared memory at 14 bytes per cycle, and the epilogue
@@ -67,6 +69,7 @@ inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, 
       if (best_time != 0 && t >= best_time) continue;
       best_time = t;
       best = s;
+      best.cycles = t;
       best.split = n;
       best.stages = std::min(most, blocks);
       const int cols = parts * s.tile_tokens + best.stages * scales;
@@ -200,11 +203,18 @@ inline ManyPlan MakeManyPlan(const ManyShape* shape, int n, const DeviceSlots& d
   return m;
 }
 
-// Whether the streaming kernel takes a product instead of the pair kernel.  Whole block, streaming and pair kernels:
-// 64 tokens of 2048 x 768 14.8 and 20.9 us, of 1024 x 4096 18.8 and 21.0, of 2048 x 6144 29 and 32.6; 96 tokens 17.9
-// and 20.9, 22.2 and 21.2, 33.6 and 32.9; 128 tokens 21.0 and 21.0, 25.3 and 21.4, 38 and 33.
-inline bool UseStream(int64_t tokens) { return tokens <= 96; }
-
+// Whether the streaming kernel takes the products of `tokens` rows instead of the pair kernel.  It reads weights faster,
+// which counts by their bytes, and its partial sums and epilogue cost more with every token.  Whole block of `bytes` of
+// weights, streaming and pair kernels in us: 96 tokens of 512 x 1024 12.3 and 12.3, of 1024 x 4096 18.8 and 19.6, of
+// 2048 x 6144 28.3 and 31.2; 128 tokens of 1024 x 4096 21.2 and 19.8, of 2048 x 6144 31.6 and 31.6, of 4096 x 12288 67
+// and 84.5; 160 tokens of 4096 x 4096 38.3 and 36.1, of 4096 x 12288 70.5 and 85, of 8192 x 28672 298 and 297.
+inline bool UseStream(int64_t tokens, int64_t bytes) {
+  return tokens <= std::min<int64_t>(96 + (bytes >> 21), FDMOE_STREAM_TOKENS);
+}
+// 4-bit operands: one tile of tokens.  128 tokens times 4096 x 12288 (rows, columns) 13.0 and 15.4 us, 2048 x 6144 8.7
+// and 11.0, 28672 x 8192 28.7 and 31.7, 12288 x 4096 12.0 and 11.0; 160 tokens 14.8 and 15.3, 9.3 and 11.0, 45 and 32,
+// 13.9 and 10.9.
+inline bool UseStreamMx4(int64_t tokens) { return tokens <= FDMOE_STREAM_TOKENS_MX4; }
 
 inline size_t AlignBytes(size_t v) { return (v + 255) / 256 * 256; }
 

@@ -17,7 +17,8 @@ enum {
   FDMOE_PAIR_MOST = 96,       // most pairs of such a launch
   FDMOE_PAIR_LIST = 64,       // most tiles of a pair in it
   FDMOE_STREAM_ROWS = 128,    // weight rows of a tile of the streaming kernel
-  FDMOE_STREAM_TOKENS = 128,  // most tokens of a tile of the streaming kernel
+  FDMOE_STREAM_TOKENS = 160,  // most tokens of a tile of the streaming kernel
+  FDMOE_STREAM_TOKENS_MX4 = 128,  // with 4-bit operands: a tile lies in one block of 128 rows of scales
   FDMOE_STREAM_SPLIT = 8,     // most CTAs that share the k axis of a tile of the streaming kernel
   FDMOE_STREAM_STAGES = 12,   // most shared-memory stages of the streaming kernel
   FDMOE_MX4_BLOCK = 32,       // elements that share a scale
@@ -78,7 +79,7 @@ typedef struct {
   uint64_t timeout_ns;
   int64_t ld;
   int32_t rows, tokens;
-  int32_t tile_tokens;        // 16..128, a multiple of 16
+  int32_t tile_tokens;        // a multiple of 16, up to FDMOE_STREAM_TOKENS or FDMOE_STREAM_TOKENS_MX4
   int32_t split;              // CTAs per tile along k: the cluster
   int32_t kblocks;
   int32_t stages;

@@ -32,10 +32,10 @@ int main() {
               const StreamPlan s = MakeStreamPlan(rows, tokens, kb, gated, mx4, dev);
               const int parts = gated ? 2 : 1;
               const int stage = parts * 16384 + s.tile_tokens * 128 + (mx4 ? (parts + 1) * 1024 : 0);
-              CHECK(s.tile_tokens % 16 == 0 && s.tile_tokens >= 16 && s.tile_tokens <= FDMOE_STREAM_TOKENS);
+              CHECK(s.tile_tokens % 16 == 0 && s.tile_tokens >= 16 && s.tile_tokens <= (mx4 ? FDMOE_STREAM_TOKENS_MX4 : FDMOE_STREAM_TOKENS));
               CHECK((int64_t)s.tile_tokens * s.token_tiles >= tokens && (int64_t)s.tile_tokens * (s.token_tiles - 1) < tokens);
               // a tile of tokens lies within one block of 128 rows of scales and starts on a column of them
-              if (s.token_tiles > 1) CHECK(s.tile_tokens == 128 || (128 % s.tile_tokens == 0 && s.tile_tokens % 32 == 0));
+              if (s.token_tiles > 1 && mx4) CHECK(s.tile_tokens == 128 || (128 % s.tile_tokens == 0 && s.tile_tokens % 32 == 0));
               CHECK(s.row_tiles * FDMOE_STREAM_ROWS >= rows && s.row_tiles <= 65535);
               CHECK(s.split >= 1 && s.split <= FDMOE_STREAM_SPLIT && s.split <= kb);
               CHECK(s.stages >= 1 && s.stages <= FDMOE_STREAM_STAGES);

@@ -28,6 +28,14 @@ def test_forward(tokens, hidden, inter, dtype):
     assert torch.equal(y, gated_ffn(x, w13, w2))  # the same call, the same bits
 
 
+@pytest.mark.parametrize("tokens", [97, 130, 147, 160, 161])
+def test_more_tokens_of_large_weights(tokens):
+    x, w13, w2, _ = dl.make(tokens, 4120, 5480, BF16, seed=10)  # 129 MB
+    y = gated_ffn(x, w13, w2)
+    dl.assert_within(y, *dl.ffn(x, w13, w2))
+    assert torch.equal(y, gated_ffn(x, w13, w2))
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("tokens,hidden,inter", SIZES)
 def test_training_step(tokens, hidden, inter, dtype):
