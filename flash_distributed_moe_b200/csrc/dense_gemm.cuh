@@ -190,7 +190,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
   uint64_t* acc_full = empty + S::kStages;
   uint64_t* acc_empty = acc_full + S::kAccs;
   uint64_t* gu_full = acc_empty + S::kAccs;  // gradient: one per epilogue warp
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gu_full + 8);
+  uint64_t* sums_full = gu_full + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums_full + 1);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   uint32_t* list = tmem_slot + 2;  // [0]: how many; product << 28 | tile
 
@@ -211,8 +212,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       ptx::mbar_init(acc_empty + a, 16);  // eight epilogue warps of each CTA
     }
     for (int w = 0; w < 8; ++w) ptx::mbar_init(gu_full + w, 1);
+    ptx::mbar_init(sums_full, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
+    if (split > 1) ptx::mbar_expect_tx(sums_full, p.product[0].tile_n * 512 / split * (split - 1));  // the other pairs'
   }
   if (warp == 0 && ptx::elect_one()) {
     ptx::prefetch_tmap(&p.product[0].a);
@@ -382,20 +385,23 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
   } else if (warp >= 4) {
     // ---- epilogue: warps w and w + 4 read the same 32 lanes and take turns with the groups of columns
     const bool elected = ptx::elect_one();
-    const int w = warp - 4, quad = warp & 3, half = w >> 2;
+    const int w = warp - 4, quad = warp & 3;
     uint8_t* buf = staging + w * S::kStaging;
     const uint32_t sbuf = ptx::smem_u32(buf);
-    // This warp's groups of columns, a box wide: the first, and the distance to the next (of all pairs' and halves').
+    // Boxes of 32 rows and a group of columns are dealt out to the pairs and to their warps; box i is quarter i & 3 of
+    // the rows of group i >> 2, so that a pair on its own reads its warps' own lanes.
     constexpr int kGroup = kF32 ? 32 : 64;
-    constexpr int kMost = (kGated ? 128 : 256) / kGroup / 2;  // groups of a warp
-    const int first_group = half * split + (int)part, group_step = 2 * split;
+    constexpr int kMost = (kGated ? 128 : 256) / kGroup / 2;  // boxes of a warp
+    const int box0 = (int)part + split * w, box_step = 8 * split;
+    const auto box_at = [&](int j) { return box0 + j * box_step; };
     // Gradient: the boxes first take the upper halves of g and u of a group of columns, which dg and du then replace;
     // the lower bytes of this lane's row come straight into registers.
     uint32_t gu_count = 0;
     uint4 lower[8];
-    auto fetch_gu = [&](const PairTile& t, int c) {
+    auto fetch_gu = [&](const PairTile& t, int box) {
       const FdmoePairProduct& pr = p.product[0];
-      const int row = t.m * 256 + (int)rank * 128 + quad * 32 + lane, col = t.n * pr.tile_n + c * 64;
+      const int y = t.m * 256 + (int)rank * 128 + (box & 3) * 32, x = t.n * pr.tile_n + (box >> 2) * 64;
+      const int row = y + lane, col = x;
       const uint16_t* at = static_cast<const uint16_t*>(p.lower) + (int64_t)row * pr.cols + col;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -403,7 +409,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       if (elected) {
         ptx::bulk_wait_group_read0();
         ptx::mbar_expect_tx(gu_full + w, 8192);
-        const int x = t.n * pr.tile_n + c * 64, y = t.m * 256 + (int)rank * 128 + quad * 32;
         ptx::tma_load_2d(buf, &p.gu[0], gu_full + w, x, y);
         ptx::tma_load_2d(buf + 4096, &p.gu[1], gu_full + w, x, y);
       }
@@ -412,43 +417,65 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     PairTile t;
     for (int n = 0; tile_at(n, g, t); ++n) {
       const FdmoePairProduct& pr = p.product[g];
-      const int half_n = pr.tile_n >> 1, tile_cols = kGated ? half_n : pr.tile_n, groups = tile_cols / kGroup;
+      const int half_n = pr.tile_n >> 1, tile_cols = kGated ? half_n : pr.tile_n, boxes = tile_cols / kGroup * 4;
       const int acc = n % S::kAccs;
       if constexpr (EPI == FDMOE_EPI_GATED_GRAD)
-        if (first_group < groups) fetch_gu(t, first_group);
-      const bool done = wt.wait_warp(acc_full + acc, (n / S::kAccs) & 1, FDMOE_DENSE_TIMEOUT_DONE);
+        if (box_at(0) < boxes) fetch_gu(t, box_at(0));
+      bool done = wt.wait_warp(acc_full + acc, (n / S::kAccs) & 1, FDMOE_DENSE_TIMEOUT_DONE);
       ptx::tcgen05_fence_after();
       const uint32_t d = tmem + acc * kAccCols + (uint32_t(quad * 32) << 16);
-      const int row0 = t.m * 256 + (int)rank * 128 + quad * 32;
+      const int tile_row = t.m * 256 + (int)rank * 128;
+      // Where the k axis is shared (a cluster's only tile) every pair stores its partial sums of a box into the shared
+      // memory of the box's owner, [box of the owner][pair][part][column / 4][row][4], where the stages were: all MMAs
+      // have read theirs once every CTA has arrived at the cluster's barrier.
+      constexpr int kParts = kGated ? 2 : 1, kBoxSums = kGroup * 128;  // bytes
+      const int shift = split >> 1;  // log2
+      const auto sums_at = [&](int box, int pair) { return ((box >> shift << shift) + pair) * kParts * kBoxSums; };
       if (split > 1) {
-        // the cluster's only tile: the partial sums go where the stages were, [column / 4][row][4]
+        ptx::cluster_sync_relaxed();
         if (done)
-          for (int c = half; c < pr.tile_n >> 5; c += 2) {
+          for (int c = w >> 2; c < pr.tile_n >> 5; c += 2) {
             uint32_t v[32];
             ptx::tmem_ld_32x32(d + c * 32, v);
+            const int q = kGated && c * 32 >= half_n, col = c * 32 - q * half_n, box = col / kGroup * 4 + quad;
+            const uint32_t owner = box & (split - 1);
+            const uint32_t at = sums_at(box, part) + q * kBoxSums + (col % kGroup) * 128 + lane * 16;
+            const uint32_t to = ptx::map_rank(ptx::smem_u32(stages) + at, 2 * owner + rank);
+            const uint32_t bar = ptx::map_rank(ptx::smem_u32(sums_full), 2 * owner + rank);
             ptx::tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<uint4*>(stages + ((c * 8 + j) * 128 + quad * 32 + lane) * 16) =
-                  make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            for (int j = 0; j < 8; ++j) {
+              if (owner == part)
+                *reinterpret_cast<uint4*>(stages + at + j * 512) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+              else
+                ptx::st_async_u32x4(to + j * 512, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], bar);
+            }
           }
-        ptx::cluster_sync();
+        ptx::epilogue_sync();
+        done = done && wt.wait_warp(sums_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
       }
       if (!done) break;
-      // 32 columns of the tile from the accumulator, or from all pairs' partial sums in the order of their ranks
-      auto load = [&](int column, uint32_t (&v)[32]) {
+      // 32 columns (from `column` of part q on) of a box from the accumulator, or from all pairs' partial sums in the
+      // order of their ranks
+      auto load = [&](int box, int q, int column, uint32_t (&v)[32]) {
         if (split == 1) {
-          ptx::tmem_ld_32x32(d + column, v);
+          ptx::tmem_ld_32x32(d + q * half_n + (box >> 2) * kGroup + column, v);
           return;
         }
-        const uint32_t at = ptx::smem_u32(stages) + ((column >> 2) * 128 + quad * 32 + lane) * 16;
+        const uint32_t from = ptx::smem_u32(stages) + sums_at(box, 0) + q * kBoxSums + column * 128 + lane * 16;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = 0;
-        for (int r = 0; r < split; ++r) {
-          const uint32_t from = ptx::map_rank(at, 2 * r + rank);
+        for (int j = 0; j < 8; ++j) {
+          const float4 f = ptx::ld_shared_f32x4(from + j * 512);
+          v[4 * j] = __float_as_uint(f.x);
+          v[4 * j + 1] = __float_as_uint(f.y);
+          v[4 * j + 2] = __float_as_uint(f.z);
+          v[4 * j + 3] = __float_as_uint(f.w);
+        }
+#pragma unroll 1
+        for (int r = 1; r < split; ++r) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float4 f = ptx::ld_cluster_f32x4(from + j * 2048);
+            const float4 f = ptx::ld_shared_f32x4(from + r * (kParts * kBoxSums) + j * 512);
             v[4 * j] = __float_as_uint(__uint_as_float(v[4 * j]) + f.x);
             v[4 * j + 1] = __float_as_uint(__uint_as_float(v[4 * j + 1]) + f.y);
             v[4 * j + 2] = __float_as_uint(__uint_as_float(v[4 * j + 2]) + f.z);
@@ -471,20 +498,21 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
         __syncwarp();
       };
       const int col0 = t.n * tile_cols;
-      // Sends box b, which all lanes have written, to columns from `col` on of result `map`.
-      auto send = [&](int map, int b, int col) {
-        if (elected && row0 < pr.rows && col < pr.cols) ptx::tma_store_2d(&pr.out[map], sbuf + b * 4096, col, row0);
+      // Sends buffer b, which all lanes have written, to where `box` lies in result `map`.
+      auto send = [&](int map, int b, int box) {
+        const int row = tile_row + (box & 3) * 32, col = col0 + (box >> 2) * kGroup;
+        if (elected && row < pr.rows && col < pr.cols) ptx::tma_store_2d(&pr.out[map], sbuf + b * 4096, col, row);
       };
       if constexpr (EPI == FDMOE_EPI_HALF) {
         // All of the warp's columns are read, rounded and the accumulator given back before the first is stored.
         uint32_t w[kMost][32];
 #pragma unroll
         for (int j = 0; j < kMost; ++j) {
-          const int c = first_group + j * group_step;
-          if (c >= groups) break;
+          const int box = box_at(j);
+          if (box >= boxes) break;
           uint32_t v[2][32];
-          load(c * 64, v[0]);
-          load(c * 64 + 32, v[1]);
+          load(box, 0, 0, v[0]);
+          load(box, 0, 32, v[1]);
           ptx::tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 32; ++i) w[j][i] = pack2(as_f2(v[i >> 4][(2 * i) & 31], v[i >> 4][(2 * i + 1) & 31]), BF16);
@@ -493,47 +521,47 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
         if constexpr (S::kBoxes >= kMost) boxes_free();
 #pragma unroll
         for (int j = 0; j < kMost; ++j) {
-          const int c = first_group + j * group_step, b = S::kBoxes >= kMost ? j : 0;
-          if (c >= groups) break;
+          const int box = box_at(j), b = S::kBoxes >= kMost ? j : 0;
+          if (box >= boxes) break;
           if constexpr (S::kBoxes < kMost) boxes_free();
 #pragma unroll
           for (int i = 0; i < 8; ++i) stage16(buf + b * 4096, lane, i, w[j][4 * i], w[j][4 * i + 1], w[j][4 * i + 2], w[j][4 * i + 3]);
           boxes_written();
-          send(0, b, col0 + c * 64);
+          send(0, b, box);
           if (elected) ptx::bulk_commit_group();
         }
       } else if constexpr (EPI == FDMOE_EPI_F32) {
         uint32_t v[kMost][32];
 #pragma unroll
         for (int j = 0; j < kMost; ++j)
-          if (first_group + j * group_step < groups) load((first_group + j * group_step) * 32, v[j]);
+          if (box_at(j) < boxes) load(box_at(j), 0, 0, v[j]);
         ptx::tmem_ld_wait();
         release();
 #pragma unroll
         for (int j = 0; j < kMost; ++j) {
-          const int c = first_group + j * group_step;
-          if (c >= groups) break;
+          const int box = box_at(j);
+          if (box >= boxes) break;
           boxes_free();
 #pragma unroll
           for (int i = 0; i < 8; ++i) stage16(buf, lane, i, v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3]);
           boxes_written();
-          send(0, 0, col0 + c * 32);
+          send(0, 0, box);
           if (elected) ptx::bulk_commit_group();
         }
       } else if constexpr (EPI == FDMOE_EPI_GATED_F32) {
         uint32_t g[kMost][32], u[kMost][32];
 #pragma unroll
         for (int j = 0; j < kMost; ++j)
-          if (first_group + j * group_step < groups) {
-            load((first_group + j * group_step) * 32, g[j]);
-            load(half_n + (first_group + j * group_step) * 32, u[j]);
+          if (box_at(j) < boxes) {
+            load(box_at(j), 0, 0, g[j]);
+            load(box_at(j), 1, 0, u[j]);
           }
         ptx::tmem_ld_wait();
         release();
 #pragma unroll
         for (int j = 0; j < kMost; ++j) {
-          const int c = first_group + j * group_step;
-          if (c >= groups) break;
+          const int box = box_at(j);
+          if (box >= boxes) break;
           boxes_free();
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -543,26 +571,26 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
             stage16(buf, lane, i, __float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
           }
           boxes_written();
-          send(0, 0, col0 + c * 32);
+          send(0, 0, box);
           if (elected) ptx::bulk_commit_group();
         }
       } else if constexpr (kGated) {
-        // One group of 64 columns, 32 at a time; 4-bit operands have one accumulator, which is given back before the
+        // One box of 64 columns, 32 at a time; 4-bit operands have one accumulator, which is given back before the
         // activation is computed.
-        const int c = first_group;
+        const int box = box_at(0);
         uint32_t g[MX4 ? 2 : 1][32], u[MX4 ? 2 : 1][32];
-        if (MX4 && c < groups) {
+        if (MX4 && box < boxes) {
 #pragma unroll
           for (int i = 0; i < (MX4 ? 2 : 1); ++i) {
-            load(c * 64 + i * 32, g[i]);
-            load(half_n + c * 64 + i * 32, u[i]);
+            load(box, 0, i * 32, g[i]);
+            load(box, 1, i * 32, u[i]);
           }
         }
         if constexpr (MX4) {
           ptx::tmem_ld_wait();
           release();
         }
-        if (c < groups) {
+        if (box < boxes) {
           boxes_free();
           uint32_t up[EPI == FDMOE_EPI_GATED_SAVE ? 32 : 1];
 #pragma unroll
@@ -570,8 +598,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
             uint32_t(&gi)[32] = g[MX4 ? i : 0];
             uint32_t(&ui)[32] = u[MX4 ? i : 0];
             if constexpr (!MX4) {
-              load(c * 64 + i * 32, gi);
-              load(half_n + c * 64 + i * 32, ui);
+              load(box, 0, i * 32, gi);
+              load(box, 1, i * 32, ui);
               ptx::tmem_ld_wait();
             }
 #pragma unroll
@@ -590,7 +618,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
               stage16(buf, lane, i * 4 + j, h[0], h[1], h[2], h[3]);
               if constexpr (EPI == FDMOE_EPI_GATED_SAVE) {
                 stage16(buf + 4096, lane, i * 4 + j, gw[0], gw[1], gw[2], gw[3]);
-                const int row = row0 + lane, col = col0 + c * 64 + i * 32 + j * 8;  // columns come in eights
+                const int row = tile_row + (box & 3) * 32 + lane;
+                const int col = col0 + (box >> 2) * 64 + i * 32 + j * 8;  // columns come in eights
                 if (row < pr.rows && col < pr.cols)
                   *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.lower) + (int64_t)row * pr.cols + col) =
                       make_uint4(lower[0], lower[1], lower[2], lower[3]);
@@ -599,10 +628,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
           }
           if constexpr (!MX4) release();
           boxes_written();
-          send(0, 0, col0 + c * 64);
+          send(0, 0, box);
           if constexpr (EPI == FDMOE_EPI_GATED_SAVE) {
             if (elected) ptx::bulk_commit_group();
-            send(1, 1, col0 + c * 64);
+            send(1, 1, box);
             if (elected) {
               ptx::bulk_commit_group();
               ptx::bulk_wait_group_read1();  // h has left
@@ -611,7 +640,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
 #pragma unroll
             for (int i = 0; i < 8; ++i) stage16(buf, lane, i, up[4 * i], up[4 * i + 1], up[4 * i + 2], up[4 * i + 3]);
             boxes_written();
-            send(2, 0, col0 + c * 64);
+            send(2, 0, box);
           }
           if (elected) ptx::bulk_commit_group();
         } else if constexpr (!MX4) {
@@ -619,13 +648,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
         }
       } else {
 #pragma unroll 1
-        for (int c = first_group; c < groups; c += group_step) {
-          if (c != first_group) fetch_gu(t, c);
+        for (int n = 0; n < kMost; ++n) {
+          const int box = box_at(n);
+          if (box >= boxes) break;
+          if (n > 0) fetch_gu(t, box);
           wt.wait_warp(gu_full + w, gu_count++ & 1, FDMOE_DENSE_TIMEOUT_FULL);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             uint32_t v[32];
-            load(c * 64 + i * 32, v);
+            load(box, 0, i * 32, v);
             ptx::tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 4; ++j) {  // eight columns
@@ -650,8 +681,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
             }
           }
           boxes_written();
-          send(0, 0, col0 + c * 64);
-          send(1, 1, col0 + c * 64);
+          send(0, 0, box);
+          send(1, 1, box);
           if (elected) ptx::bulk_commit_group();
         }
         release();
@@ -660,7 +691,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     if (elected) ptx::bulk_wait_group_read0();  // the boxes stay until they have been read
   }
   __syncwarp();
-  if (warp < 4 && split > 1) ptx::cluster_sync();  // the epilogue warps' exchange of partial sums
+  if (warp < 4 && split > 1) ptx::cluster_sync_relaxed();  // the epilogue warps' exchange of partial sums
   ptx::tcgen05_fence_before();
   __syncthreads();
   wt.drain();
@@ -703,10 +734,10 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
     ptx::mbar_init(&sums_full, 1);
     abort_flag = 0;
     ptx::fence_mbar_init();
-    // the partial sums of this CTA's groups of four tokens, from every CTA of the cluster
+    // the partial sums of this CTA's groups of four tokens, from every other CTA of the cluster
     const int groups = (min(nt, p.tokens - tok0) + 3) >> 2;
     if (rank < groups)
-      ptx::mbar_expect_tx(&sums_full, (uint32_t)((groups - rank + p.split - 1) / p.split * p.split * kParts * 2048));
+      ptx::mbar_expect_tx(&sums_full, (uint32_t)((groups - rank + p.split - 1) / p.split * (p.split - 1) * kParts * 2048));
   }
   if (warp == kStreamLoads) {
     if (ptx::elect_one()) {
@@ -802,12 +833,13 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
     }
   } else {
     const int count = min(nt, p.tokens - tok0);
-    const bool done = wt.wait_warp(&acc_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
-    ptx::tcgen05_fence_after();
     // warps w and w + 4 read the same 32 lanes (rows) and take turns with the tokens
     const int quad = warp & 3, half = warp >> 2;
     const uint32_t d = tmem + (uint32_t(quad * 32) << 16);
     const int row = row0 + quad * 32 + lane;
+    int owner = half * 4 % p.split, slot = half * 4 / p.split;  // of this warp's next group of tokens
+    const bool done = wt.wait_warp(&acc_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
+    ptx::tcgen05_fence_after();
     // Four tokens' results of this row (of each part).  Neighbouring lanes exchange two, so that each stores two rows
     // of two tokens.
     constexpr bool kF32 = EPI == FDMOE_EPI_F32 || EPI == FDMOE_EPI_GATED_F32;
@@ -870,7 +902,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
       // CTA's MMAs have read theirs once all have arrived at the cluster's barrier.  The bytes are counted on a barrier
       // of the owner, which a releasing and acquiring barrier of the cluster would take 900 cycles longer than.
       ptx::cluster_sync_relaxed();
-      const uint32_t mine = ptx::smem_u32(smem) + (quad * 32 + lane) * 16;
+      uint8_t* const own = smem + (quad * 32 + lane) * 16;
+      const uint32_t mine = ptx::smem_u32(own);
       if (done)
         for (int c = half * 16; c < count; c += 32) {
           uint32_t v[kParts][16];
@@ -879,19 +912,23 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
           ptx::tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
-            const int group = (c + i) >> 2, owner = group % p.split, slot = group / p.split;
             if (c + i < count) {
-              const uint32_t to = ptx::map_rank(mine + (slot * p.split + rank) * kParts * 2048, owner);
+              const uint32_t at = (slot * p.split + rank) * kParts * 2048, to = ptx::map_rank(mine + at, owner);
               const uint32_t bar = ptx::map_rank(ptx::smem_u32(&sums_full), owner);
 #pragma unroll
               for (int q = 0; q < kParts; ++q)
-                ptx::st_async_u32x4(to + q * 2048, v[q][i], v[q][i + 1], v[q][i + 2], v[q][i + 3], bar);
+                if (owner == rank)
+                  *reinterpret_cast<uint4*>(own + at + q * 2048) = make_uint4(v[q][i], v[q][i + 1], v[q][i + 2], v[q][i + 3]);
+                else
+                  ptx::st_async_u32x4(to + q * 2048, v[q][i], v[q][i + 1], v[q][i + 2], v[q][i + 3], bar);
             }
+            if (++owner == p.split) owner = 0, ++slot;
           }
+          for (owner += 4; owner >= p.split; owner -= p.split) ++slot;  // the other warp's four groups
         }
-      const uint8_t* own = smem + (quad * 32 + lane) * 16;
+      ptx::epilogue_sync();
       const bool have = rank * 4 < count && wt.wait_warp(&sums_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
-      for (int slot = half, group = rank + half * p.split; have && group * 4 < count; slot += 2, group += 2 * p.split) {
+      for (slot = half; have && (slot * p.split + rank) * 4 < count; slot += 2) {
         float f[kParts][4] = {};
 #pragma unroll 4
         for (int r = 0; r < p.split; ++r)
@@ -903,7 +940,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
             f[q][2] += v.z;
             f[q][3] += v.w;
           }
-        finish(group * 4, f);
+        finish((slot * p.split + rank) * 4, f);
       }
     }
   }

@@ -205,11 +205,11 @@ inline ManyPlan MakeManyPlan(const ManyShape* shape, int n, const DeviceSlots& d
 
 // Whether the streaming kernel takes the products of `tokens` rows instead of the pair kernel.  It reads weights faster,
 // which counts by their bytes, and its partial sums and epilogue cost more with every token.  Whole block of `bytes` of
-// weights, streaming and pair kernels in us: 96 tokens of 512 x 1024 12.3 and 12.3, of 1024 x 4096 18.8 and 19.6, of
-// 2048 x 6144 28.3 and 31.2; 128 tokens of 1024 x 4096 21.2 and 19.8, of 2048 x 6144 31.6 and 31.6, of 4096 x 12288 67
-// and 84.5; 160 tokens of 4096 x 4096 38.3 and 36.1, of 4096 x 12288 70.5 and 85, of 8192 x 28672 298 and 297.
+// weights, streaming and pair kernels in us: 96 tokens of 512 x 1024 12.0 and 11.5, of 1024 x 4096 17.9 and 19.2, of
+// 2048 x 6144 27.6 and 30.5; 128 tokens of 1024 x 4096 19.8 and 19.3, of 2048 x 6144 30.4 and 31.0, of 4096 x 12288 68
+// and 84.6; 160 tokens of 2048 x 6144 32.6 and 30.7, of 4096 x 12288 73.8 and 85.7, of 8192 x 28672 303 and 304.
 inline bool UseStream(int64_t tokens, int64_t bytes) {
-  return tokens <= std::min<int64_t>(96 + (bytes >> 21), FDMOE_STREAM_TOKENS);
+  return tokens <= std::min<int64_t>(104 + (bytes >> 21), FDMOE_STREAM_TOKENS);
 }
 // 4-bit operands: one tile of tokens.  128 tokens times 4096 x 12288 (rows, columns) 13.0 and 15.4 us, 2048 x 6144 8.7
 // and 11.0, 28672 x 8192 28.7 and 31.7, 12288 x 4096 12.0 and 11.0; 160 tokens 14.8 and 15.3, 9.3 and 11.0, 45 and 32,
