@@ -199,23 +199,22 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
   // A cluster is `split` pairs, which share the k axis of a tile.
   const uint32_t cta = ptx::cluster_rank(), rank = cta & 1, leader = cta & ~1u, part = cta >> 1;
   const int split = p.split;
-  const int first = blockIdx.x / (2 * split), step = gridDim.x / (2 * split);
+  const int shift = split >> 1;  // log2
+  const int first = blockIdx.x >> (1 + shift), step = gridDim.x >> (1 + shift);
   const Waiter wt{abort_flag, p.status, p.timeout_ns};
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
-      ptx::mbar_init(full + s, 1);
-      ptx::mbar_init(empty + s, 1);
-    }
-    for (int a = 0; a < S::kAccs; ++a) {
-      ptx::mbar_init(acc_full + a, 1);
-      ptx::mbar_init(acc_empty + a, 16);  // eight epilogue warps of each CTA
-    }
-    for (int w = 0; w < 8; ++w) ptx::mbar_init(gu_full + w, 1);
-    ptx::mbar_init(sums_full, 1);
-    *abort_flag = 0;
+  // What comes before the first load is a fixed cost of every launch, and most of it is the fetching of instructions
+  // that run once: barriers are set up by the lanes of a warp, and the first tile is looked up (its divisions) while
+  // another warp waits for the tensor memory.
+  if (warp == 1) {
+    constexpr int kEmptyAcc = 2 * S::kStages + S::kAccs, kCount = kEmptyAcc + S::kAccs + 8 + 1;
+    static_assert(kCount <= 32, "one barrier per lane");
+    if (lane < kCount) ptx::mbar_init(full + lane, lane >= kEmptyAcc && lane < kEmptyAcc + S::kAccs ? 16 : 1);  // 16: the epilogue warps of both
+    if (lane == 0) *abort_flag = 0;
     ptx::fence_mbar_init();
-    if (split > 1) ptx::mbar_expect_tx(sums_full, p.product[0].tile_n * 512 / split * (split - 1));  // the other pairs'
+    __syncwarp();
+    if (lane == 0 && split > 1)
+      ptx::mbar_expect_tx(sums_full, (p.product[0].tile_n * 512 >> shift) * (split - 1));  // the other pairs'
   }
   if (warp == 0 && ptx::elect_one()) {
     ptx::prefetch_tmap(&p.product[0].a);
@@ -250,14 +249,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       if (lane == 0) list[0] = min(n, (uint32_t)FDMOE_PAIR_LIST - 3);
     }
   }
-  ptx::tcgen05_fence_before();
-  __syncthreads();
-  ptx::cluster_sync_relaxed();  // all CTAs' barriers are set up
-  ptx::tcgen05_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  ptx::grid_wait_dependency();  // nothing of global memory is touched before this
-  ptx::grid_launch_dependents();
-
   // The i-th tile of this pair (cluster) and its product.
   const auto tile_at = [&](int i, int& g, PairTile& t) {
     g = 0;
@@ -272,30 +263,41 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     t = pair_tile(tile, p.product[g].tiles_m, p.product[g].tiles_n);
     return true;
   };
+  int g;
+  PairTile t;
+  const bool listed = kMany && p.products > 1;
+  bool have = !listed && tile_at(0, g, t);
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  ptx::cluster_sync_relaxed();  // all CTAs' barriers are set up
+  ptx::tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (listed) have = tile_at(0, g, t);
+  ptx::grid_wait_dependency();  // nothing of global memory is touched before this
+  ptx::grid_launch_dependents();
 
   if (warp == 0) {
     // ---- loads: both CTAs fill their own stages; the bytes are counted on the even CTA's barriers
     {
       const bool elected = ptx::elect_one();
-      uint32_t it = 0;
+      int stage = 0;
+      uint32_t parity = 1;
       bool ok = true;
-      int g;
-      PairTile t;
-      for (int i = 0; ok && tile_at(i, g, t); ++i) {
+      for (int i = 0; ok && have; have = tile_at(++i, g, t)) {
         const FdmoePairProduct& pr = p.product[g];
         const int half_n = pr.tile_n >> 1;  // rows of B per CTA; gated: columns of each projection
-        const int kb0 = pr.kblocks * (int)part / split, kb1 = pr.kblocks * ((int)part + 1) / split;
+        const int kb0 = pr.kblocks * (int)part >> shift, kb1 = pr.kblocks * ((int)part + 1) >> shift;
         // rows along N come in boxes of 64, the second of which may be used in part
         const uint32_t b_bytes = pr.b_mn && half_n > 64 ? kStageOperand : half_n * 128;
         const int ax = t.m * 256 + (int)rank * 128;
         const int bx = kGated ? t.n * half_n + (int)rank * p.up_row : t.n * pr.tile_n + (int)rank * half_n;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % S::kStages;
-          const uint32_t ph = (it / S::kStages) & 1;
-          if (!wt.wait(empty + s, ph ^ 1, FDMOE_DENSE_TIMEOUT_EMPTY)) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          const int s = stage;
+          if (!wt.wait(empty + s, parity, FDMOE_DENSE_TIMEOUT_EMPTY)) {
             ok = false;
             break;
           }
+          if (++stage == S::kStages) stage = 0, parity ^= 1;
           if (p.stall || !elected) continue;
           if (rank == 0) ptx::mbar_expect_tx(full + s, 2 * (kStageOperand + b_bytes + S::kScales));
           const uint32_t bar = ptx::map_rank(ptx::smem_u32(full + s), leader);
@@ -331,13 +333,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     // ---- MMAs: one thread of the even CTA
     if (rank == 0) {
       const bool elected = ptx::elect_one();
-      uint32_t it = 0;
+      int stage = 0;
+      uint32_t parity = 0;
       bool ok = true;
-      int g;
-      PairTile t;
-      for (int n = 0; ok && tile_at(n, g, t); ++n) {
+      for (int n = 0; ok && have; have = tile_at(++n, g, t)) {
         const FdmoePairProduct& pr = p.product[g];
-        const int kb0 = pr.kblocks * (int)part / split, kb1 = pr.kblocks * ((int)part + 1) / split;
+        const int kb0 = pr.kblocks * (int)part >> shift, kb1 = pr.kblocks * ((int)part + 1) >> shift;
         const uint32_t idesc = ptx::make_idesc_f16(256, pr.tile_n, BF16, pr.a_mn, pr.b_mn);
         // 16 k further: 32 bytes along a row, or 16 rows of 128 bytes
         const uint32_t a_step = pr.a_mn ? 2048 >> 4 : 32 >> 4, b_step = pr.b_mn ? 2048 >> 4 : 32 >> 4;
@@ -347,12 +348,13 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
         if (!wt.wait(acc_empty + acc, aph ^ 1, FDMOE_DENSE_TIMEOUT_ACC)) break;
         ptx::tcgen05_fence_after();
         const uint32_t d = tmem + acc * kAccCols;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % S::kStages;
-          if (!wt.wait(full + s, (it / S::kStages) & 1, FDMOE_DENSE_TIMEOUT_FULL)) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          const int s = stage;
+          if (!wt.wait(full + s, parity, FDMOE_DENSE_TIMEOUT_FULL)) {
             ok = false;
             break;
           }
+          if (++stage == S::kStages) stage = 0, parity ^= 1;
           ptx::tcgen05_fence_after();
           if (!elected) continue;
           const uint32_t sa = ptx::smem_u32(stages + s * 2 * kStageOperand), sb = sa + kStageOperand;
@@ -413,9 +415,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
         ptx::tma_load_2d(buf + 4096, &p.gu[1], gu_full + w, x, y);
       }
     };
-    int g;
-    PairTile t;
-    for (int n = 0; tile_at(n, g, t); ++n) {
+    for (int n = 0; have; have = tile_at(++n, g, t)) {
       const FdmoePairProduct& pr = p.product[g];
       const int half_n = pr.tile_n >> 1, tile_cols = kGated ? half_n : pr.tile_n, boxes = tile_cols / kGroup * 4;
       const int acc = n % S::kAccs;
@@ -429,7 +429,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       // memory of the box's owner, [box of the owner][pair][part][column / 4][row][4], where the stages were: all MMAs
       // have read theirs once every CTA has arrived at the cluster's barrier.
       constexpr int kParts = kGated ? 2 : 1, kBoxSums = kGroup * 128;  // bytes
-      const int shift = split >> 1;  // log2
       const auto sums_at = [&](int box, int pair) { return ((box >> shift << shift) + pair) * kParts * kBoxSums; };
       if (split > 1) {
         ptx::cluster_sync_relaxed();
@@ -722,29 +721,69 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x;  // in the cluster (split, 1, 1)
   const int row0 = blockIdx.y * FDMOE_STREAM_ROWS, tok0 = blockIdx.z * nt;
-  const int kb0 = (int)((int64_t)p.kblocks * rank / p.split), kb1 = (int)((int64_t)p.kblocks * (rank + 1) / p.split);
+  const int kb0 = rank * p.kblocks_each + min(rank, p.kblocks_more);
+  const int kb1 = kb0 + p.kblocks_each + (rank < p.kblocks_more);
   const Waiter wt{&abort_flag, p.status, p.timeout_ns};
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) {
-      ptx::mbar_init(full + s, 1);
-      ptx::mbar_init(empty + s, 1);
+  // The first loads need no more than their barriers: they are on their way before the CTA's other warps are ready.
+  const int filled = min(p.stages, kb1 - kb0);
+  const bool elected = ptx::elect_one();
+  auto load_weights = [&](int s, int kb) {
+    uint64_t* bar = full + s;
+    uint8_t* sa = smem + s * stage_bytes;
+    uint8_t* sf = sa + kParts * kStageOperand + nt * 128;
+    ptx::mbar_expect_tx(bar, stage_bytes);
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) {
+      ptx::tma_load_2d(sa + q * kStageOperand, &p.a, bar, kb * (MX4 ? 128 : 64), row0 + q * p.up_row);
+      if (MX4)
+        ptx::tma_load_2d(sf + q * 2 * kScaleBlock, &p.sfa, bar, 0,
+                         ((int)blockIdx.y + q * p.sf_up_block) * p.sf_chunks + kb * 2);
     }
-    ptx::mbar_init(&acc_full, 1);
-    ptx::mbar_init(&sums_full, 1);
-    abort_flag = 0;
-    ptx::fence_mbar_init();
-    // the partial sums of this CTA's groups of four tokens, from every other CTA of the cluster
-    const int groups = (min(nt, p.tokens - tok0) + 3) >> 2;
-    if (rank < groups)
-      ptx::mbar_expect_tx(&sums_full, (uint32_t)((groups - rank + p.split - 1) / p.split * (p.split - 1) * kParts * 2048));
-  }
+  };
+  auto load_tokens = [&](int s, int kb) {
+    uint8_t* sb = smem + s * stage_bytes + kParts * kStageOperand;
+    ptx::tma_load_2d(sb, &p.b, full + s, kb * (MX4 ? 128 : 64), tok0);
+    if (MX4) ptx::tma_load_2d(sb + nt * 128 + kParts * 2 * kScaleBlock, &p.sfb, full + s, 0,
+                              (tok0 >> 7) * p.sf_chunks + kb * 2);
+  };
   if (warp == kStreamLoads) {
-    if (ptx::elect_one()) {
+    if (elected) {
       ptx::prefetch_tmap(&p.a);
       ptx::prefetch_tmap(&p.b);
     }
+    if (lane < FDMOE_STREAM_STAGES) {
+      ptx::mbar_init(full + lane, 1);
+      ptx::mbar_init(empty + lane, 1);
+    }
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async_shared();
     __syncwarp();
+    // The weights may be read while the launch before this one still writes the tokens.
+    if (p.early_weights && elected)
+      for (int i = 0; i < filled; ++i) load_weights(i, kb0 + i);
+    ptx::grid_wait_dependency();
+    // Only now may the next launch start: what it reads early was written before this launch's predecessor ended.
+    ptx::grid_launch_dependents();
+    if (elected)
+      for (int i = 0; i < filled; ++i) {
+        if (!p.early_weights) load_weights(i, kb0 + i);
+        load_tokens(i, kb0 + i);
+      }
+    __syncwarp();
+  } else if (warp == kStreamMmas) {
+    if (lane == 0) {
+      ptx::mbar_init(&acc_full, 1);
+      ptx::mbar_init(&sums_full, 1);
+      abort_flag = 0;
+      ptx::fence_mbar_init();
+      // the partial sums of this CTA's groups of four tokens, from every other CTA of the cluster
+      const int groups = (min(nt, p.tokens - tok0) + 3) >> 2;
+      if (rank < groups && p.split > 1)
+        ptx::mbar_expect_tx(&sums_full, (uint32_t)((groups - rank + p.split - 1) / p.split * (p.split - 1) * kParts * 2048));
+    }
+    __syncwarp();
+  } else if (warp == 0) {
     ptx::tmem_alloc(&tmem_slot, p.tmem_cols);
     ptx::tmem_relinquish();
   }
@@ -754,51 +793,28 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
   const uint32_t tmem = tmem_slot;
 
   if (warp == kStreamLoads) {
-    {
-      const bool elected = ptx::elect_one();
-      auto load_weights = [&](int s, int kb) {
-        uint64_t* bar = full + s;
-        uint8_t* sa = smem + s * stage_bytes;
-        uint8_t* sf = sa + kParts * kStageOperand + nt * 128;
-        ptx::mbar_expect_tx(bar, stage_bytes);
-#pragma unroll
-        for (int q = 0; q < kParts; ++q) {
-          ptx::tma_load_2d(sa + q * kStageOperand, &p.a, bar, kb * (MX4 ? 128 : 64), row0 + q * p.up_row);
-          if (MX4)
-            ptx::tma_load_2d(sf + q * 2 * kScaleBlock, &p.sfa, bar, 0,
-                             ((int)blockIdx.y + q * p.sf_up_block) * p.sf_chunks + kb * 2);
-        }
-      };
-      // The weights of the first stages may be read while the launch before this one still writes the tokens.
-      int ahead = 0;
-      if (p.early_weights)
-        for (; ahead < p.stages && kb0 + ahead < kb1; ++ahead)
-          if (elected) load_weights(ahead, kb0 + ahead);
-      ptx::grid_wait_dependency();
-      // Only now may the next launch start: what it reads early was written before this launch's predecessor ended.
-      ptx::grid_launch_dependents();
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int i = kb - kb0, s = i % p.stages;
-        if (i >= ahead && !wt.wait(empty + s, ((i / p.stages) & 1) ^ 1, FDMOE_DENSE_TIMEOUT_EMPTY)) break;
-        if (!elected) continue;
-        if (i >= ahead) load_weights(s, kb);
-        uint8_t* sb = smem + s * stage_bytes + kParts * kStageOperand;
-        ptx::tma_load_2d(sb, &p.b, full + s, kb * (MX4 ? 128 : 64), tok0);
-        if (MX4) ptx::tma_load_2d(sb + nt * 128 + kParts * 2 * kScaleBlock, &p.sfb, full + s, 0,
-                                  (tok0 >> 7) * p.sf_chunks + kb * 2);
+    int s = 0;
+    uint32_t parity = 0;
+    for (int kb = kb0 + filled; kb < kb1; ++kb) {
+      if (!wt.wait(empty + s, parity, FDMOE_DENSE_TIMEOUT_EMPTY)) break;
+      if (elected) {
+        load_weights(s, kb);
+        load_tokens(s, kb);
       }
+      if (++s == p.stages) s = 0, parity ^= 1;
     }
   } else if (warp == kStreamMmas) {
     {
-      const bool elected = ptx::elect_one();
       const uint32_t idesc = ptx::make_idesc_f16(128, nt, p.bf16, false, false);
       bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int i = kb - kb0, s = i % p.stages;
-        if (!wt.wait(full + s, (i / p.stages) & 1, FDMOE_DENSE_TIMEOUT_FULL)) {
+      uint32_t parity = 0;
+      for (int i = 0, stage = 0; i < kb1 - kb0; ++i) {
+        const int s = stage;
+        if (!wt.wait(full + s, parity, FDMOE_DENSE_TIMEOUT_FULL)) {
           ok = false;
           break;
         }
+        if (++stage == p.stages) stage = 0, parity ^= 1;
         ptx::tcgen05_fence_after();
         if (!elected) continue;
         const uint32_t sa = ptx::smem_u32(smem + s * stage_bytes), sb = sa + kParts * kStageOperand;
@@ -950,7 +966,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
   __syncthreads();
   wt.drain();
   ptx::tcgen05_fence_after();
-  if (warp == kStreamLoads) ptx::tmem_dealloc(tmem, p.tmem_cols);
+  if (warp == 0) ptx::tmem_dealloc(tmem, p.tmem_cols);
 }
 
 }  // namespace dense

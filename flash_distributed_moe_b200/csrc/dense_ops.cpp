@@ -277,7 +277,8 @@ int StreamProduct(const Call& c, const void* x, const void* w, void* out, int64_
   p.tokens = (int32_t)tokens;
   p.tile_tokens = s.tile_tokens;
   p.split = s.split;
-  p.kblocks = kblocks;
+  p.kblocks_each = kblocks / s.split;
+  p.kblocks_more = kblocks % s.split;
   p.stages = s.stages;
   p.up_row = (int32_t)rows;
   p.bf16 = bf16;
@@ -375,7 +376,8 @@ int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, 
     p.tokens = (int32_t)tokens;
     p.tile_tokens = s.tile_tokens;
     p.split = s.split;
-    p.kblocks = kblocks;
+    p.kblocks_each = kblocks / s.split;
+    p.kblocks_more = kblocks % s.split;
     p.stages = s.stages;
     p.up_row = (int32_t)rows;
     p.sf_chunks = chunks;

@@ -81,7 +81,7 @@ typedef struct {
   int32_t rows, tokens;
   int32_t tile_tokens;        // a multiple of 16, up to FDMOE_STREAM_TOKENS or FDMOE_STREAM_TOKENS_MX4
   int32_t split;              // CTAs per tile along k: the cluster
-  int32_t kblocks;
+  int32_t kblocks_each, kblocks_more;  // stages of k of every CTA; one more for the first few
   int32_t stages;
   int32_t up_row;
   int32_t sf_chunks;
