@@ -12,6 +12,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "dense_types.h"
 #include "ptx_cluster.cuh"
 
@@ -854,14 +856,14 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
     const uint32_t d = tmem + (uint32_t(quad * 32) << 16);
     const int row = row0 + quad * 32 + lane;
     int owner = half * 4 % p.split, slot = half * 4 / p.split;  // of this warp's next group of tokens
+    const int slots = (((count + 3) >> 2) - rank + p.split - 1) / p.split;  // groups that this CTA finishes
     const bool done = wt.wait_warp(&acc_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
     ptx::tcgen05_fence_after();
-    // Four tokens' results of this row (of each part).  Neighbouring lanes exchange two, so that each stores two rows
-    // of two tokens.
     constexpr bool kF32 = EPI == FDMOE_EPI_F32 || EPI == FDMOE_EPI_GATED_F32;
     const bool even_ld = (p.ld & 1) == 0;
-    auto finish = [&](int t, const float(&v)[kParts][4]) {
-      float y[4];
+    // Four tokens' results of this row.  Several groups' are computed before the first is stored: one after the other
+    // they took 800 cycles each, nearly all of it latency.
+    auto results = [&](const float(&v)[kParts][4], float(&y)[4]) {
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
         if constexpr (kGated)
@@ -869,6 +871,9 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
         else
           y[i] = v[0][i], y[i + 1] = v[0][i + 1];
       }
+    };
+    // Neighbouring lanes exchange two of the four, so that each stores two rows of two tokens.
+    auto store = [&](int t, const float(&y)[4]) {
       const int64_t at = (int64_t)(tok0 + t) * p.ld;
       if constexpr (kF32) {
 #pragma unroll
@@ -903,13 +908,20 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
           for (int q = 0; q < kParts; ++q) ptx::tmem_ld_32x16(d + q * nt + c, v[q]);
           ptx::tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            float f[kParts][4];
+          for (int i = 0; i < 16; i += 8) {
+            if (c + i >= count) break;
+            float y[2][4];
 #pragma unroll
-            for (int q = 0; q < kParts; ++q)
+            for (int g = 0; g < 2; ++g) {
+              float f[kParts][4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) f[q][j] = __uint_as_float(v[q][i + j]);
-            if (c + i < count) finish(c + i, f);
+              for (int q = 0; q < kParts; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[q][j] = __uint_as_float(v[q][i + 4 * g + j]);
+              results(f, y[g]);
+            }
+            store(c + i, y[0]);
+            store(c + i + 4, y[1]);
           }
         }
     } else {
@@ -943,21 +955,30 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
           for (owner += 4; owner >= p.split; owner -= p.split) ++slot;  // the other warp's four groups
         }
       ptx::epilogue_sync();
-      const bool have = rank * 4 < count && wt.wait_warp(&sums_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
-      for (slot = half; have && (slot * p.split + rank) * 4 < count; slot += 2) {
-        float f[kParts][4] = {};
-#pragma unroll 4
+      const bool have = slots > 0 && wt.wait_warp(&sums_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
+      auto finish = [&](auto groups, int slot) {
+        constexpr int kGroups = decltype(groups)::value;
+        float f[kGroups][kParts][4] = {}, y[kGroups][4];
+#pragma unroll(4 / kGroups)
         for (int r = 0; r < p.split; ++r)
 #pragma unroll
-          for (int q = 0; q < kParts; ++q) {
-            const float4 v = *reinterpret_cast<const float4*>(own + ((slot * p.split + r) * kParts + q) * 2048);
-            f[q][0] += v.x;
-            f[q][1] += v.y;
-            f[q][2] += v.z;
-            f[q][3] += v.w;
-          }
-        finish((slot * p.split + rank) * 4, f);
-      }
+          for (int q = 0; q < kParts; ++q)
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+              const float4 v = *reinterpret_cast<const float4*>(own + (((slot + 2 * g) * p.split + r) * kParts + q) * 2048);
+              f[g][q][0] += v.x;
+              f[g][q][1] += v.y;
+              f[g][q][2] += v.z;
+              f[g][q][3] += v.w;
+            }
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) results(f[g], y[g]);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) store(((slot + 2 * g) * p.split + rank) * 4, y[g]);
+      };
+      slot = have ? half : slots;
+      for (; slot + 2 < slots; slot += 4) finish(std::integral_constant<int, 2>(), slot);
+      if (slot < slots) finish(std::integral_constant<int, 1>(), slot);
     }
   }
   __syncwarp();
