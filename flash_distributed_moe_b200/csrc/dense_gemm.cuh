@@ -2,7 +2,7 @@
 // scale per 32 elements.  Two kernels:
 //
 //   pair_gemm    D[256 x 256], D[256 x 192] or D[256 x 128] tiles on pairs of CTAs.
-//   stream_gemm  the weights are the M operand (128 rows a tile), up to 160 tokens the N operand, and a cluster of
+//   stream_gemm  the weights are the M operand (128 rows a tile), up to 192 tokens the N operand, and a cluster of
 //                up to eight CTAs shares the k axis of a tile: for few tokens, where every byte of the weights is
 //                read once and that read has to be spread over all SMs.
 //

@@ -362,7 +362,7 @@ int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, 
   const int chunks = (int)fdmoe::ScaleChunks(k), up_block = (int)((rows + 127) / 128);
   const int epi = gated ? (dtype == kF32 ? FDMOE_EPI_GATED_F32 : FDMOE_EPI_GATED)
                         : (dtype == kF32 ? FDMOE_EPI_F32 : FDMOE_EPI_HALF);
-  if (fdmoe::UseStreamMx4(tokens) || (dtype == kF32 ? rows % 4 : rows % 8) != 0) {
+  if (fdmoe::UseStreamMx4(tokens, rows, gated) || (dtype == kF32 ? rows % 4 : rows % 8) != 0) {
     FdmoeStreamParams p;
     memset(&p, 0, sizeof(p));
     const fdmoe::StreamPlan s = fdmoe::MakeStreamPlan((int)rows, (int)tokens, kblocks, gated, true, *c.slots);

@@ -29,10 +29,11 @@ struct DeviceSlots {
 // `rows` weight rows (gated: of each projection), `tokens` >= 1, `kblocks` stages of k in all.
 //
 // Time in cycles.  A k block takes as long as its MMAs' issue, or as the weights of `active` CTAs do at the rate at which
-// their stages in flight are filled, at most the memory's 3500 bytes per cycle; a wave has a beginning and an end.  Two
-// CTAs per SM hide each other's beginning and end and issue at the same time, but have half the stages each.  Cold
-// weights, CTAs per tile of the two products of a block: 1 token of 2048 x 6144 22.7 us with 2 and 8, 21.3 with 4 and 8;
-// 32 tokens of 4096 x 12288 63.5 with 1 and 6, 56.3 with 2 and 8, and 59.6 with one CTA per SM, 1 and 4.
+// their stages in flight are filled, at most the memory's 3400 bytes per cycle; another wave of CTAs costs far more than
+// its k blocks.  The constants are those with which the choice is on average 0.7 % and at most 6 % slower than the best
+// of all splits with one and two CTAs per SM, over 124 products (1 to 128 tokens; 512 x 1024 to 8192 x 8192; cold
+// weights).  In us, with 2, 3, 4, 6 and 8 CTAs per tile: 64 tokens, gated, 4096 rows, k 1024 8.5, 8.5, 8.4, 11.0 and 11.0;
+// with 4 bits, 2048 rows, k 2048 6.8, 6.5, 6.1, 6.7 and 7.9; 1 token, 2048 rows, k 6144 12.7, 10.0, 8.7, 8.0 and 7.9.
 inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, bool mx4, const DeviceSlots& dev) {
   StreamPlan best = {};
   double best_time = 0;
@@ -52,19 +53,19 @@ inline StreamPlan MakeStreamPlan(int rows, int tokens, int kblocks, bool gated, 
     int most = std::min(room / stage, (int)FDMOE_STREAM_STAGES);
     if (scales) most = std::min(most, ((per_sm == 2 ? 256 : 512) - parts * s.tile_tokens) / scales);
     if (per_sm == 2 && (most < 2 || parts * s.tile_tokens > 256)) continue;
-    const double weights = parts * (mx4 ? 16384 + 1024 : 16384), issue = mx4 ? 430 + 210 * parts : 380 + 160 * parts;
+    const double weights = parts * (mx4 ? 16384 + 1024 : 16384), issue = mx4 ? 650 + 40 * parts : 560 + 160 * parts;
     for (int n = 1; n <= FDMOE_STREAM_SPLIT && n <= kblocks; ++n) {
       const int64_t slots = per_sm == 2 ? dev.stream_two[n] : dev.stream_one[n];
       if (slots < 1 || (n > 1 && sums > room)) continue;  // the device cannot hold such a cluster, or a CTA the sums
       const int blocks = (kblocks + n - 1) / n;
-      double t = per_sm == 1 ? 2000 : 0;  // the launches before and after it cannot overlap with it
+      double t = per_sm == 1 ? 250 : 0;  // the launches before and after it cannot overlap with it
       // the partial sums' way through the cluster's shared memory at 14 bytes per cycle, and the epilogue
-      t += (n > 1 ? 600 + 200 * n : 0) + s.tile_tokens * parts * (36.0 * (n - 1) + 20.0) / n;
+      t += (n > 1 ? 1000 + 250 * n : 0) + s.tile_tokens * parts * (42.0 * (n - 1) + 20.0) / n;
       int64_t clusters = (int64_t)s.row_tiles * s.token_tiles;
       for (int wave = 0; clusters > 0 && wave < 64; ++wave, clusters -= slots) {
         const double active = (double)std::min(clusters, slots) * n;
-        const double rate = std::min(3500.0, active * most * weights / 4000);
-        t += blocks * std::max(issue, active * weights / rate) + 5000;
+        const double rate = std::min(3400.0, active * most * weights / 4200);
+        t += blocks * std::max(issue, active * weights / rate) + 16000;
       }
       if (best_time != 0 && t >= best_time) continue;
       best_time = t;
@@ -205,16 +206,19 @@ inline ManyPlan MakeManyPlan(const ManyShape* shape, int n, const DeviceSlots& d
 
 // Whether the streaming kernel takes the products of `tokens` rows instead of the pair kernel.  It reads weights faster,
 // which counts by their bytes, and its partial sums and epilogue cost more with every token.  Whole block of `bytes` of
-// weights, streaming and pair kernels in us: 96 tokens of 512 x 1024 12.0 and 11.5, of 1024 x 4096 17.9 and 19.2, of
-// 2048 x 6144 27.6 and 30.5; 128 tokens of 1024 x 4096 19.8 and 19.3, of 2048 x 6144 30.4 and 31.0, of 4096 x 12288 68
-// and 84.6; 160 tokens of 2048 x 6144 32.6 and 30.7, of 4096 x 12288 73.8 and 85.7, of 8192 x 28672 303 and 304.
+// weights, streaming and pair kernels in us: 96 tokens of 512 x 1024 10.9 and 10.5, of 2048 x 768 12.7 and 13.9; 128
+// tokens of 2048 x 768 14.4 and 14.1, of 1024 x 4096 18.2 and 18.1, of 2048 x 6144 27.4 and 29.6; 160 tokens of
+// 2048 x 6144 29.7 and 29.7, of 4096 x 4096 32.2 and 34.0, of 4096 x 12288 66 and 83, of 8192 x 28672 249 and 289.
 inline bool UseStream(int64_t tokens, int64_t bytes) {
-  return tokens <= std::min<int64_t>(104 + (bytes >> 21), FDMOE_STREAM_TOKENS);
+  return tokens <= std::min<int64_t>(96 + (bytes >> 20), FDMOE_STREAM_TOKENS);
 }
-// 4-bit operands: one tile of tokens.  128 tokens times 4096 x 12288 (rows, columns) 13.0 and 15.4 us, 2048 x 6144 8.7
-// and 11.0, 28672 x 8192 28.7 and 31.7, 12288 x 4096 12.0 and 11.0; 160 tokens 14.8 and 15.3, 9.3 and 11.0, 45 and 32,
-// 13.9 and 10.9.
-inline bool UseStreamMx4(int64_t tokens) { return tokens <= FDMOE_STREAM_TOKENS_MX4; }
+// 4-bit operands: one tile of tokens, or two where the pair kernel's tiles leave most pairs idle.  128 tokens times
+// 4096 x 12288 (rows, columns) 10.3 and 14.1 us, 2048 x 6144 7.2 and 9.2, 12288 x 4096 10.8 and 10.7, gated 16.4 and
+// 18.2, gated 8192 x 8192 19.4 and 18.1; 256 tokens times 1024 x 4096 6.3 and 8.8, 4096 x 12288 13.3 and 14.2,
+// 8192 x 8192 14.5 and 13.7, gated 1024 x 4096 9.7 and 9.4.
+inline bool UseStreamMx4(int64_t tokens, int64_t rows, bool gated) {
+  return tokens <= (!gated && rows <= 4096 ? 2 * FDMOE_STREAM_TOKENS_MX4 : FDMOE_STREAM_TOKENS_MX4);
+}
 
 inline size_t AlignBytes(size_t v) { return (v + 255) / 256 * 256; }
 

@@ -28,7 +28,7 @@ def test_forward(tokens, hidden, inter, dtype):
     assert torch.equal(y, gated_ffn(x, w13, w2))  # the same call, the same bits
 
 
-@pytest.mark.parametrize("tokens", [97, 130, 147, 160, 161])
+@pytest.mark.parametrize("tokens", [97, 130, 147, 160, 161, 183, 192, 193])
 def test_more_tokens_of_large_weights(tokens):
     x, w13, w2, _ = dl.make(tokens, 4120, 5480, BF16, seed=10)  # 129 MB
     y = gated_ffn(x, w13, w2)
