@@ -133,6 +133,40 @@ __device__ __forceinline__ F2 from24(uint32_t upper, uint32_t lower) {
   return as_f2(__byte_perm(upper, lower, which ? 0x1055 : 0x1044), __byte_perm(upper, lower, which ? 0x3277 : 0x3266));
 }
 
+// Eight columns of a row: the activation from both projections, what is kept of them, and their gradients from dh.
+template <bool BF16>
+__device__ __forceinline__ uint4 gate8(const uint32_t* g, const uint32_t* u) {
+  uint32_t h[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) h[q] = pack2(gate(as_f2(g[2 * q], g[2 * q + 1]), as_f2(u[2 * q], u[2 * q + 1])), BF16);
+  return make_uint4(h[0], h[1], h[2], h[3]);
+}
+__device__ __forceinline__ void keep8(const uint32_t* g, const uint32_t* u, uint4& upper_g, uint4& upper_u, uint4& lower) {
+  upper_g = make_uint4(upper16(g[0], g[1]), upper16(g[2], g[3]), upper16(g[4], g[5]), upper16(g[6], g[7]));
+  upper_u = make_uint4(upper16(u[0], u[1]), upper16(u[2], u[3]), upper16(u[4], u[5]), upper16(u[6], u[7]));
+  lower = make_uint4(next8(g[0], u[0], g[1], u[1]), next8(g[2], u[2], g[3], u[3]), next8(g[4], u[4], g[5], u[5]),
+                     next8(g[6], u[6], g[7], u[7]));
+}
+template <bool BF16>
+__device__ __forceinline__ void gradient8(uint4 upper_g, uint4 upper_u, uint4 lower, const uint32_t* d, uint4& grad_g,
+                                          uint4& grad_u) {
+  const uint32_t gw[4] = {upper_g.x, upper_g.y, upper_g.z, upper_g.w}, uw[4] = {upper_u.x, upper_u.y, upper_u.z, upper_u.w};
+  const uint32_t lw[4] = {lower.x, lower.y, lower.z, lower.w};
+  uint32_t dg[4], du[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const F2 g = from24<0>(gw[q], lw[q]), u = from24<1>(uw[q], lw[q]);
+    const F2 dh = as_f2(d[2 * q], d[2 * q + 1]);
+    const F2 sg = sigmoid(g), silu = g * sg;
+    // silu' = s + g s (1 - s)
+    const F2 slope = fma2(silu, fma2(sg, F2(-1.0f, -1.0f), F2(1.0f, 1.0f)), sg);
+    dg[q] = pack2(dh * u * slope, BF16);
+    du[q] = pack2(dh * silu, BF16);
+  }
+  grad_g = make_uint4(dg[0], dg[1], dg[2], dg[3]);
+  grad_u = make_uint4(du[0], du[1], du[2], du[3]);
+}
+
 // -------------------------------------------------------------- pair kernel
 // A pair of CTAs works on D[256 x tile_n] tiles: CTA r holds rows [128 r, 128 r + 128) of A, of D, and half of the
 // rows of B (gated: CTA 0 the gate projection's, CTA 1 the up projection's, so that D holds tile_n / 2 columns of
@@ -392,12 +426,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
     const int w = warp - 4, quad = warp & 3;
     uint8_t* buf = staging + w * S::kStaging;
     const uint32_t sbuf = ptx::smem_u32(buf);
-    // Boxes of 32 rows and a group of columns are dealt out to the pairs and to their warps; box i is quarter i & 3 of
-    // the rows of group i >> 2, so that a pair on its own reads its warps' own lanes.
+    // Box i: 32 rows (quarter i & 3 of the CTA's, which are the warp's own lanes) of a group of columns (i >> 2).
     constexpr int kGroup = kF32 ? 32 : 64;
     constexpr int kMost = (kGated ? 128 : 256) / kGroup / 2;  // boxes of a warp
-    const int box0 = (int)part + split * w, box_step = 8 * split;
-    const auto box_at = [&](int j) { return box0 + j * box_step; };
+    const auto box_at = [&](int j) { return w + 8 * j; };
     // Gradient: the boxes first take the upper halves of g and u of a group of columns, which dg and du then replace;
     // the lower bytes of this lane's row come straight into registers.
     uint32_t gu_count = 0;
@@ -422,67 +454,126 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       const int half_n = pr.tile_n >> 1, tile_cols = kGated ? half_n : pr.tile_n, boxes = tile_cols / kGroup * 4;
       const int acc = n % S::kAccs;
       if constexpr (EPI == FDMOE_EPI_GATED_GRAD)
-        if (box_at(0) < boxes) fetch_gu(t, box_at(0));
-      bool done = wt.wait_warp(acc_full + acc, (n / S::kAccs) & 1, FDMOE_DENSE_TIMEOUT_DONE);
+        if (split == 1 && box_at(0) < boxes) fetch_gu(t, box_at(0));
+      const bool done = wt.wait_warp(acc_full + acc, (n / S::kAccs) & 1, FDMOE_DENSE_TIMEOUT_DONE);
       ptx::tcgen05_fence_after();
       const uint32_t d = tmem + acc * kAccCols + (uint32_t(quad * 32) << 16);
       const int tile_row = t.m * 256 + (int)rank * 128;
-      // Where the k axis is shared (a cluster's only tile) every pair stores its partial sums of a box into the shared
-      // memory of the box's owner, [box of the owner][pair][part][column / 4][row][4], where the stages were: all MMAs
-      // have read theirs once every CTA has arrived at the cluster's barrier.
-      constexpr int kParts = kGated ? 2 : 1, kBoxSums = kGroup * 128;  // bytes
-      const auto sums_at = [&](int box, int pair) { return ((box >> shift << shift) + pair) * kParts * kBoxSums; };
+      const int col0 = t.n * tile_cols;
       if (split > 1) {
+        // The k axis is shared, and this is the cluster's only tile.  Every pair stores its partial sums of a box into
+        // the shared memory of the box's owner, [box of the owner][pair][part][column / 4][row][4], where the stages
+        // were: all MMAs have read theirs once every CTA has arrived at the cluster's barrier.
+        constexpr int kParts = kGated ? 2 : 1, kBoxSums = kGroup * 128;  // bytes
+        // Each of the owner's eight warps then adds them, in the order of the pairs, for eight rows of a box at a time:
+        // eight lanes write 128 bytes of a row (a lane per row took eight times the stores' cycles, and whole boxes
+        // through the copy engine left most warps idle).  A row's place in its 512 bytes is turned by the eighth of
+        // the box's columns, so that such lanes read from different banks.
+        constexpr int kCols = kF32 ? 4 : 8;  // of a lane: 16 bytes of a result
+        const int quarters = boxes >> shift << 2, eighth = lane & 7;
+        int row, col;  // this lane's first row; the second is four further
+        const auto place = [&](int i) {
+          const int box = ((i >> 2) << shift) + (int)part;
+          row = tile_row + (box & 3) * 32 + (i & 3) * 8 + (lane >> 3), col = col0 + (box >> 2) * kGroup + eighth * kCols;
+        };
+        uint4 gu[3][2];
+        const auto fetch = [&](int i) {  // gradient: g, u and their lower bytes
+          place(i);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const bool in = i < quarters && row + 4 * k < pr.rows && col < pr.cols;
+            const int64_t at = (int64_t)(row + 4 * k) * pr.cols, at2 = 2 * at + col;
+            gu[0][k] = in ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.from[0]) + at2)) : uint4();
+            gu[1][k] = in ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.from[1]) + at2)) : uint4();
+            gu[2][k] = in ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.lower) + at + col)) : uint4();
+          }
+        };
+        if constexpr (EPI == FDMOE_EPI_GATED_GRAD) fetch(w);
         ptx::cluster_sync_relaxed();
         if (done)
           for (int c = w >> 2; c < pr.tile_n >> 5; c += 2) {
             uint32_t v[32];
             ptx::tmem_ld_32x32(d + c * 32, v);
-            const int q = kGated && c * 32 >= half_n, col = c * 32 - q * half_n, box = col / kGroup * 4 + quad;
+            const int q = kGated && c * 32 >= half_n, column = c * 32 - q * half_n, box = column / kGroup * 4 + quad;
             const uint32_t owner = box & (split - 1);
-            const uint32_t at = sums_at(box, part) + q * kBoxSums + (col % kGroup) * 128 + lane * 16;
+            const uint32_t at = (((box >> shift << shift) + part) * kParts + q) * kBoxSums + (column % kGroup) * 128;
             const uint32_t to = ptx::map_rank(ptx::smem_u32(stages) + at, 2 * owner + rank);
             const uint32_t bar = ptx::map_rank(ptx::smem_u32(sums_full), 2 * owner + rank);
             ptx::tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
+              const uint32_t on = j * 512 + (lane ^ (kF32 ? j : (column % kGroup) / 8 + j / 2)) * 16;
               if (owner == part)
-                *reinterpret_cast<uint4*>(stages + at + j * 512) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                *reinterpret_cast<uint4*>(stages + at + on) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
               else
-                ptx::st_async_u32x4(to + j * 512, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], bar);
+                ptx::st_async_u32x4(to + on, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], bar);
             }
           }
         ptx::epilogue_sync();
-        done = done && wt.wait_warp(sums_full, 0, FDMOE_DENSE_TIMEOUT_DONE);
-      }
-      if (!done) break;
-      // 32 columns (from `column` of part q on) of a box from the accumulator, or from all pairs' partial sums in the
-      // order of their ranks
-      auto load = [&](int box, int q, int column, uint32_t (&v)[32]) {
-        if (split == 1) {
-          ptx::tmem_ld_32x32(d + q * half_n + (box >> 2) * kGroup + column, v);
-          return;
-        }
-        const uint32_t from = ptx::smem_u32(stages) + sums_at(box, 0) + q * kBoxSums + column * 128 + lane * 16;
+        if (!done || !wt.wait_warp(sums_full, 0, FDMOE_DENSE_TIMEOUT_DONE)) break;
+        for (int i = w; i < quarters; i += 8) {
+          if (EPI == FDMOE_EPI_GATED_GRAD && i != w) fetch(i);
+          place(i);
+          uint32_t v[kParts][2][kCols];
+          const uint32_t from = ptx::smem_u32(stages) + ((i >> 2) << shift) * kParts * kBoxSums + eighth * kCols * 128;
+          const int turned = ((i & 3) * 8 + (lane >> 3)) ^ eighth;  // the second row, four further: bit 2 the other way
+          for (int r = 0; r < split; ++r)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float4 f = ptx::ld_shared_f32x4(from + j * 512);
-          v[4 * j] = __float_as_uint(f.x);
-          v[4 * j + 1] = __float_as_uint(f.y);
-          v[4 * j + 2] = __float_as_uint(f.z);
-          v[4 * j + 3] = __float_as_uint(f.w);
-        }
-#pragma unroll 1
-        for (int r = 1; r < split; ++r) {
+            for (int q = 0; q < kParts; ++q)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float4 f = ptx::ld_shared_f32x4(from + r * (kParts * kBoxSums) + j * 512);
-            v[4 * j] = __float_as_uint(__uint_as_float(v[4 * j]) + f.x);
-            v[4 * j + 1] = __float_as_uint(__uint_as_float(v[4 * j + 1]) + f.y);
-            v[4 * j + 2] = __float_as_uint(__uint_as_float(v[4 * j + 2]) + f.z);
-            v[4 * j + 3] = __float_as_uint(__uint_as_float(v[4 * j + 3]) + f.w);
+              for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int j = 0; j < kCols; j += 4) {
+                  const float4 f = ptx::ld_shared_f32x4(from + (r * kParts + q) * kBoxSums + j * 128 + (turned ^ (4 * k)) * 16);
+                  const float add[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    v[q][k][j + e] = __float_as_uint(r == 0 ? add[e] : __uint_as_float(v[q][k][j + e]) + add[e]);
+                }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t* const v0 = v[0][k];
+            const uint32_t* const v1 = v[kParts - 1][k];
+            const auto put = [&](void* to, int width, uint4 x) {  // 16 bytes; `to` has `width` times the columns
+              if (row + 4 * k < pr.rows && col < pr.cols)
+                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(to) + ((int64_t)(row + 4 * k) * pr.cols * width + col) * (kF32 ? 4 : 2)) = x;
+            };
+            if constexpr (kF32) {
+              float y[4];
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                const F2 a = as_f2(v0[e], v0[e + 1]);
+                (kGated ? gate(a, as_f2(v1[e], v1[e + 1])) : a).get(y[e], y[e + 1]);
+              }
+              put(p.to[0], 1, make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])));
+            } else if constexpr (kGated) {
+              put(p.to[0], 1, gate8<BF16>(v0, v1));
+              if constexpr (EPI == FDMOE_EPI_GATED_SAVE) {
+                uint4 x[3];
+                keep8(v0, v1, x[0], x[1], x[2]);
+                put(p.to[1], 2, x[0]);
+                put(p.to[2], 2, x[1]);
+                put(p.lower, 1, x[2]);
+              }
+            } else if constexpr (EPI == FDMOE_EPI_GATED_GRAD) {
+              uint4 x[2];
+              gradient8<BF16>(gu[0][k], gu[1][k], gu[2][k], v0, x[0], x[1]);
+              put(p.to[0], 2, x[0]);
+              put(p.to[1], 2, x[1]);
+            } else {
+              uint32_t h[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) h[e] = pack2(as_f2(v0[2 * e], v0[2 * e + 1]), BF16);
+              put(p.to[0], 1, make_uint4(h[0], h[1], h[2], h[3]));
+            }
           }
         }
+        break;
+      }
+      if (!done) break;
+      // 32 columns (from `column` of part q on) of a box from the accumulator
+      auto load = [&](int box, int q, int column, uint32_t (&v)[32]) {
+        ptx::tmem_ld_32x32(d + q * half_n + (box >> 2) * kGroup + column, v);
       };
       auto release = [&]() {  // this warp has read its part of the accumulator
         ptx::tcgen05_fence_before();
@@ -498,7 +589,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
         ptx::fence_proxy_async_shared();
         __syncwarp();
       };
-      const int col0 = t.n * tile_cols;
       // Sends buffer b, which all lanes have written, to where `box` lies in result `map`.
       auto send = [&](int map, int b, int box) {
         const int row = tile_row + (box & 3) * 32, col = col0 + (box >> 2) * kGroup;
@@ -605,25 +695,18 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {  // eight columns
-              uint32_t h[4], gw[4], lower[4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const int at = 8 * j + 2 * q;
-                h[q] = pack2(gate(as_f2(gi[at], gi[at + 1]), as_f2(ui[at], ui[at + 1])), BF16);
-                if constexpr (EPI == FDMOE_EPI_GATED_SAVE) {
-                  gw[q] = upper16(gi[at], gi[at + 1]);
-                  up[16 * i + 4 * j + q] = upper16(ui[at], ui[at + 1]);
-                  lower[q] = next8(gi[at], ui[at], gi[at + 1], ui[at + 1]);
-                }
-              }
-              stage16(buf, lane, i * 4 + j, h[0], h[1], h[2], h[3]);
+              const uint4 h = gate8<BF16>(gi + 8 * j, ui + 8 * j);
+              stage16(buf, lane, i * 4 + j, h.x, h.y, h.z, h.w);
               if constexpr (EPI == FDMOE_EPI_GATED_SAVE) {
-                stage16(buf + 4096, lane, i * 4 + j, gw[0], gw[1], gw[2], gw[3]);
+                uint4 upper_g, upper_u, lower;
+                keep8(gi + 8 * j, ui + 8 * j, upper_g, upper_u, lower);
+                stage16(buf + 4096, lane, i * 4 + j, upper_g.x, upper_g.y, upper_g.z, upper_g.w);
+                up[16 * i + 4 * j] = upper_u.x, up[16 * i + 4 * j + 1] = upper_u.y;
+                up[16 * i + 4 * j + 2] = upper_u.z, up[16 * i + 4 * j + 3] = upper_u.w;
                 const int row = tile_row + (box & 3) * 32 + lane;
                 const int col = col0 + (box >> 2) * 64 + i * 32 + j * 8;  // columns come in eights
                 if (row < pr.rows && col < pr.cols)
-                  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.lower) + (int64_t)row * pr.cols + col) =
-                      make_uint4(lower[0], lower[1], lower[2], lower[3]);
+                  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.lower) + (int64_t)row * pr.cols + col) = lower;
               }
             }
           }
@@ -663,22 +746,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
             for (int j = 0; j < 4; ++j) {  // eight columns
               uint4* const g_at = reinterpret_cast<uint4*>(buf + lane * 128 + (((i * 4 + j) ^ (lane & 7)) << 4));
               uint4* const u_at = g_at + 4096 / 16;
-              const uint4 g4 = *g_at, u4 = *u_at, l4 = lower[i * 4 + j];
-              const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
-              const uint32_t lw[4] = {l4.x, l4.y, l4.z, l4.w};
-              uint32_t dg[4], du[4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const F2 g = from24<0>(gw[q], lw[q]), u = from24<1>(uw[q], lw[q]);
-                const F2 dh = as_f2(v[8 * j + 2 * q], v[8 * j + 2 * q + 1]);
-                const F2 sg = sigmoid(g), silu = g * sg;
-                // silu' = s + g s (1 - s)
-                const F2 slope = fma2(silu, fma2(sg, F2(-1.0f, -1.0f), F2(1.0f, 1.0f)), sg);
-                dg[q] = pack2(dh * u * slope, BF16);
-                du[q] = pack2(dh * silu, BF16);
-              }
-              *g_at = make_uint4(dg[0], dg[1], dg[2], dg[3]);
-              *u_at = make_uint4(du[0], du[1], du[2], du[3]);
+              uint4 dg, du;
+              gradient8<BF16>(*g_at, *u_at, lower[i * 4 + j], v + 8 * j, dg, du);
+              *g_at = dg;
+              *u_at = du;
             }
           }
           boxes_written();

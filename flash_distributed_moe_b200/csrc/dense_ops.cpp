@@ -196,6 +196,7 @@ int PairProduct(const Call& c, const Product& w, bool bf16) {
   memset(&p, 0, sizeof(p));
   const int clusters = PairShape(p, c, w.rows(), w.cols(), w.k(), false, false);
   DENSE_TRY(ProductMaps(c, p.product[0], w));
+  p.to[0] = w.out;
   p.bf16 = bf16;
   return fdmoe_pair_launch(&p, FDMOE_EPI_HALF, 0, clusters, c.stream);
 }
@@ -310,10 +311,13 @@ int GatedProduct(const Call& c, const void* x, const void* w13, void* h, const S
   DENSE_TRY(MakeMap(c, &q.a, x, 2, T, H, H * 2, 64, 128));
   DENSE_TRY(MakeMap(c, &q.b, w13, 2, 2 * I, H, H * 2, 64, q.tile_n / 2));
   DENSE_TRY(MakeMap(c, &q.out[0], h, 2, T, I, I * 2, 64, 32));
+  p.to[0] = h;
   if (saved.gu) {
     // two matrices side by side: what a tile has beyond column I of the gate projection is not stored
     DENSE_TRY(MakeMap(c, &q.out[1], saved.gu, 2, T, I, I * 4, 64, 32));
     DENSE_TRY(MakeMap(c, &q.out[2], saved.gu + I * 2, 2, T, I, I * 4, 64, 32));
+    p.to[1] = saved.gu;
+    p.to[2] = saved.gu + I * 2;
     p.lower = saved.lower;
   }
   p.up_row = (int32_t)I;
@@ -334,6 +338,8 @@ int GatedGradient(const Call& c, const void* dy, const void* w2, const Saved& sa
   for (int i = 0; i < 2; ++i) {
     DENSE_TRY(MakeMap(c, &p.gu[i], saved.gu + i * I * 2, 2, T, I, I * 4, 64, 32));
     DENSE_TRY(MakeMap(c, &q.out[i], static_cast<uint8_t*>(dgu) + i * I * 2, 2, T, I, I * 4, 64, 32));
+    p.from[i] = saved.gu + i * I * 2;
+    p.to[i] = static_cast<uint8_t*>(dgu) + i * I * 2;
   }
   p.lower = saved.lower;
   q.b_mn = 1;
@@ -394,6 +400,7 @@ int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, 
   DENSE_TRY(Mx4Maps(c, &p.product[0].b, &p.sfb, b, k, 128));
   const int size = dtype == kF32 ? 4 : 2;
   DENSE_TRY(MakeMap(c, &p.product[0].out[0], out, size, tokens, rows, rows * size, 128 / size, 32));
+  p.to[0] = out;
   p.up_row = (int32_t)rows;
   p.sf_chunks = chunks;
   p.sf_up_block = up_block;

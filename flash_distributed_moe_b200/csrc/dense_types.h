@@ -59,6 +59,8 @@ typedef struct {
   FdmoeTensorMap sfa, sfb;    // scales of 4-bit operands
   FdmoeTensorMap gu[2];       // upper halves of gate and up projections (FDMOE_EPI_GATED_GRAD)
   void* lower;                // [rows, cols] lower bytes of both (FDMOE_EPI_GATED_SAVE and FDMOE_EPI_GATED_GRAD)
+  void* to[3];                // product[0].out and `gu` as pointers, for tiles whose k axis is shared
+  const void* from[2];
   uint32_t* status;
   uint64_t timeout_ns;
   int32_t products;           // above 1: FDMOE_EPI_HALF, `split` 1, tiles dealt out by `count`
