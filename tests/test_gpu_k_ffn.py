@@ -261,12 +261,13 @@ def test_wrapper_runs_a_dense_block():
         FlashFfnBlockWrapper(m)
 
 
-def test_a_wait_that_runs_out(monkeypatch):
-    x, w13, w2, _ = dl.make(300, 256, 256, BF16)
+@pytest.mark.parametrize("hidden,inter", [(256, 256), (2048, 128)])  # the second with a shared k axis
+def test_a_wait_that_runs_out(monkeypatch, hidden, inter):
+    x, w13, w2, _ = dl.make(300, hidden, inter, BF16)
     want = gated_ffn(x, w13, w2)
     torch.cuda.synchronize()
     monkeypatch.setenv("FLASHMOE_TIMEOUT_MS", "50")
-    lib, cfg = _lib.lib(), C.byref(_lib.FlashMoeFfnConfig(256, 256, 0, (C.c_int32 * 5)()))
+    lib, cfg = _lib.lib(), C.byref(_lib.FlashMoeFfnConfig(hidden, inter, 0, (C.c_int32 * 5)()))
     ws = torch.empty(lib.FlashMoeFfnWorkspaceBytes(cfg, 300, 0), dtype=torch.uint8, device="cuda")
     y = torch.empty_like(x)
     assert lib.FlashMoeTestFfnStall(cfg, x.data_ptr(), w13.data_ptr(), w2.data_ptr(), y.data_ptr(), ws.data_ptr(), ws.numel(),
