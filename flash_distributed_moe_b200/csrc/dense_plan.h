@@ -92,7 +92,8 @@ struct PairPlan {
 inline double BlockCycles(int tile_n) { return tile_n == 256 ? 520 : tile_n == 192 ? 455 : 365; }
 
 // `cols`: of the result; `kblocks` stages of k.  Time in cycles: the waves of tiles, each its k blocks (about 520,
-// 455 and 365 cycles at widths of 256, 192 and 128) and once per launch, or per cluster where pairs share a tile, its
+// 455 and 365 cycles at widths of 256, 192 and 128: what a stage's operands take to be written to and read from shared
+// memory, 128 bytes a cycle, is 512, 448 and 384, and its MMAs 512, 384 and 256) and once per launch, or per cluster where pairs share a tile, its
 // beginning and end; sharing also takes the partial sums' way through the cluster's shared memory, at 14 bytes a cycle.
 // In us, for width / pairs per tile: 4096 x 2048 x 6144 (rows, columns, k) 69 with 256/1, 80 with 192/1, 95 with
 // 128/1, 90 with 256/2; 777 x 1000 x 5488 36, 32, 28 and 24, 19 with 128/2, 36 with 128/4.
