@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       const uint16_t* at = static_cast<const uint16_t*>(p.lower) + (int64_t)row * pr.cols + col;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        lower[j] = row < pr.rows && col + 8 * j < pr.cols ? __ldg(reinterpret_cast<const uint4*>(at) + j) : make_uint4(0, 0, 0, 0);
+        lower[j] = row < pr.rows && col + 8 * j < pr.cols ? ptx::ld_global_u32x4(at + 8 * j) : make_uint4(0, 0, 0, 0);
       if (elected) {
         ptx::bulk_wait_group_read0();
         ptx::mbar_expect_tx(gu_full + w, 8192);
@@ -483,9 +483,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
           for (int k = 0; k < 2; ++k) {
             const bool in = i < quarters && row + 4 * k < pr.rows && col < pr.cols;
             const int64_t at = (int64_t)(row + 4 * k) * pr.cols, at2 = 2 * at + col;
-            gu[0][k] = in ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.from[0]) + at2)) : uint4();
-            gu[1][k] = in ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.from[1]) + at2)) : uint4();
-            gu[2][k] = in ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.lower) + at + col)) : uint4();
+            gu[0][k] = in ? ptx::ld_global_u32x4(static_cast<const uint16_t*>(p.from[0]) + at2) : uint4();
+            gu[1][k] = in ? ptx::ld_global_u32x4(static_cast<const uint16_t*>(p.from[1]) + at2) : uint4();
+            gu[2][k] = in ? ptx::ld_global_u32x4(static_cast<const uint16_t*>(p.lower) + at + col) : uint4();
           }
         };
         if constexpr (EPI == FDMOE_EPI_GATED_GRAD) fetch(w);

@@ -28,7 +28,7 @@ struct Eight {
   uint4 w[T == kF32 ? 2 : 1];
   __device__ __forceinline__ void load(const uint8_t* at) {
 #pragma unroll
-    for (int i = 0; i < (T == kF32 ? 2 : 1); ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
+    for (int i = 0; i < (T == kF32 ? 2 : 1); ++i) w[i] = ptx::ld_global_u32x4(at + 16 * i);
   }
   // Bits of the largest magnitude, as stored: infinities and NaN are above every number.
   __device__ __forceinline__ uint32_t top() const {
@@ -172,10 +172,10 @@ __global__ void __launch_bounds__(kQuantThreads) mx4_dequantize_kernel(const Deq
   uint32_t in[kRows];
 #pragma unroll
   for (int i = 0; i < kRows; ++i)
-    if (in_cols && r0 + i * kQuantStep < rows) in[i] = __ldg(reinterpret_cast<const uint32_t*>(p.values + ((at + i * step) >> 1)));
+    if (in_cols && r0 + i * kQuantStep < rows) in[i] = ptx::ld_global_u32(p.values + ((at + i * step) >> 1));
   if (threadIdx.x < kScaleBlock / 16) {
     const uint8_t* src = p.scales + ((batch * gridDim.x + blockIdx.x) * gridDim.y + blockIdx.y) * kScaleBlock;
-    reinterpret_cast<uint4*>(sc)[threadIdx.x] = __ldg(reinterpret_cast<const uint4*>(src) + threadIdx.x);
+    reinterpret_cast<uint4*>(sc)[threadIdx.x] = ptx::ld_global_u32x4(src + 16 * threadIdx.x);
   }
   __syncthreads();
   if (!in_cols) return;

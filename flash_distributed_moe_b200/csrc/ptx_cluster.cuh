@@ -134,6 +134,20 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint32_t leader)
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_wait_dependency() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Loads of what an earlier launch has written.  A kernel that starts before the launch before it has ended may not read
+// that launch's results through the read-only path: what is loaded there has to be constant while the kernel runs, and
+// such a load may be moved above grid_wait_dependency.  These are coherent, read L2 and keep their place behind it.
+__device__ __forceinline__ uint4 ld_global_u32x4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_global_u32(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
 // ------------------------------------------------------------- descriptors
 // Shared-memory matrix descriptor with 128-byte swizzle.  A tile whose rows run along K: rows of 128 bytes, groups of
 // eight rows 1024 bytes apart (`lead` unused).  A tile whose rows run along M or N: rows of 64 elements of one k,

@@ -1,0 +1,25 @@
+"""What the kernels of the dense operators have to keep to and no run can show: read from their sources."""
+import os
+import re
+
+import moe_testlib as tl
+
+CSRC = os.path.join(tl.ROOT, "flash_distributed_moe_b200", "csrc")
+KERNELS = ("dense_gemm.cuh", "dense_kernels.cu", "dense_launch.cuh", "mx4_kernels.cu", "ptx_cluster.cuh")
+
+
+def source(name):
+    """A source file without its comments."""
+    with open(os.path.join(CSRC, name)) as f:
+        return re.sub(r"//[^\n]*", "", f.read())
+
+
+def test_no_read_only_loads_in_kernels_that_start_early():
+    """Every launch may start while the launch before it still writes what it is going to read."""
+    assert "programmaticStreamSerializationAllowed = 1" in source("dense_launch.cuh")
+    for name in KERNELS:
+        text = source(name)
+        for word in ("__ldg", "ld.global.nc", "__restrict__", "__ldca", "__ldcs", "__ldlu"):
+            assert word not in text, f"{name}: {word}"
+    for load in re.findall(r'asm\s*(\w*)\("(ld\.global[^"]*)".*?;\n', source("ptx_cluster.cuh"), re.S):
+        assert load[0] == "volatile", load
