@@ -24,9 +24,10 @@ namespace dense {
 // Every wait ends: after `limit_ns` it records what it waited for, raises the CTA's abort flag, and all roles leave.
 // The warps that issue copies and MMAs run their loops with all lanes and let one elected lane issue: inside a branch
 // on the lane the compiler cannot tell that one thread is active, and instructions whose operands have to be uniform
-// cost several times as much (the pair kernel's k block took 684 cycles so, whatever the tile's width; it takes 365 at a
-// width of up to 192 and 520 at 256, where the tensor cores set the pace).  Their lanes wait each for itself: a vote
-// after every wait cost 40 cycles per k block.
+// cost several times as much (the pair kernel's k block took 684 cycles so, whatever the tile's width).  Their lanes
+// come together after every wait: a lane that fell behind by a whole ring of stages would look at a parity that had
+// flipped twice, and wait for a phase that does not come.  For that all lanes make the same number of steps, also after
+// a wait that ran out, which stops the waits and the issuing only.
 struct Waiter {
   volatile uint32_t* abort_flag;
   uint32_t* status;
@@ -39,6 +40,12 @@ struct Waiter {
   // The same by a whole warp that goes on together.
   __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, uint32_t code) const {
     return __all_sync(0xffffffffu, wait(bar, parity, code));
+  }
+  // The same by the lanes of a warp that issues, each with its own answer; `ok`: none of this lane's has run out yet.
+  __device__ __forceinline__ bool wait_together(uint64_t* bar, uint32_t parity, uint32_t code, bool ok) const {
+    if (ok) ok = wait(bar, parity, code);
+    __syncwarp();
+    return ok;
   }
   __device__ __noinline__ bool slow(uint64_t* bar, uint32_t parity, uint32_t code) const {
     const uint64_t t0 = ptx::globaltimer_ns();
@@ -319,7 +326,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       int stage = 0;
       uint32_t parity = 1;
       bool ok = true;
-      for (int i = 0; ok && have; have = tile_at(++i, g, t)) {
+      for (int i = 0; have; have = tile_at(++i, g, t)) {
         const FdmoePairProduct& pr = p.product[g];
         const int half_n = pr.tile_n >> 1;  // rows of B per CTA; gated: columns of each projection
         const int kb0 = pr.kblocks * (int)part >> shift, kb1 = pr.kblocks * ((int)part + 1) >> shift;
@@ -329,12 +336,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
         const int bx = kGated ? t.n * half_n + (int)rank * p.up_row : t.n * pr.tile_n + (int)rank * half_n;
         for (int kb = kb0; kb < kb1; ++kb) {
           const int s = stage;
-          if (!wt.wait(empty + s, parity, FDMOE_DENSE_TIMEOUT_EMPTY)) {
-            ok = false;
-            break;
-          }
+          ok = wt.wait_together(empty + s, parity, FDMOE_DENSE_TIMEOUT_EMPTY, ok);
           if (++stage == S::kStages) stage = 0, parity ^= 1;
-          if (p.stall || !elected) continue;
+          if (!ok || p.stall || !elected) continue;
           if (rank == 0) ptx::mbar_expect_tx(full + s, 2 * (kStageOperand + b_bytes + S::kScales));
           const uint32_t bar = ptx::map_rank(ptx::smem_u32(full + s), leader);
           const uint32_t sa = ptx::smem_u32(stages + s * 2 * kStageOperand), sb = sa + kStageOperand;
@@ -372,7 +376,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
       int stage = 0;
       uint32_t parity = 0;
       bool ok = true;
-      for (int n = 0; ok && have; have = tile_at(++n, g, t)) {
+      for (int n = 0; have; have = tile_at(++n, g, t)) {
         const FdmoePairProduct& pr = p.product[g];
         const int kb0 = pr.kblocks * (int)part >> shift, kb1 = pr.kblocks * ((int)part + 1) >> shift;
         const uint32_t idesc = ptx::make_idesc_f16(256, pr.tile_n, BF16, pr.a_mn, pr.b_mn);
@@ -381,18 +385,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
         const uint32_t a_lead = pr.a_mn ? 8192 : 16, b_lead = pr.b_mn ? 8192 : 16;
         const int acc = n % S::kAccs;
         const uint32_t aph = (n / S::kAccs) & 1;
-        if (!wt.wait(acc_empty + acc, aph ^ 1, FDMOE_DENSE_TIMEOUT_ACC)) break;
+        ok = wt.wait_together(acc_empty + acc, aph ^ 1, FDMOE_DENSE_TIMEOUT_ACC, ok);
         ptx::tcgen05_fence_after();
         const uint32_t d = tmem + acc * kAccCols;
         for (int kb = kb0; kb < kb1; ++kb) {
           const int s = stage;
-          if (!wt.wait(full + s, parity, FDMOE_DENSE_TIMEOUT_FULL)) {
-            ok = false;
-            break;
-          }
+          ok = wt.wait_together(full + s, parity, FDMOE_DENSE_TIMEOUT_FULL, ok);
           if (++stage == S::kStages) stage = 0, parity ^= 1;
           ptx::tcgen05_fence_after();
-          if (!elected) continue;
+          if (!ok || !elected) continue;
           const uint32_t sa = ptx::smem_u32(stages + s * 2 * kStageOperand), sb = sa + kStageOperand;
           if (MX4) {
             const uint32_t sf = ptx::smem_u32(scales + s * S::kScales);
@@ -868,9 +869,10 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
   if (warp == kStreamLoads) {
     int s = 0;
     uint32_t parity = 0;
+    bool ok = true;
     for (int kb = kb0 + filled; kb < kb1; ++kb) {
-      if (!wt.wait(empty + s, parity, FDMOE_DENSE_TIMEOUT_EMPTY)) break;
-      if (elected) {
+      ok = wt.wait_together(empty + s, parity, FDMOE_DENSE_TIMEOUT_EMPTY, ok);
+      if (ok && elected) {
         load_weights(s, kb);
         load_tokens(s, kb);
       }
@@ -883,13 +885,10 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
       uint32_t parity = 0;
       for (int i = 0, stage = 0; i < kb1 - kb0; ++i) {
         const int s = stage;
-        if (!wt.wait(full + s, parity, FDMOE_DENSE_TIMEOUT_FULL)) {
-          ok = false;
-          break;
-        }
+        ok = wt.wait_together(full + s, parity, FDMOE_DENSE_TIMEOUT_FULL, ok);
         if (++stage == p.stages) stage = 0, parity ^= 1;
         ptx::tcgen05_fence_after();
-        if (!elected) continue;
+        if (!ok || !elected) continue;
         const uint32_t sa = ptx::smem_u32(smem + s * stage_bytes), sb = sa + kParts * kStageOperand;
         const uint64_t db = ptx::smem_desc_sw128(sb, 16);
         if (MX4) {

@@ -23,3 +23,17 @@ def test_no_read_only_loads_in_kernels_that_start_early():
             assert word not in text, f"{name}: {word}"
     for load in re.findall(r'asm\s*(\w*)\("(ld\.global[^"]*)".*?;\n', source("ptx_cluster.cuh"), re.S):
         assert load[0] == "volatile", load
+
+
+def test_lanes_that_issue_come_together_after_every_wait():
+    """A lane left behind by a whole ring of stages would wait for a phase that is over; nothing but the source makes the
+    lanes of a warp go on together.  So no role waits lane by lane, and no lane leaves a loop of waits before the others."""
+    text = source("dense_gemm.cuh")
+    waiter, kernels = text[:text.index("pack2(")], text[text.index("pack2("):]
+    assert re.search(r"bool wait_together\([^)]*\) const \{\s*if \(ok\) ok = wait\([^)]*\);\s*__syncwarp\(\);\s*return ok;", waiter)
+    assert re.search(r"bool wait_warp\([^)]*\) const \{\s*return __all_sync\(", waiter)
+    calls = re.findall(r"wt\.(wait\w*|slow)\(", kernels)
+    assert calls.count("wait_together") == 5 and set(calls) == {"wait_together", "wait_warp"}
+    for call in re.finditer(r"(\S+) = wt\.wait_together\([^;]*, (\w+)\);", kernels):
+        assert call.group(1) == call.group(2) == "ok"
+    assert not re.search(r"for \([^;]*; *ok\b", kernels)
