@@ -30,7 +30,7 @@ def test_lanes_that_issue_come_together_after_every_wait():
     lanes of a warp go on together.  So no role waits lane by lane, and no lane leaves a loop of waits before the others."""
     text = source("dense_gemm.cuh")
     waiter, kernels = text[:text.index("pack2(")], text[text.index("pack2("):]
-    assert re.search(r"bool wait_together\([^)]*\) const \{\s*if \(ok\) ok = wait\([^)]*\);\s*__syncwarp\(\);\s*return ok;", waiter)
+    assert re.search(r"bool wait_together\([^)]*\) const \{\s*if \(__all_sync\([^;]*\)\) return true;\s*if \(ok\) ok = wait\([^)]*\);\s*__syncwarp\(\);\s*return ok;", waiter)
     assert re.search(r"bool wait_warp\([^)]*\) const \{\s*return __all_sync\(", waiter)
     calls = re.findall(r"wt\.(wait\w*|slow)\(", kernels)
     assert calls.count("wait_together") == 5 and set(calls) == {"wait_together", "wait_warp"}
