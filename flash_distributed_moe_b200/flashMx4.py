@@ -60,6 +60,10 @@ class Mx4Tensor:
         self._tensors, self._buffer, self._pointers = None, buffer, pointers
         return self
 
+    def __reduce__(self):
+        # copies and unpickled matrices have memory of their own, and with it addresses of their own
+        return Mx4Tensor, (self.values, self.scales)
+
     def _split(self):
         if self._tensors is None:
             n = self.shape.numel() // 2
