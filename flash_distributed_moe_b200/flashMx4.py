@@ -12,6 +12,7 @@ None of these functions has a gradient.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -22,6 +23,15 @@ def _check_dtype(dtype: torch.dtype) -> int:
     if dtype not in DTYPES:
         raise RuntimeError("dtype must be bfloat16, float16 or float32")
     return DTYPES[dtype]
+
+
+def check_no_tangent(*tensors) -> None:
+    """Forward-mode derivatives are refused: a result without a tangent would stand for a derivative of zero."""
+    if forward_ad._current_level < 0:  # no dual tensors outside a level
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("forward-mode derivatives are not supported")
 
 
 def _scale_bytes(batch: int, rows: int, cols: int) -> int:
@@ -96,6 +106,7 @@ def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
         raise RuntimeError("x tensor is undefined")
     if not x.is_cuda:
         raise RuntimeError("x must be a CUDA tensor")
+    check_no_tangent(x)
     code, shape, device = _check_dtype(x.dtype), x.shape, x.device
     if len(shape) not in (2, 3) or shape[-1] == 0 or shape[-1] % 32 != 0:
         raise RuntimeError("x must be [rows, cols] or [batch, rows, cols] with cols a multiple of 32")
