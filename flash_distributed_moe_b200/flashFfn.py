@@ -14,7 +14,7 @@ from typing import Tuple, Union
 import torch
 
 from . import _lib
-from .flashMx4 import Mx4Tensor, check_no_tangent, mx4_quantize
+from .flashMx4 import Mx4Tensor, check_no_tangent, check_not_traced, mx4_quantize
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 2}
 Weight = Union[torch.Tensor, Mx4Tensor]
@@ -110,6 +110,7 @@ def gated_ffn(x: torch.Tensor, w13: Weight, w2: Weight) -> torch.Tensor:
     _check(x, "x")
     if x.dim() < 1:
         raise RuntimeError("x must be [..., hidden]")
+    check_not_traced()
     check_no_tangent(x, w13, w2)
     if isinstance(w13, Mx4Tensor) or isinstance(w2, Mx4Tensor):
         return _mx4_ffn(x, w13, w2)

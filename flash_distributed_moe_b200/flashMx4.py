@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib
 
@@ -32,6 +33,13 @@ def check_no_tangent(*tensors) -> None:
     for t in tensors:
         if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
             raise RuntimeError("forward-mode derivatives are not supported")
+
+
+def check_not_traced() -> None:
+    """A recorder of torch operators (torch.jit.trace, make_fx) sees the allocation of a result and not the call that fills
+    it: its program would return memory as it is found.  torch.compile runs these calls between its graphs."""
+    if torch.jit.is_tracing() or (torch._C._len_torch_dispatch_stack() > 0 and get_proxy_mode() is not None):
+        raise RuntimeError("the dense operators cannot be recorded by torch.jit.trace or make_fx")
 
 
 def _scale_bytes(batch: int, rows: int, cols: int) -> int:
@@ -90,6 +98,7 @@ class Mx4Tensor:
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values that the matrix stands for.  Exact in fp32; in bf16 and fp16 unless they leave the type's range."""
+        check_not_traced()
         code, shape, device = _check_dtype(dtype), self.shape, self.device
         if device.type != "cuda":
             raise RuntimeError("values must be a CUDA tensor")
@@ -106,6 +115,7 @@ def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
         raise RuntimeError("x tensor is undefined")
     if not x.is_cuda:
         raise RuntimeError("x must be a CUDA tensor")
+    check_not_traced()
     check_no_tangent(x)
     code, shape, device = _check_dtype(x.dtype), x.shape, x.device
     if len(shape) not in (2, 3) or shape[-1] == 0 or shape[-1] % 32 != 0:
@@ -131,6 +141,7 @@ def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
 def _product(a: Mx4Tensor, b: Mx4Tensor, out_dtype: torch.dtype, gated: bool) -> torch.Tensor:
     if not isinstance(a, Mx4Tensor) or not isinstance(b, Mx4Tensor):
         raise RuntimeError("operands must be Mx4Tensors")
+    check_not_traced()
     code = _check_dtype(out_dtype)
     device, sa, sb = a.device, a.shape, b.shape
     if device != b.device or device.type != "cuda":

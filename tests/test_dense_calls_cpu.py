@@ -7,7 +7,8 @@ import pytest
 import torch
 
 import moe_testlib  # noqa: F401  (sets sys.path)
-from flash_distributed_moe_b200 import Mx4Tensor, gated_ffn, mx4_quantize, quantize_ffn_weights
+from flash_distributed_moe_b200 import (Mx4Tensor, gated_ffn, mx4_gated_matmul, mx4_matmul, mx4_quantize,
+                                        quantize_ffn_weights)
 
 
 def matrix(*shape, seed=0):
@@ -97,3 +98,51 @@ def test_forward_mode_derivatives_are_refused(calls):
         with pytest.raises(RuntimeError, match="forward-mode"):
             quantize_ffn_weights(args[1], fw.make_dual(args[2], torch.ones_like(args[2])))
     assert calls == ["FlashMoeFfnForward", "FlashMoeMx4Quantize"]  # the weights of the last call that are no dual tensor
+
+
+def recorders():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    return {"trace": lambda f, x: torch.jit.trace(f, x, check_trace=False), "make_fx": lambda f, x: make_fx(f)(x),
+            "make_fx symbolic": lambda f, x: make_fx(f, tracing_mode="symbolic")(x), "export": lambda f, x: torch.export.export(Call(f), (x,))}
+
+
+class Call(torch.nn.Module):
+    def __init__(self, f):
+        super().__init__()
+        self.forward = f
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("recorder", sorted(recorders()))
+def test_recorders_of_operators_are_refused(calls, monkeypatch, recorder):
+    """They would record the allocation of the result and not the call that fills it."""
+    from flash_distributed_moe_b200 import flashFfn
+    monkeypatch.setattr(flashFfn, "_check", lambda t, name: None)  # recorders' own tensors are not OnGpu
+    x, w13, w2 = (t.as_subclass(torch.Tensor) for t in block())
+    q, q13 = matrix(64, 64), matrix(2, 64, 64)
+    q.device = q13.device = torch.device("cuda", 0)
+
+    def through(f):
+        with pytest.raises(Exception, match="cannot be recorded|FakeTensor|Unsupported|data_ptr|data pointer|not supported"):
+            recorders()[recorder](f, x)
+
+    through(lambda a: gated_ffn(a, w13, w2))
+    through(lambda a: gated_ffn(a.clone().requires_grad_(), w13, w2))
+    if recorder in ("trace", "make_fx"):
+        through(lambda a: mx4_quantize(on_gpu(a)).values)
+        monkeypatch.setattr(torch, "empty", lambda *s, **k: torch.zeros(*s, dtype=k["dtype"]))
+        through(lambda a: a + q.dequantize())
+        through(lambda a: a + mx4_matmul(q, q))
+        through(lambda a: a + mx4_gated_matmul(q, q13))
+    assert not calls
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_compiled_programs_make_the_call(calls, monkeypatch):
+    from flash_distributed_moe_b200 import flashFfn
+    monkeypatch.setattr(flashFfn, "_check", lambda t, name: None)
+    x, w13, w2 = (t.as_subclass(torch.Tensor) for t in block())
+    for grad in (False, True):
+        f = torch.compile(lambda a: gated_ffn(2 * a, w13, w2) + 1, backend="eager")
+        assert f(x.clone().requires_grad_(grad)).requires_grad == grad
+    assert calls == ["FlashMoeFfnForward"] * 2
