@@ -7,7 +7,8 @@
 The values are E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), the scales E8M0; a block's scale is
 2^(floor(log2(largest magnitude)) - 2), elements are rounded to nearest even and saturate at 6, and a block that
 holds a NaN or an infinity stands for NaN.  Products are exact in their operands and accumulated in fp32.
-None of these functions has a gradient.
+None of these functions has a gradient: 4-bit weights are constants, and a product refuses activations whose origin needs
+one, where gradients are on.
 """
 from __future__ import annotations
 
@@ -52,7 +53,7 @@ class Mx4Tensor:
     even element in the low half of a byte; `scales` uint8, in blocks of 512 for 128 rows and 128 columns, where those of
     columns that do not exist are not 255 (which stands for NaN; mx4_quantize writes 0)."""
 
-    __slots__ = ("shape", "device", "_tensors", "_buffer", "_pointers")
+    __slots__ = ("shape", "device", "_tensors", "_buffer", "_pointers", "_needs_gradient")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
         for t, name in ((values, "values"), (scales, "scales")):
@@ -69,18 +70,20 @@ class Mx4Tensor:
         self.device = values.device
         self._tensors, self._buffer = (values, scales), None
         self._pointers = values.data_ptr(), scales.data_ptr()
+        self._needs_gradient = False
 
     @classmethod
-    def _of_buffer(cls, buffer: torch.Tensor, shape: torch.Size, pointers) -> "Mx4Tensor":
+    def _of_buffer(cls, buffer: torch.Tensor, shape: torch.Size, pointers, needs_gradient: bool = False) -> "Mx4Tensor":
         """Values and scales one after the other in a buffer of the right size."""
         self = cls.__new__(cls)
         self.shape, self.device = shape, buffer.device
         self._tensors, self._buffer, self._pointers = None, buffer, pointers
+        self._needs_gradient = needs_gradient
         return self
 
     def __reduce__(self):
         # copies and unpickled matrices have memory of their own, and with it addresses of their own
-        return Mx4Tensor, (self.values, self.scales)
+        return Mx4Tensor, (self.values, self.scales), (None, {"_needs_gradient": self._needs_gradient})
 
     def _split(self):
         if self._tensors is None:
@@ -110,7 +113,8 @@ class Mx4Tensor:
 
 def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
     """x [rows, cols] or [batch, rows, cols], bf16, fp16 or fp32, cols a multiple of 32; rows may be strided if they
-    start on 16 bytes.  Asynchronous on the current torch stream of x's device."""
+    start on 16 bytes.  Asynchronous on the current torch stream of x's device.  What comes of the result is a constant to
+    autograd."""
     if not isinstance(x, torch.Tensor):
         raise RuntimeError("x tensor is undefined")
     if not x.is_cuda:
@@ -135,13 +139,15 @@ def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
     buffer = torch.empty(n + _scale_bytes(batch, rows, cols), dtype=torch.uint8, device=device)
     to = buffer.data_ptr()
     _lib.run(device.index, "FlashMoeMx4Quantize", ptr, code, batch, rows, cols, batch_stride, row_stride, to, to + n)
-    return Mx4Tensor._of_buffer(buffer, shape, (to, to + n))
+    return Mx4Tensor._of_buffer(buffer, shape, (to, to + n), x.requires_grad and torch.is_grad_enabled())
 
 
 def _product(a: Mx4Tensor, b: Mx4Tensor, out_dtype: torch.dtype, gated: bool) -> torch.Tensor:
     if not isinstance(a, Mx4Tensor) or not isinstance(b, Mx4Tensor):
         raise RuntimeError("operands must be Mx4Tensors")
     check_not_traced()
+    if a._needs_gradient and torch.is_grad_enabled():
+        raise RuntimeError("products of 4-bit matrices have no gradient; quantise x.detach() or run under torch.no_grad()")
     code = _check_dtype(out_dtype)
     device, sa, sb = a.device, a.shape, b.shape
     if device != b.device or device.type != "cuda":

@@ -146,3 +146,33 @@ def test_compiled_programs_make_the_call(calls, monkeypatch):
         f = torch.compile(lambda a: gated_ffn(2 * a, w13, w2) + 1, backend="eager")
         assert f(x.clone().requires_grad_(grad)).requires_grad == grad
     assert calls == ["FlashMoeFfnForward"] * 2
+
+
+def test_products_do_not_drop_the_gradient_of_their_activations(calls, monkeypatch):
+    """As gated_ffn does on 4-bit weights: what needs a gradient and has none is refused.  Weights are constants."""
+    monkeypatch.setattr(torch, "empty", lambda *s, **k: torch.zeros(*s, dtype=k["dtype"]))
+    x, w = (block()[i].clone() for i in (0, 2))
+
+    def quantize(t):
+        q = mx4_quantize(t)
+        q.device = torch.device("cuda", 0)
+        return q
+
+    w13 = quantize(w.repeat(2, 1, 1))
+    leaf, param = x.clone().requires_grad_(), w.clone().requires_grad_()
+    for a, needs in ((x, False), (leaf, True), (2 * leaf, True), (leaf.detach(), False)):
+        for call in (lambda q: mx4_matmul(q, quantize(w)), lambda q: mx4_matmul(q, quantize(param)), lambda q: mx4_gated_matmul(q, w13)):
+            q = quantize(a)
+            if needs:
+                with pytest.raises(RuntimeError, match="no gradient"):
+                    call(q)
+            else:
+                assert not call(q).requires_grad
+            with torch.no_grad():
+                assert not call(q).requires_grad and not call(quantize(a)).requires_grad
+    with torch.no_grad():
+        q = quantize(leaf)
+    assert not mx4_matmul(q, quantize(w)).requires_grad  # cut off when it was quantised
+    assert not quantize(leaf).dequantize().requires_grad  # a value like any other
+    with pytest.raises(RuntimeError, match="no gradient"):
+        mx4_matmul(copy.copy(quantize(leaf)), quantize(w))
