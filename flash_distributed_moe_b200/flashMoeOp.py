@@ -41,16 +41,45 @@ class FlashMoeBlockWrapper(torch.nn.Module):
         return self.qwen3MoeSparseMoeBlockModule(hidden_states)
 
 
+# A module of these (by name: several projects have one of their own) is SiLU, with or without the product by the other half.
+_SILU = {"SiLU", "SiluAndMul", "SiLUActivation", "Swish", "silu", "swish", "silu_and_mul"}
+
+
+def _refuse_what_is_more_than_the_block(mlp: torch.nn.Module) -> None:
+    """The wrapper replaces the whole forward of `mlp`, so there may be nothing in it but the two products and SiLU."""
+    projections = (mlp.gate_up_proj, mlp.down_proj)
+    for projection in projections:
+        if getattr(projection, "bias", None) is not None:
+            raise RuntimeError("projections with a bias are not supported")
+    for projection, flag, default in ((mlp.gate_up_proj, "gather_output", False), (mlp.down_proj, "reduce_results", True)):
+        if int(getattr(projection, "tp_size", 1)) > 1 and getattr(projection, flag, default):
+            raise RuntimeError("projections whose results are put together over ranks are not supported")
+    for name, child in mlp.named_children():
+        if child in projections or isinstance(child, torch.nn.Identity) or type(child).__name__ in _SILU:
+            continue
+        if isinstance(child, torch.nn.Dropout) and child.p == 0:
+            continue
+        raise RuntimeError(f"{name} ({type(child).__name__}) is no part of a block with SiLU between its projections")
+    for name, _ in mlp.named_parameters(recurse=False):
+        raise RuntimeError(f"{name} is no part of a block with SiLU between its projections")
+    for name in ("act_fn", "activation_fn", "activation", "act", "hidden_act"):
+        act = getattr(mlp, name, None)
+        if act is None or isinstance(act, torch.nn.Module):  # modules: above
+            continue
+        if (act if isinstance(act, str) else getattr(act, "__name__", "")) not in _SILU:
+            raise RuntimeError(f"{name} of the block is not SiLU")
+
+
 class FlashFfnBlockWrapper(torch.nn.Module):
     """The same for a dense block: any module exposing `gate_up_proj.weight` [2I,H] (gate rows first) and
-    `down_proj.weight` [H,I], without biases and with SiLU between them, e.g. the dense layers and shared experts of the same models.  With `fourBit` the
-    weights are quantised once, here, and the forward pass reads them at half a byte per value."""
+    `down_proj.weight` [H,I] that computes down_proj(silu(gate) * up) and nothing else, e.g. the dense layers and
+    shared experts of the same models.  Refused are biases, a factor on the result (`expert_gate`), other activations
+    than SiLU, and projections that sum or gather over ranks.  With `fourBit` the weights are quantised once, here, and
+    the forward pass reads them at half a byte per value."""
 
     def __init__(self, mlpModule: torch.nn.Module, fourBit: bool = False):
         super().__init__()
-        for projection in (mlpModule.gate_up_proj, mlpModule.down_proj):
-            if getattr(projection, "bias", None) is not None:
-                raise RuntimeError("projections with a bias are not supported")
+        _refuse_what_is_more_than_the_block(mlpModule)
         self.mlpModule = mlpModule
         self.fourBitWeights = None
         if fourBit:

@@ -7,8 +7,8 @@ import pytest
 import torch
 
 import moe_testlib  # noqa: F401  (sets sys.path)
-from flash_distributed_moe_b200 import (Mx4Tensor, gated_ffn, mx4_gated_matmul, mx4_matmul, mx4_quantize,
-                                        quantize_ffn_weights)
+from flash_distributed_moe_b200 import (FlashFfnBlockWrapper, Mx4Tensor, gated_ffn, mx4_gated_matmul, mx4_matmul,
+                                        mx4_quantize, quantize_ffn_weights)
 
 
 def matrix(*shape, seed=0):
@@ -176,3 +176,49 @@ def test_products_do_not_drop_the_gradient_of_their_activations(calls, monkeypat
     assert not quantize(leaf).dequantize().requires_grad  # a value like any other
     with pytest.raises(RuntimeError, match="no gradient"):
         mx4_matmul(copy.copy(quantize(leaf)), quantize(w))
+
+
+class Mlp(torch.nn.Module):
+    def __init__(self, act=None, **more):
+        super().__init__()
+        self.gate_up_proj = torch.nn.Linear(64, 2 * 32, bias=False)
+        self.down_proj = torch.nn.Linear(32, 64, bias=False)
+        if act is not None:
+            self.act_fn = act
+        for name, value in more.items():
+            setattr(self, name, value)
+
+
+class SiluAndMul(torch.nn.Module):
+    pass
+
+
+class GeluAndMul(torch.nn.Module):
+    pass
+
+
+def with_attributes(mlp, where, **attributes):
+    for name, value in attributes.items():
+        setattr(getattr(mlp, where), name, value)
+    return mlp
+
+
+def test_the_wrapper_takes_blocks_that_are_what_it_computes():
+    for mlp in (Mlp(), Mlp(torch.nn.SiLU()), Mlp(SiluAndMul()), Mlp(torch.nn.functional.silu), Mlp(hidden_act="silu"),
+                Mlp(dropout=torch.nn.Dropout(0.0)), Mlp(expert_gate=None), Mlp(torch.nn.Identity(), hidden_act="silu"),
+                with_attributes(Mlp(), "down_proj", tp_size=1, reduce_results=True),
+                with_attributes(Mlp(), "down_proj", tp_size=2, reduce_results=False)):
+        assert FlashFfnBlockWrapper(mlp).mlpModule is mlp
+
+
+def test_the_wrapper_refuses_blocks_that_compute_more():
+    """Its forward replaces the module's: a sum over ranks, a factor or another activation would be left out."""
+    for mlp in (Mlp(torch.nn.GELU()), Mlp(GeluAndMul()), Mlp(torch.nn.functional.gelu), Mlp(torch.tanh), Mlp(hidden_act="gelu"),
+                Mlp(activation_fn=torch.nn.functional.gelu), Mlp(expert_gate=torch.nn.Linear(64, 1)),
+                Mlp(scale=torch.nn.Parameter(torch.ones(64))), Mlp(norm=torch.nn.LayerNorm(64)), Mlp(dropout=torch.nn.Dropout(0.1)),
+                with_attributes(Mlp(), "down_proj", tp_size=2, reduce_results=True), with_attributes(Mlp(), "down_proj", tp_size=4),
+                with_attributes(Mlp(), "gate_up_proj", tp_size=2, gather_output=True),
+                with_attributes(Mlp(), "down_proj", bias=torch.nn.Parameter(torch.zeros(64)))):
+        for four_bit in (False, True):
+            with pytest.raises(RuntimeError):
+                FlashFfnBlockWrapper(mlp, fourBit=four_bit)
