@@ -1057,6 +1057,9 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
   if (warp >= kStreamLoads && p.split > 1) ptx::cluster_sync_relaxed();
   ptx::tcgen05_fence_before();
   __syncthreads();
+  // A CTA that has given up did not wait for the others' partial sums, which may still be on their way here: it stays
+  // until every CTA of the cluster has ended (exited threads count as arrived) or has given up too.
+  if (p.split > 1 && abort_flag) ptx::cluster_sync_relaxed();
   wt.drain();
   ptx::tcgen05_fence_after();
   if (warp == 0) ptx::tmem_dealloc(tmem, p.tmem_cols);

@@ -37,3 +37,14 @@ def test_lanes_that_issue_come_together_after_every_wait():
     for call in re.finditer(r"(\S+) = wt\.wait_together\([^;]*, (\w+)\);", kernels):
         assert call.group(1) == call.group(2) == "ok"
     assert not re.search(r"for \([^;]*; *ok\b", kernels)
+
+
+def test_a_ctas_shared_memory_outlives_the_stores_of_its_cluster():
+    """A CTA whose wait ran out has not counted the partial sums that the others store into its shared memory.  It may not
+    leave before they have; one that waited for all of them may."""
+    text = source("dense_gemm.cuh")
+    for kernel, until in (("stream_gemm(", r"if \(p\.split > 1 && abort_flag\) ptx::cluster_sync_relaxed\(\);\s*wt\.drain\(\);"),
+                          ("pair_gemm(", r"wt\.drain\(\);\s*ptx::cluster_sync_relaxed\(\);")):
+        body = text[text.index(kernel):]
+        end = body[body.rindex("__syncthreads();", 0, re.search(r"ptx::tmem_dealloc\w*\(", body).start()):]
+        assert re.match(r"__syncthreads\(\);\s*" + until, end), kernel
