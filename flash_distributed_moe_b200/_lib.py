@@ -19,7 +19,7 @@ EXPORTED_SYMBOLS = [
     "FlashMoeTestQueueGemm", "FlashMoeTestStall", "FlashMoeErrorString", "FlashMoeLaunchNoAlloc",
     "FlashMoeFfnWorkspaceBytes", "FlashMoeFfnSavedBytes", "FlashMoeFfnForward", "FlashMoeFfnBackward",
     "FlashMoeMx4ScaleBytes", "FlashMoeMx4Quantize", "FlashMoeMx4Dequantize", "FlashMoeMx4Matmul", "FlashMoeMx4FfnWorkspaceBytes",
-    "FlashMoeMx4FfnForward", "FlashMoeDenseStatus", "FlashMoeTestFfnStall",
+    "FlashMoeMx4FfnForward", "FlashMoeDenseStatus", "FlashMoeTestFfnStall", "FlashMoeTestDenseStall",
 ]
 
 
@@ -81,6 +81,7 @@ def lib() -> C.CDLL:
             ("FlashMoeMx4FfnWorkspaceBytes", size, [ffn, i64]),
             ("FlashMoeMx4FfnForward", C.c_int, [ffn] + [vp] * 7 + [size, i64, vp]),
             ("FlashMoeDenseStatus", C.c_int, [C.POINTER(C.c_uint32), C.c_int]),
+            ("FlashMoeTestDenseStall", C.c_int, [C.c_int]),
             ("FlashMoeTestFfnStall", C.c_int, [ffn] + [vp] * 5 + [size, i64, vp])):
         getattr(L, name).argtypes, getattr(L, name).restype = args, restype
     _lib = L

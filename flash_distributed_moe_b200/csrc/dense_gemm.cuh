@@ -836,12 +836,12 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
     ptx::fence_proxy_async_shared();
     __syncwarp();
     // The weights may be read while the launch before this one still writes the tokens.
-    if (p.early_weights && elected)
+    if (p.early_weights && elected && !p.stall)
       for (int i = 0; i < filled; ++i) load_weights(i, kb0 + i);
     ptx::grid_wait_dependency();
     // Only now may the next launch start: what it reads early was written before this launch's predecessor ended.
     ptx::grid_launch_dependents();
-    if (elected)
+    if (elected && !p.stall)
       for (int i = 0; i < filled; ++i) {
         if (!p.early_weights) load_weights(i, kb0 + i);
         load_tokens(i, kb0 + i);
@@ -874,7 +874,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
     bool ok = true;
     for (int kb = kb0 + filled; kb < kb1; ++kb) {
       ok = wt.wait_together(empty + s, parity, FDMOE_DENSE_TIMEOUT_EMPTY, ok);
-      if (ok && elected) {
+      if (ok && elected && !p.stall) {
         load_weights(s, kb);
         load_tokens(s, kb);
       }

@@ -55,7 +55,10 @@ struct Call {
   const fdmoe::DeviceSlots* slots;
   uint64_t timeout_ns;
   cudaStream_t stream;
+  bool stall;
 };
+
+thread_local bool g_stall = false;  // test hook: products load nothing
 
 int BeginCall(Call* c, void* stream) {
   int dev = 0;
@@ -109,6 +112,7 @@ int BeginCall(Call* c, void* stream) {
   const char* env = getenv("FLASHMOE_TIMEOUT_MS");
   c->timeout_ns = (uint64_t)std::max(1, env && *env ? atoi(env) : 2000) * 1000000ull;
   c->stream = static_cast<cudaStream_t>(stream);
+  c->stall = g_stall;
   return 0;
 }
 
@@ -162,6 +166,7 @@ int PairShape(FdmoePairParams& p, const Call& c, int64_t rows, int64_t cols, int
   FdmoePairProduct& q = p.product[0];
   p.status = c.status;
   p.timeout_ns = c.timeout_ns;
+  p.stall = c.stall;
   p.products = 1;
   q.rows = (int32_t)rows;
   q.cols = (int32_t)cols;
@@ -243,6 +248,7 @@ int PairProducts(const Call& c, const Product* w, int n, bool bf16) {
   memset(&p, 0, sizeof(p));
   p.status = c.status;
   p.timeout_ns = c.timeout_ns;
+  p.stall = c.stall;
   p.products = n;
   p.split = 1;
   p.bf16 = bf16;
@@ -273,6 +279,7 @@ int StreamProduct(const Call& c, const void* x, const void* w, void* out, int64_
   p.out = out;
   p.status = c.status;
   p.timeout_ns = c.timeout_ns;
+  p.stall = c.stall;
   p.ld = rows;
   p.rows = (int32_t)rows;
   p.tokens = (int32_t)tokens;
@@ -303,7 +310,7 @@ struct Saved {
 
 // h[T, I] = silu(g) * u with [g, u] = x w13^T; also what is to be kept, where `saved` has room for it.
 int GatedProduct(const Call& c, const void* x, const void* w13, void* h, const Saved& saved, int64_t T, int64_t H,
-                 int64_t I, bool bf16, bool stall) {
+                 int64_t I, bool bf16) {
   FdmoePairParams p;
   memset(&p, 0, sizeof(p));
   const int clusters = PairShape(p, c, T, I, H, true, false);
@@ -322,7 +329,6 @@ int GatedProduct(const Call& c, const void* x, const void* w13, void* h, const S
   }
   p.up_row = (int32_t)I;
   p.bf16 = bf16;
-  p.stall = stall;
   return fdmoe_pair_launch(&p, saved.gu ? FDMOE_EPI_GATED_SAVE : FDMOE_EPI_GATED, 0, clusters, c.stream);
 }
 
@@ -377,6 +383,7 @@ int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, 
     p.out = out;
     p.status = c.status;
     p.timeout_ns = c.timeout_ns;
+    p.stall = c.stall;
     p.ld = rows;
     p.rows = (int32_t)rows;
     p.tokens = (int32_t)tokens;
@@ -456,8 +463,8 @@ extern "C" size_t FlashMoeFfnSavedBytes(const FlashMoeFfnConfig* cfg, int64_t to
   return Saved::Bytes(tokensNum, cfg->intermediateSize);
 }
 
-static int FfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y, void* savedFor,
-                      void* workspace, size_t workspaceBytes, int64_t T, void* stream, bool stall) {
+extern "C" int FlashMoeFfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y,
+                                  void* savedFor, void* workspace, size_t workspaceBytes, int64_t T, void* stream) {
   DENSE_TRY(CheckFfn(cfg, T));
   if (T == 0) return 0;
   if (!x || !w13 || !w2 || !y || !Aligned(x) || !Aligned(w13) || !Aligned(w2) || !Aligned(y) || !Aligned(savedFor) ||
@@ -467,25 +474,28 @@ static int FfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w
   DENSE_TRY(BeginCall(&c, stream));
   const int64_t H = cfg->hiddenSize, I = cfg->intermediateSize;
   const bool bf16 = cfg->dtype == kBf16;
-  if (!savedFor && !stall && fdmoe::UseStream(T, 6 * H * I)) {
+  if (!savedFor && fdmoe::UseStream(T, 6 * H * I)) {
     DENSE_TRY(StreamProduct(c, x, w13, workspace, T, I, H, true, bf16, false));
     return StreamProduct(c, workspace, w2, y, T, H, I, false, bf16, true);
   }
   const Saved saved = savedFor ? Saved(savedFor, T, I) : Saved();
   void* h = savedFor ? saved.h : workspace;
-  DENSE_TRY(GatedProduct(c, x, w13, h, saved, T, H, I, bf16, stall));
-  if (stall) return 0;
+  DENSE_TRY(GatedProduct(c, x, w13, h, saved, T, H, I, bf16));
   return PairProduct(c, {{h, T, I, false}, {w2, H, I, false}, y}, bf16);
 }
 
-extern "C" int FlashMoeFfnForward(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y,
-                                  void* saved, void* workspace, size_t workspaceBytes, int64_t tokensNum, void* stream) {
-  return FfnForward(cfg, x, w13, w2, y, saved, workspace, workspaceBytes, tokensNum, stream, false);
+extern "C" int FlashMoeTestDenseStall(int on) {
+  g_stall = on != 0;
+  return 0;
 }
 
 extern "C" int FlashMoeTestFfnStall(const FlashMoeFfnConfig* cfg, const void* x, const void* w13, const void* w2, void* y,
                                     void* workspace, size_t workspaceBytes, int64_t tokensNum, void* stream) {
-  return FfnForward(cfg, x, w13, w2, y, nullptr, workspace, workspaceBytes, tokensNum, stream, true);
+  const bool before = g_stall;
+  g_stall = true;
+  const int r = FlashMoeFfnForward(cfg, x, w13, w2, y, nullptr, workspace, workspaceBytes, tokensNum, stream);
+  g_stall = before;
+  return r;
 }
 
 extern "C" int FlashMoeFfnBackward(const FlashMoeFfnConfig* cfg, const void* dy, const void* x, const void* w13,

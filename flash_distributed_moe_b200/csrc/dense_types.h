@@ -91,6 +91,7 @@ typedef struct {
   int32_t bf16;
   int32_t tmem_cols;
   int32_t early_weights;      // the launch before this one does not write the weights: load them before it has ended
+  int32_t stall;              // test hook, as above
 } FdmoeStreamParams;
 
 // Launchers; return a cudaError_t.  `mx4` selects 4-bit operands.

@@ -174,8 +174,10 @@ int FlashMoeMx4FfnForward(const FlashMoeFfnConfig* config, const void* x, const 
  * until `reset` != 0 clears it. */
 int FlashMoeDenseStatus(uint32_t* code, int reset);
 
-/* Test hook: a forward call whose loads are left out, so that every wait runs out after
- * FLASHMOE_TIMEOUT_MS.  Nothing faults or hangs. */
+/* Test hooks: products whose loads are left out, so that their waits run out after FLASHMOE_TIMEOUT_MS.
+ * Nothing faults or hangs.  FlashMoeTestDenseStall: those of the calling thread's dense calls, until it is
+ * turned off; FlashMoeTestFfnStall: those of one forward call. */
+int FlashMoeTestDenseStall(int on);
 int FlashMoeTestFfnStall(const FlashMoeFfnConfig* config, const void* x, const void* w13, const void* w2,
                          void* y, void* workspace, size_t workspaceBytes, int64_t tokensNum, void* stream);
 

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import dense_testlib as dl
-from flash_distributed_moe_b200 import _lib, mx4_quantize
+from flash_distributed_moe_b200 import _lib, dense_status, mx4_quantize, quantize_ffn_weights
 
 pytestmark = pytest.mark.gpu
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -46,3 +46,91 @@ def test_a_launch_reads_what_the_one_before_has_written(m, n, k):
     assert all(got)
     for out, h in zip(outs, kept):
         assert torch.equal(out, dl.mx4(h).float())
+
+
+def config(hidden, inter, dtype=0):
+    return C.byref(_lib.FlashMoeFfnConfig(hidden, inter, dtype, (C.c_int32 * 5)()))
+
+
+def room(nbytes):
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device="cuda")
+
+
+def forward(tokens, hidden, inter):
+    x, w13, w2, _ = dl.make(tokens, hidden, inter, BF16)
+    lib, cfg, y = _lib.lib(), config(hidden, inter), torch.empty_like(x)
+    ws = room(lib.FlashMoeFfnWorkspaceBytes(cfg, tokens, 0))
+    return [y], (x, w13, w2, ws), lambda: lib.FlashMoeFfnForward(cfg, x.data_ptr(), w13.data_ptr(), w2.data_ptr(), y.data_ptr(), None,
+                                                             ws.data_ptr(), ws.numel(), tokens, stream())
+
+
+def training_forward(tokens, hidden, inter):
+    x, w13, w2, _ = dl.make(tokens, hidden, inter, BF16)
+    lib, cfg, y = _lib.lib(), config(hidden, inter), torch.empty_like(x)
+    saved = room(lib.FlashMoeFfnSavedBytes(cfg, tokens))
+    return [y], (x, w13, w2, saved), lambda: lib.FlashMoeFfnForward(cfg, x.data_ptr(), w13.data_ptr(), w2.data_ptr(), y.data_ptr(),
+                                                                saved.data_ptr(), None, 0, tokens, stream())
+
+
+def backward(tokens, hidden, inter):
+    x, w13, w2, dy = dl.make(tokens, hidden, inter, BF16)
+    lib, cfg = _lib.lib(), config(hidden, inter)
+    saved, ws = room(lib.FlashMoeFfnSavedBytes(cfg, tokens)), room(lib.FlashMoeFfnWorkspaceBytes(cfg, tokens, 1))
+    y, grads = torch.empty_like(x), [torch.empty_like(t) for t in (x, w13, w2)]
+    assert lib.FlashMoeFfnForward(cfg, x.data_ptr(), w13.data_ptr(), w2.data_ptr(), y.data_ptr(), saved.data_ptr(), None, 0,
+                                  tokens, stream()) == 0
+    return grads, (x, w13, w2, dy, saved, ws), lambda: lib.FlashMoeFfnBackward(
+        cfg, dy.data_ptr(), x.data_ptr(), w13.data_ptr(), w2.data_ptr(), saved.data_ptr(), *[t.data_ptr() for t in grads],
+        ws.data_ptr(), ws.numel(), tokens, stream())
+
+
+def product(m, n, k, gated=0, dtype=BF16):
+    g = torch.Generator().manual_seed(3)
+    a = mx4_quantize(torch.randn(m, k, generator=g).cuda())
+    b = mx4_quantize(torch.randn(*((2, n, k) if gated else (n, k)), generator=g).cuda())
+    out = torch.empty(m, n, dtype=dtype, device="cuda")
+    return [out], (a, b), lambda: _lib.lib().FlashMoeMx4Matmul(*a._pointers, *b._pointers, out.data_ptr(), {BF16: 0, FP32: 1}[dtype],
+                                                              m, n, k, gated, stream())
+
+
+def block_of_4_bits(tokens, hidden, inter):
+    x, w13, w2, _ = dl.make(tokens, hidden, inter, BF16)
+    q13, q2 = quantize_ffn_weights(w13, w2)
+    lib, cfg, y = _lib.lib(), config(hidden, inter), torch.empty_like(x)
+    ws = room(lib.FlashMoeMx4FfnWorkspaceBytes(cfg, tokens))
+    return [y], (x, q13, q2, ws), lambda: lib.FlashMoeMx4FfnForward(cfg, x.data_ptr(), *q13._pointers, *q2._pointers, y.data_ptr(),
+                                                                ws.data_ptr(), ws.numel(), tokens, stream())
+
+
+# the streaming kernel with one CTA per tile (one k block) and with several, the pair kernel with one pair per tile and
+# with several, every epilogue, several products in one launch
+@pytest.mark.parametrize("make,size", [
+    (forward, (4, 64, 64)), (forward, (4, 2048, 768)), (forward, (120, 4096, 1024)), (forward, (300, 256, 256)),
+    (forward, (300, 2048, 128)), (training_forward, (40, 256, 256)), (training_forward, (300, 2048, 128)),
+    (backward, (40, 256, 264)), (backward, (300, 2048, 128)), (backward, (1000, 1024, 1032)),
+    (product, (3, 512, 256)), (product, (3, 512, 8192)), (product, (200, 133, 4096)), (product, (300, 264, 512)),
+    (product, (300, 256, 16384)), (product, (5, 512, 4096, 1)), (product, (300, 512, 4096, 1)),
+    (product, (5, 512, 4096, 1, FP32)), (product, (300, 512, 4096, 0, FP32)), (product, (300, 512, 4096, 1, FP32)),
+    (block_of_4_bits, (20, 2048, 768)), (block_of_4_bits, (300, 320, 544))])
+def test_every_wait_ends(monkeypatch, make, size):
+    results, kept, call = make(*size)
+    assert call() == 0
+    torch.cuda.synchronize()
+    want = [t.clone() for t in results]
+    lib = _lib.lib()
+    monkeypatch.setenv("FLASHMOE_TIMEOUT_MS", "30")
+    lib.FlashMoeTestDenseStall(1)
+    try:
+        assert call() == 0
+    finally:
+        lib.FlashMoeTestDenseStall(0)
+    torch.cuda.synchronize()  # the kernels returned, the context is alive
+    assert dense_status() in (21, 22, 23, 24)
+    assert call() != 0  # refused
+    assert dense_status(reset=True) != 0 and dense_status() == 0
+    monkeypatch.delenv("FLASHMOE_TIMEOUT_MS")
+    for t in results:
+        t.fill_(float("nan"))
+    assert call() == 0
+    torch.cuda.synchronize()
+    assert dense_status() == 0 and all(torch.equal(a, b) for a, b in zip(results, want))
