@@ -60,6 +60,14 @@ struct Call {
 
 thread_local bool g_stall = false;  // test hook: products load nothing
 
+// After a device-side error nothing is launched on what it has left.  The caller holds the mutex.
+int RefuseAfterError() {
+  const uint32_t seen = g_shared.status ? *static_cast<volatile uint32_t*>(g_shared.status) : 0;
+  if (!seen) return 0;
+  MOE_ERROR_LOG("refused after device-side error %u; see FlashMoeDenseStatus", seen);
+  return (int)cudaErrorUnknown;
+}
+
 int BeginCall(Call* c, void* stream) {
   int dev = 0;
   DENSE_CHECK(cudaGetDevice(&dev));
@@ -101,11 +109,7 @@ int BeginCall(Call* c, void* stream) {
     for (int n = 1; n <= FDMOE_PAIR_SPLIT; n *= 2) DENSE_CHECK(fdmoe_pair_clusters(2 * n, &d.pair[n]));
     g_shared.known[dev] = true;
   }
-  const uint32_t seen = *static_cast<volatile uint32_t*>(g_shared.status);
-  if (seen) {
-    MOE_ERROR_LOG("refused after device-side error %u; see FlashMoeDenseStatus", seen);
-    return (int)cudaErrorUnknown;
-  }
+  if (const int refused = RefuseAfterError()) return refused;
   c->status = g_shared.status;
   c->encode = g_shared.encode;
   c->slots = &g_shared.slots[dev];
@@ -541,6 +545,10 @@ extern "C" int FlashMoeMx4Quantize(const void* x, int dtype, int64_t batch, int6
   if (!x || !values || !scales || !Aligned(x) || !Aligned(values) || !Aligned(scales) || batchStride < 0 || rowStride < 0 ||
       batchStride % per16 || rowStride % per16)
     return (int)cudaErrorInvalidValue;
+  {
+    std::lock_guard<std::mutex> lock(g_shared.mutex);
+    DENSE_TRY(RefuseAfterError());
+  }
   return fdmoe_mx4_quantize(x, dtype, batch, rows, cols, batchStride, rowStride, values, scales, stream);
 }
 
@@ -550,6 +558,10 @@ extern "C" int FlashMoeMx4Dequantize(const void* values, const void* scales, int
   if (dtype != kBf16 && dtype != kF32 && dtype != kF16) return (int)cudaErrorInvalidValue;
   if (batch == 0 || rows == 0) return 0;
   if (!values || !scales || !out || !Aligned(values) || !Aligned(scales) || !Aligned(out)) return (int)cudaErrorInvalidValue;
+  {
+    std::lock_guard<std::mutex> lock(g_shared.mutex);
+    DENSE_TRY(RefuseAfterError());
+  }
   return fdmoe_mx4_dequantize(values, scales, batch, rows, cols, dtype, out, stream);
 }
 

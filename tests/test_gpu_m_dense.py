@@ -134,3 +134,22 @@ def test_every_wait_ends(monkeypatch, make, size):
     assert call() == 0
     torch.cuda.synchronize()
     assert dense_status() == 0 and all(torch.equal(a, b) for a, b in zip(results, want))
+
+
+def test_quantisation_is_refused_after_an_error_too(monkeypatch):
+    """It would take the result of the product that failed for numbers."""
+    _, kept, call = product(3, 512, 256)
+    x, q = torch.ones(4, 64, dtype=BF16, device="cuda"), kept[0]
+    want = mx4_quantize(x).dequantize()
+    monkeypatch.setenv("FLASHMOE_TIMEOUT_MS", "30")
+    _lib.lib().FlashMoeTestDenseStall(1)
+    try:
+        assert call() == 0
+    finally:
+        _lib.lib().FlashMoeTestDenseStall(0)
+    torch.cuda.synchronize()
+    for refused in (lambda: mx4_quantize(x), q.dequantize, lambda: quantize_ffn_weights(x.repeat(32, 1), x.repeat(16, 1))):
+        with pytest.raises(RuntimeError, match="999"):
+            refused()
+    assert dense_status(reset=True) != 0
+    assert torch.equal(mx4_quantize(x).dequantize(), want)
