@@ -378,7 +378,7 @@ int Mx4Product(const Call& c, const Mx4& a, const Mx4& b, void* out, int dtype, 
   const int chunks = (int)fdmoe::ScaleChunks(k), up_block = (int)((rows + 127) / 128);
   const int epi = gated ? (dtype == kF32 ? FDMOE_EPI_GATED_F32 : FDMOE_EPI_GATED)
                         : (dtype == kF32 ? FDMOE_EPI_F32 : FDMOE_EPI_HALF);
-  if (fdmoe::UseStreamMx4(tokens, rows, gated) || (dtype == kF32 ? rows % 4 : rows % 8) != 0) {
+  if (fdmoe::ChooseMx4Kernel(tokens, rows, gated, dtype == kF32) == fdmoe::Mx4Kernel::kStream) {
     FdmoeStreamParams p;
     memset(&p, 0, sizeof(p));
     const fdmoe::StreamPlan s = fdmoe::MakeStreamPlan((int)rows, (int)tokens, kblocks, gated, true, *c.slots);
@@ -574,6 +574,11 @@ extern "C" int FlashMoeMx4Matmul(const void* aValues, const void* aScales, const
   if (!aValues || !aScales || !bValues || !bScales || !out || !Aligned(aValues) || !Aligned(aScales) || !Aligned(bValues) ||
       !Aligned(bScales) || !Aligned(out))
     return (int)cudaErrorInvalidValue;
+  if (fdmoe::ChooseMx4Kernel(m, n, gated != 0, dtype == kF32) == fdmoe::Mx4Kernel::kNone) {
+    MOE_ERROR_LOG("unsupported product m=%lld n=%lld (above 8388480 of either, n is a multiple of 8, of fp32 results of 4)",
+                  (long long)m, (long long)n);
+    return (int)cudaErrorInvalidValue;
+  }
   Call c;
   DENSE_TRY(BeginCall(&c, stream));
   return Mx4Product(c, {aValues, aScales, m, 1}, {bValues, bScales, n, gated ? 2 : 1}, out, dtype, k, gated != 0, false);

@@ -221,6 +221,19 @@ inline bool UseStreamMx4(int64_t tokens, int64_t rows, bool gated) {
   return tokens <= (!gated && rows <= 4096 ? 2 * FDMOE_STREAM_TOKENS_MX4 : FDMOE_STREAM_TOKENS_MX4);
 }
 
+// The kernel for a 4-bit product.  The streaming kernel writes results whose rows do not start on 16 bytes, at any number
+// of tokens (it then reads the weights again for every 128); its grid has a block per 128 weight rows along y and one
+// per tile of tokens along z, which a launch has no more than 65535 of.
+enum class Mx4Kernel { kStream, kPair, kNone };
+inline Mx4Kernel ChooseMx4Kernel(int64_t tokens, int64_t rows, bool gated, bool f32) {
+  constexpr int64_t kGrid = 65535;
+  const bool aligned = rows % (f32 ? 4 : 8) == 0;
+  const bool fits = (rows + FDMOE_STREAM_ROWS - 1) / FDMOE_STREAM_ROWS <= kGrid &&
+                    (tokens + FDMOE_STREAM_TOKENS_MX4 - 1) / FDMOE_STREAM_TOKENS_MX4 <= kGrid;
+  if (fits && (!aligned || UseStreamMx4(tokens, rows, gated))) return Mx4Kernel::kStream;
+  return aligned ? Mx4Kernel::kPair : Mx4Kernel::kNone;
+}
+
 inline size_t AlignBytes(size_t v) { return (v + 255) / 256 * 256; }
 
 // 512-byte blocks of scales per 128 rows: an even number, as many as the stages of 256 columns take.

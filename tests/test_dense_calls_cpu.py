@@ -1,14 +1,16 @@
 """The dense operators' Python and C entries without a GPU: what a call must not do silently."""
 import copy
 import io
+import os
 import pickle
+import subprocess
 
 import pytest
 import torch
 
-import moe_testlib  # noqa: F401  (sets sys.path)
+import moe_testlib as tl
 from flash_distributed_moe_b200 import (FlashFfnBlockWrapper, Mx4Tensor, gated_ffn, mx4_gated_matmul, mx4_matmul,
-                                        mx4_quantize, quantize_ffn_weights)
+                                        mx4_quantize, quantize_ffn_weights, _lib, build as build_mod)
 
 
 def matrix(*shape, seed=0):
@@ -222,3 +224,17 @@ def test_the_wrapper_refuses_blocks_that_compute_more():
         for four_bit in (False, True):
             with pytest.raises(RuntimeError):
                 FlashFfnBlockWrapper(mlp, fourBit=four_bit)
+
+
+def test_every_accepted_product_has_a_grid_that_can_be_launched(tmp_path):
+    exe = str(tmp_path / "dense_limits_test.bin")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-o", exe, os.path.join(tl.ROOT, "tests", "cpp", "dense_limits_test.cpp")], check=True)
+    out = subprocess.run([exe], capture_output=True, text=True)
+    assert out.returncode == 0, out.stdout
+
+
+@pytest.mark.parametrize("m,n,dtype", [(1, 8388484, 0), (1, 8388482, 1), (8388481, 12, 0), (1 << 30, 1, 2), (1 << 30, 2, 1)])
+def test_products_without_a_grid_are_refused(m, n, dtype):
+    build_mod.build()
+    for gated in (0, 1):
+        assert _lib.lib().FlashMoeMx4Matmul(*[4096] * 5, dtype, m, n, 32, gated, None) == 1  # cudaErrorInvalidValue

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import dense_testlib as dl
-from flash_distributed_moe_b200 import _lib, dense_status, mx4_quantize, quantize_ffn_weights
+from flash_distributed_moe_b200 import _lib, dense_status, mx4_matmul, mx4_quantize, quantize_ffn_weights
 
 pytestmark = pytest.mark.gpu
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -153,3 +153,14 @@ def test_quantisation_is_refused_after_an_error_too(monkeypatch):
             refused()
     assert dense_status(reset=True) != 0
     assert torch.equal(mx4_quantize(x).dequantize(), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_more_weight_rows_than_a_grid_has_blocks(dtype):
+    n, k = 8388608, 32  # 65536 tiles of 128
+    g = torch.Generator(device="cuda").manual_seed(7)
+    a = mx4_quantize(torch.randn(3, k, generator=g, device="cuda"))
+    b = mx4_quantize(torch.randn(n, k, generator=g, device="cuda"))
+    y = mx4_matmul(a, b, dtype)
+    want, e = dl.product(a.dequantize(FP32).double(), b.dequantize(FP32).double())
+    dl.assert_within(y, want, dl.rounded(want, e, dtype))
