@@ -786,6 +786,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
   constexpr bool kGated = EPI == FDMOE_EPI_GATED || EPI == FDMOE_EPI_GATED_F32;
   constexpr int kParts = kGated ? 2 : 1;
   constexpr int kScales = MX4 ? (kParts + 1) * 2 * kScaleBlock : 0;
+  static_assert(!MX4 || FDMOE_STREAM_TOKENS_MX4 == 128, "where there are several tiles of tokens, each is a block of scales");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
   const int nt = p.tile_tokens;
@@ -899,8 +900,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
 #pragma unroll
           for (int q = 0; q < 2 * (kParts + 1); ++q)
             ptx::tmem_copy_scales(tsf + q * 4, ptx::smem_desc_scales(sf + q * kScaleBlock));
-          // tokens of a tile may start inside their block of 128: every 32 of them are one column of scales
-          const uint32_t tsb = tsf + kParts * 8 + ((tok0 & 127) >> 5);
+          const uint32_t tsb = tsf + kParts * 8;  // a tile of tokens begins with a block of 128 rows of scales
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t id = ptx::make_idesc_mx4(128, nt, (k & 1) * 2);

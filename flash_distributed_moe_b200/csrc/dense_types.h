@@ -18,7 +18,7 @@ enum {
   FDMOE_PAIR_LIST = 64,       // most tiles of a pair in it
   FDMOE_STREAM_ROWS = 128,    // weight rows of a tile of the streaming kernel
   FDMOE_STREAM_TOKENS = 192,  // most tokens of a tile of the streaming kernel: the room for a gated tile's partial sums
-  FDMOE_STREAM_TOKENS_MX4 = 128,  // with 4-bit operands: a tile lies in one block of 128 rows of scales
+  FDMOE_STREAM_TOKENS_MX4 = 128,  // with 4-bit operands: a tile is one block of 128 rows of scales, or part of the only one
   FDMOE_STREAM_SPLIT = 8,     // most CTAs that share the k axis of a tile of the streaming kernel
   FDMOE_STREAM_STAGES = 12,   // most shared-memory stages of the streaming kernel
   FDMOE_MX4_BLOCK = 32,       // elements that share a scale
