@@ -9,6 +9,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <mutex>
 
 #include "../../include/flashmoe_c.h"
@@ -445,6 +446,30 @@ int CheckMx4(int64_t batch, int64_t rows, int64_t cols) {
   return 0;
 }
 
+// Memory of a call.  What it writes may lie on nothing that it reads or writes elsewhere: launches of a call overlap, and
+// the products of a backward pass are one launch.
+struct Range {
+  const void* base;  // NULL: not there
+  size_t bytes;
+};
+bool Apart(const Range& a, const Range& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.base), y = reinterpret_cast<uintptr_t>(b.base);
+  return !x || !y || x + a.bytes <= y || y + b.bytes <= x;
+}
+int CheckApart(std::initializer_list<Range> written, std::initializer_list<Range> read) {
+  for (auto w = written.begin(); w != written.end(); ++w) {
+    bool apart = true;
+    for (const Range& r : read) apart = apart && Apart(*w, r);
+    for (auto other = written.begin(); other != w; ++other) apart = apart && Apart(*w, *other);
+    if (!apart) {
+      MOE_ERROR_LOG("results or scratch lie on other memory of the call");
+      return (int)cudaErrorInvalidValue;
+    }
+  }
+  return 0;
+}
+size_t Bytes(int64_t rows, int64_t cols, int size) { return (size_t)rows * cols * size; }
+
 }  // namespace
 
 // ---------------------------------------------------------------- C exports
@@ -474,9 +499,12 @@ extern "C" int FlashMoeFfnForward(const FlashMoeFfnConfig* cfg, const void* x, c
   if (!x || !w13 || !w2 || !y || !Aligned(x) || !Aligned(w13) || !Aligned(w2) || !Aligned(y) || !Aligned(savedFor) ||
       !Aligned(workspace) || (!savedFor && (!workspace || workspaceBytes < FlashMoeFfnWorkspaceBytes(cfg, T, 0))))
     return (int)cudaErrorInvalidValue;
+  const int64_t H = cfg->hiddenSize, I = cfg->intermediateSize;
+  const Range scratch = savedFor ? Range{savedFor, Saved::Bytes(T, I)} : Range{workspace, Bytes(T, I, 2)};
+  DENSE_TRY(CheckApart({{y, Bytes(T, H, 2)}, scratch}, {{w13, Bytes(2 * I, H, 2)}, {w2, Bytes(H, I, 2)}}));
+  DENSE_TRY(CheckApart({scratch}, {{x, Bytes(T, H, 2)}}));  // the last product writes y, the first reads x
   Call c;
   DENSE_TRY(BeginCall(&c, stream));
-  const int64_t H = cfg->hiddenSize, I = cfg->intermediateSize;
   const bool bf16 = cfg->dtype == kBf16;
   if (!savedFor && fdmoe::UseStream(T, 6 * H * I)) {
     DENSE_TRY(StreamProduct(c, x, w13, workspace, T, I, H, true, bf16, false));
@@ -517,6 +545,9 @@ extern "C" int FlashMoeFfnBackward(const FlashMoeFfnConfig* cfg, const void* dy,
       !Aligned(savedBy) || !Aligned(workspace) || workspaceBytes < FlashMoeFfnWorkspaceBytes(cfg, T, 1))
     return (int)cudaErrorInvalidValue;
   if (!dx && !dw13 && !dw2) return 0;
+  DENSE_TRY(CheckApart({{dx, Bytes(T, H, 2)}, {dw13, Bytes(2 * I, H, 2)}, {dw2, Bytes(H, I, 2)}, {workspace, Bytes(T, I, 4)}},
+                       {{dy, Bytes(T, H, 2)}, {x, Bytes(T, H, 2)}, {w13, Bytes(2 * I, H, 2)}, {w2, Bytes(H, I, 2)},
+                        {savedBy, Saved::Bytes(T, I)}}));
   Call c;
   DENSE_TRY(BeginCall(&c, stream));
   const bool bf16 = cfg->dtype == kBf16;
@@ -545,6 +576,9 @@ extern "C" int FlashMoeMx4Quantize(const void* x, int dtype, int64_t batch, int6
   if (!x || !values || !scales || !Aligned(x) || !Aligned(values) || !Aligned(scales) || batchStride < 0 || rowStride < 0 ||
       batchStride % per16 || rowStride % per16)
     return (int)cudaErrorInvalidValue;
+  const int64_t span = (batch - 1) * batchStride + (rows - 1) * rowStride + cols;
+  DENSE_TRY(CheckApart({{values, Bytes(batch * rows, cols / 2, 1)}, {scales, fdmoe::ScaleBytes(batch, rows, cols)}},
+                       {{x, Bytes(span, 1, dtype == kF32 ? 4 : 2)}}));
   {
     std::lock_guard<std::mutex> lock(g_shared.mutex);
     DENSE_TRY(RefuseAfterError());
@@ -558,6 +592,8 @@ extern "C" int FlashMoeMx4Dequantize(const void* values, const void* scales, int
   if (dtype != kBf16 && dtype != kF32 && dtype != kF16) return (int)cudaErrorInvalidValue;
   if (batch == 0 || rows == 0) return 0;
   if (!values || !scales || !out || !Aligned(values) || !Aligned(scales) || !Aligned(out)) return (int)cudaErrorInvalidValue;
+  DENSE_TRY(CheckApart({{out, Bytes(batch * rows, cols, dtype == kF32 ? 4 : 2)}},
+                       {{values, Bytes(batch * rows, cols / 2, 1)}, {scales, fdmoe::ScaleBytes(batch, rows, cols)}}));
   {
     std::lock_guard<std::mutex> lock(g_shared.mutex);
     DENSE_TRY(RefuseAfterError());
@@ -579,6 +615,10 @@ extern "C" int FlashMoeMx4Matmul(const void* aValues, const void* aScales, const
                   (long long)m, (long long)n);
     return (int)cudaErrorInvalidValue;
   }
+  const int parts = gated ? 2 : 1;
+  DENSE_TRY(CheckApart({{out, Bytes(m, n, dtype == kF32 ? 4 : 2)}},
+                       {{aValues, Bytes(m, k / 2, 1)}, {aScales, fdmoe::ScaleBytes(1, m, k)},
+                        {bValues, Bytes(parts * n, k / 2, 1)}, {bScales, fdmoe::ScaleBytes(parts, n, k)}}));
   Call c;
   DENSE_TRY(BeginCall(&c, stream));
   return Mx4Product(c, {aValues, aScales, m, 1}, {bValues, bScales, n, gated ? 2 : 1}, out, dtype, k, gated != 0, false);
@@ -625,9 +665,13 @@ extern "C" int FlashMoeMx4FfnForward(const FlashMoeFfnConfig* cfg, const void* x
       !Aligned(w13Scales) || !Aligned(w2Values) || !Aligned(w2Scales) || !Aligned(y) || !Aligned(workspace) ||
       workspaceBytes < FlashMoeMx4FfnWorkspaceBytes(cfg, T))
     return (int)cudaErrorInvalidValue;
+  const Mx4FfnLayout l = MakeMx4FfnLayout(T, H, I);
+  DENSE_TRY(CheckApart({{y, Bytes(T, H, 2)}, {workspace, l.total}},
+                       {{w13Values, Bytes(2 * I, H / 2, 1)}, {w13Scales, fdmoe::ScaleBytes(2, I, H)},
+                        {w2Values, Bytes(H, I / 2, 1)}, {w2Scales, fdmoe::ScaleBytes(1, H, I)}}));
+  DENSE_TRY(CheckApart({{workspace, l.total}}, {{x, Bytes(T, H, 2)}}));  // x is quantised before y is written
   Call c;
   DENSE_TRY(BeginCall(&c, stream));
-  const Mx4FfnLayout l = MakeMx4FfnLayout(T, H, I);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   DENSE_TRY(fdmoe_mx4_quantize(x, cfg->dtype, 1, T, H, 0, H, ws + l.xv, ws + l.xs, stream));
   DENSE_TRY(Mx4Product(c, {ws + l.xv, ws + l.xs, T, 1}, {w13Values, w13Scales, I, 2}, ws + l.h, cfg->dtype, H, true, true));

@@ -114,7 +114,9 @@ int FlashMoeLaunchNoAlloc(const void* gateWeights, const void* ffn1ExpertWeights
  * microscaled weights for it (the reference has no counterpart; its experts' FFN is
  * src/hip/kernel/moeKernel.h).  These entries need no handle: every call enqueues its work on `stream`,
  * takes scratch from the caller and can be captured into a CUDA graph; calls with different workspaces
- * may overlap.  Matrices are contiguous, row-major, on the current device, and start on 16 bytes.
+ * may overlap.  Matrices are contiguous, row-major, on the current device, and start on 16 bytes.  Results,
+ * scratch and what is kept lie on no other memory of the call (cudaErrorInvalidValue), but for `y`, which may be
+ * `x`, in the two forward calls.
  * Results are deterministic: the same call gives the same bits. */
 typedef struct {
   int32_t hiddenSize;       /* H, a multiple of 8 (4-bit weights: 32) */
@@ -159,7 +161,8 @@ int FlashMoeMx4Dequantize(const void* values, const void* scales, int64_t batch,
                           int dtype, void* out, void* stream);
 
 /* out[m,n] = a[m,k] b[n,k]^T, accumulated in fp32.  gated != 0: b is a batch of two matrices [2,n,k], gate
- * and up projection, and out = silu(a b0^T) * (a b1^T).  dtype of out: 0 bf16, 1 fp32, 2 fp16. */
+ * and up projection, and out = silu(a b0^T) * (a b1^T).  dtype of out: 0 bf16, 1 fp32, 2 fp16.  With m or n
+ * above 8388480, n is a multiple of 8 (fp32 results: 4). */
 int FlashMoeMx4Matmul(const void* aValues, const void* aScales, const void* bValues, const void* bScales,
                       void* out, int dtype, int64_t m, int64_t n, int64_t k, int gated, void* stream);
 

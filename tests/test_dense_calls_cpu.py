@@ -1,5 +1,6 @@
 """The dense operators' Python and C entries without a GPU: what a call must not do silently."""
 import copy
+import ctypes as C
 import io
 import os
 import pickle
@@ -237,4 +238,46 @@ def test_every_accepted_product_has_a_grid_that_can_be_launched(tmp_path):
 def test_products_without_a_grid_are_refused(m, n, dtype):
     build_mod.build()
     for gated in (0, 1):
-        assert _lib.lib().FlashMoeMx4Matmul(*[4096] * 5, dtype, m, n, 32, gated, None) == 1  # cudaErrorInvalidValue
+        assert _lib.lib().FlashMoeMx4Matmul(*[i << 45 for i in range(1, 6)], dtype, m, n, 32, gated, None) == 1  # cudaErrorInvalidValue
+
+
+def overlaps(read, written, sizes, but=()):
+    """Addresses far apart, but for one written range that begins with, ends in or lies within another one."""
+    base = {name: (i + 1) << 32 for i, name in enumerate([*read, *written])}
+    for w in written:
+        for other in base:
+            if other == w or (w, other) in but or (other, w) in but:
+                continue
+            for at in {base[other], base[other] + sizes[other] - 16, max(base[other] - sizes[w] + 16, 16)}:
+                yield {**base, w: at}
+
+
+def test_results_on_other_memory_of_the_call_are_refused():
+    """Launches of a call overlap: dx in the place of x would be read by the product for dw13 in parts."""
+    build_mod.build()
+    lib, T, H, I, invalid = _lib.lib(), 10, 64, 96, 1
+    cfg = C.byref(_lib.FlashMoeFfnConfig(H, I, 0, (C.c_int32 * 5)()))
+    part = -(-T * I * 2 // 256) * 256
+    size = dict(x=T * H * 2, dy=T * H * 2, y=T * H * 2, dx=T * H * 2, w13=4 * I * H, dw13=4 * I * H, w2=2 * I * H, dw2=2 * I * H,
+                saved=-(-T * I * 4 // 256) * 256 + 2 * part)
+    for ws in ("saved", "workspace"):
+        for a in overlaps(("x", "w13", "w2"), ("y", ws), {**size, "workspace": T * I * 2}, but={("y", "x")}):
+            assert lib.FlashMoeFfnForward(cfg, a["x"], a["w13"], a["w2"], a["y"], a.get("saved"), a.get("workspace"), 1 << 20, T,
+                                          None) == invalid, a
+    for a in overlaps(("dy", "x", "w13", "w2", "saved"), ("dx", "dw13", "dw2", "workspace"), {**size, "workspace": T * I * 4}):
+        assert lib.FlashMoeFfnBackward(cfg, *[a[n] for n in ("dy", "x", "w13", "w2", "saved", "dx", "dw13", "dw2", "workspace")],
+                                       1 << 20, T, None) == invalid, a
+    scales = lambda batch, rows, cols: lib.FlashMoeMx4ScaleBytes(batch, rows, cols)  # noqa: E731
+    for a in overlaps(("x",), ("values", "scales"), dict(x=(T - 1) * 80 * 2 + H * 2, values=T * H // 2, scales=scales(1, T, H))):
+        assert lib.FlashMoeMx4Quantize(a["x"], 0, 1, T, H, 0, 80, a["values"], a["scales"], None) == invalid, a
+    for a in overlaps(("values", "scales"), ("out",), dict(out=T * H * 4, values=T * H // 2, scales=scales(1, T, H))):
+        assert lib.FlashMoeMx4Dequantize(a["values"], a["scales"], 1, T, H, 1, a["out"], None) == invalid, a
+    for gated in (0, 1):
+        names, b = ("av", "as", "bv", "bs"), 1 + gated
+        for a in overlaps(names, ("out",), dict(av=T * H // 2, bv=b * I * H // 2, out=T * I * 4, **{"as": scales(1, T, H)}, bs=scales(b, I, H))):
+            assert lib.FlashMoeMx4Matmul(*[a[n] for n in names], a["out"], 1, T, I, H, gated, None) == invalid, a
+    names = ("x", "v13", "s13", "v2", "s2")
+    total = lib.FlashMoeMx4FfnWorkspaceBytes(cfg, T)
+    for a in overlaps(names, ("y", "ws"), dict(x=T * H * 2, y=T * H * 2, v13=I * H, v2=I * H // 2, s13=scales(2, I, H), s2=scales(1, H, I),
+                                               ws=total), but={("y", "x")}):
+        assert lib.FlashMoeMx4FfnForward(cfg, *[a[n] for n in names], a["y"], a["ws"], total, T, None) == invalid, a
