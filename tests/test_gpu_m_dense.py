@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import dense_testlib as dl
-from flash_distributed_moe_b200 import _lib, dense_status, mx4_matmul, mx4_quantize, quantize_ffn_weights
+from flash_distributed_moe_b200 import _lib, dense_status, gated_ffn, mx4_matmul, mx4_quantize, quantize_ffn_weights
 
 pytestmark = pytest.mark.gpu
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -164,3 +164,23 @@ def test_more_weight_rows_than_a_grid_has_blocks(dtype):
     y = mx4_matmul(a, b, dtype)
     want, e = dl.product(a.dequantize(FP32).double(), b.dequantize(FP32).double())
     dl.assert_within(y, want, dl.rounded(want, e, dtype))
+
+
+def test_weight_gradients_beyond_32_bits():
+    """[T, 2I] has 2.3e9 elements and only the last tokens have a gradient.  The products of the others are zeros, which a
+    32-bit sum takes without an error, so the bound is that of the last tokens alone: one that grew with all of them would
+    let zeros or a gradient of the other sign pass."""
+    tokens, hidden, inter, last = 70000, 64, 16384, 300
+    g = torch.Generator(device="cuda").manual_seed(13)
+    r = lambda *s, std: torch.empty(*s, device="cuda").normal_(0, std, generator=g).to(BF16)  # noqa: E731
+    x, w13, w2 = r(tokens, hidden, std=1.0), r(2 * inter, hidden, std=0.2), r(hidden, inter, std=inter ** -0.5)
+    dy = torch.zeros(tokens, hidden, dtype=BF16, device="cuda")
+    dy[-last:] = r(last, hidden, std=1.0)
+    leaves = [t.requires_grad_() for t in (x, w13, w2)]
+    _, dw13, dw2 = torch.autograd.grad(gated_ffn(*leaves), leaves, dy)
+    want = dl.ffn_grads(x[-last:].detach(), w13.detach(), w2.detach(), dy[-last:])
+    for name, got, (value, bound) in zip(("dw13", "dw2"), (dw13, dw2), want[1:]):
+        dl.assert_within(got, value, bound, name)
+        for wrong in (torch.zeros_like(got), -got, 3 * got):
+            with pytest.raises(AssertionError):
+                dl.assert_within(wrong, value, bound, name)
