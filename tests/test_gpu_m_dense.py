@@ -1,5 +1,9 @@
 """GPU: the dense operators one behind another, where they are refused, and where their waits run out."""
 import ctypes as C
+import os
+import subprocess
+import sys
+import threading
 
 import pytest
 import torch
@@ -8,6 +12,7 @@ import dense_testlib as dl
 from flash_distributed_moe_b200 import _lib, dense_status, gated_ffn, mx4_matmul, mx4_quantize, quantize_ffn_weights
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 
 
@@ -184,3 +189,99 @@ def test_weight_gradients_beyond_32_bits():
         for wrong in (torch.zeros_like(got), -got, 3 * got):
             with pytest.raises(AssertionError):
                 dl.assert_within(wrong, value, bound, name)
+
+
+def test_gradient_of_tokens_that_are_one_row():
+    # 50 equal rows of dx, added by torch in 32 bits and rounded once; zeros are far outside this bound
+    x, w13, w2, _ = dl.make(1, 72, 136, FP16, seed=3)
+    one = x.clone().requires_grad_()
+    gated_ffn(one.expand(50, 72), w13, w2).backward(torch.ones(50, 72, dtype=FP16, device="cuda"))
+    value, bound = dl.ffn_grads(x, w13, w2, torch.ones_like(x))[0]
+    value, bound = 50 * value, dl.rounded(50 * value, 50 * bound + 50 * 2.0 ** -24 * 50 * value.abs(), FP16)
+    dl.assert_within(one.grad, value, bound)
+    with pytest.raises(AssertionError):
+        dl.assert_within(torch.zeros_like(one.grad), value, bound)
+
+
+@pytest.mark.parametrize("m", [16, 300])
+@pytest.mark.parametrize("ea,eb", [(-120, 0), (-120, 118), (118, -120), (-60, -60), (60, 60), (118, 0)])
+def test_products_of_far_apart_scales(m, ea, eb):
+    g = torch.Generator().manual_seed(4)
+    a = mx4_quantize((torch.randn(m, 512, generator=g) * 2.0 ** ea).cuda())
+    b = mx4_quantize((torch.randn(264, 512, generator=g) * 2.0 ** eb).cuda())
+    want, e = dl.product(a.dequantize(FP32).double(), b.dequantize(FP32).double())
+    dl.assert_within(mx4_matmul(a, b, FP32), want, dl.rounded(want, e, FP32))
+
+
+@pytest.mark.parametrize("tokens,hidden,inter", [(40, 256, 264), (300, 2048, 128), (777, 1000, 2744), (2000, 1024, 2048)])
+def test_gradients_have_the_same_bits_each_time(tokens, hidden, inter):
+    x, w13, w2, dy = dl.make(tokens, hidden, inter, BF16, seed=9)
+    leaves = [t.requires_grad_() for t in (x, w13, w2)]
+    first = torch.autograd.grad(gated_ffn(*leaves), leaves, dy)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(gated_ffn(*leaves), leaves, dy)))
+
+
+def test_training_steps_of_several_threads():
+    args = [dl.make(t, 512, 768, BF16, seed=t) for t in (4, 90, 200, 700)]
+
+    def step(x, w13, w2, dy):
+        leaves = [t.detach().requires_grad_() for t in (x, w13, w2)]
+        y = gated_ffn(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    want = [step(*a) for a in args]
+    torch.cuda.synchronize()
+    equal = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(15):
+                got = step(*args[i])
+                s.synchronize()
+                equal.append(all(torch.equal(a, b) for a, b in zip(got, want[i])))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(args))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(equal) == 60 and all(equal) and dense_status() == 0
+
+
+@pytest.mark.parametrize("tokens", [3, 300])
+@pytest.mark.parametrize("what", ["forward", "training", "product"])
+def test_the_first_call_of_a_process_inside_a_capture(what, tokens):
+    program = f"""
+import sys
+sys.path[:0] = [{ROOT!r}, {os.path.join(ROOT, 'tests')!r}]
+import torch, dense_testlib as dl, flash_distributed_moe_b200 as fm
+x, w13, w2, dy = dl.make({tokens}, 256, 264, torch.bfloat16)
+w = w13.float()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    if "{what}" == "forward":
+        with torch.no_grad():
+            y = fm.gated_ffn(x, w13, w2)
+    elif "{what}" == "training":
+        leaves = [t.requires_grad_() for t in (x, w13, w2)]
+        y = fm.gated_ffn(*leaves)
+        grads = torch.autograd.grad(y, leaves, dy)
+    else:
+        a, b = fm.mx4_quantize(x), fm.mx4_quantize(w)
+        y = fm.mx4_matmul(a, b)
+graph.replay()
+torch.cuda.synchronize()
+if "{what}" == "product":
+    want, e = dl.product(dl.mx4(x), dl.mx4(w))
+    dl.assert_within(y, want, dl.rounded(want, e, torch.bfloat16))
+else:
+    dl.assert_within(y.detach(), *dl.ffn(x.detach(), w13.detach(), w2.detach()))
+if "{what}" == "training":
+    for got, (value, bound) in zip(grads, dl.ffn_grads(x.detach(), w13.detach(), w2.detach(), dy)):
+        dl.assert_within(got, value, bound)
+assert fm.dense_status() == 0
+"""
+    out = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0, out.stderr[-2000:]
