@@ -18,6 +18,8 @@ from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib
 
+# what torch.jit.is_tracing and get_proxy_mode ask first, at a third of their time
+_is_tracing, _dispatch_modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
 DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 
 
@@ -39,7 +41,7 @@ def check_no_tangent(*tensors) -> None:
 def check_not_traced() -> None:
     """A recorder of torch operators (torch.jit.trace, make_fx) sees the allocation of a result and not the call that fills
     it: its program would return memory as it is found.  torch.compile runs these calls between its graphs."""
-    if torch.jit.is_tracing() or (torch._C._len_torch_dispatch_stack() > 0 and get_proxy_mode() is not None):
+    if _is_tracing() or (_dispatch_modes() > 0 and get_proxy_mode() is not None):
         raise RuntimeError("the dense operators cannot be recorded by torch.jit.trace or make_fx")
 
 
