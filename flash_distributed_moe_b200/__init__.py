@@ -11,5 +11,5 @@ from .flashMoeOp import FlashFfnBlockWrapper, FlashMoeBlockWrapper  # noqa: F401
 from .flashMx4 import Mx4Tensor, mx4_gated_matmul, mx4_matmul, mx4_quantize  # noqa: F401
 from .flashFfn import dense_status, gated_ffn, quantize_ffn_weights  # noqa: F401
 
-__all__ = ["MoeKernelLauncher", "FlashMoeBlockWrapper", "FlashFfnBlockWrapper", "flashMoeLauncher", "Mx4Tensor", "mx4_quantize", 
-           "mx4_matmul", "mx4_gated_matmul", "gated_ffn", "quantize_ffn_weights", "dense_status"]
+__all__ = ["MoeKernelLauncher", "FlashMoeBlockWrapper", "FlashFfnBlockWrapper", "flashMoeLauncher", "Mx4Tensor",
+           "mx4_quantize", "mx4_matmul", "mx4_gated_matmul", "gated_ffn", "quantize_ffn_weights", "dense_status"]

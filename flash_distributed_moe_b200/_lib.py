@@ -18,8 +18,9 @@ EXPORTED_SYMBOLS = [
     "FlashMoeDestroy", "FlashMoeGetLastStatus", "FlashMoeDebugRead", "FlashMoeTestTaskSystem",
     "FlashMoeTestQueueGemm", "FlashMoeTestStall", "FlashMoeErrorString", "FlashMoeLaunchNoAlloc",
     "FlashMoeFfnWorkspaceBytes", "FlashMoeFfnSavedBytes", "FlashMoeFfnForward", "FlashMoeFfnBackward",
-    "FlashMoeMx4ScaleBytes", "FlashMoeMx4Quantize", "FlashMoeMx4Dequantize", "FlashMoeMx4Matmul", "FlashMoeMx4FfnWorkspaceBytes",
-    "FlashMoeMx4FfnForward", "FlashMoeDenseStatus", "FlashMoeTestFfnStall", "FlashMoeTestDenseStall",
+    "FlashMoeMx4ScaleBytes", "FlashMoeMx4Quantize", "FlashMoeMx4Dequantize", "FlashMoeMx4Matmul",
+    "FlashMoeMx4FfnWorkspaceBytes", "FlashMoeMx4FfnForward", "FlashMoeDenseStatus", "FlashMoeTestFfnStall",
+    "FlashMoeTestDenseStall",
 ]
 
 

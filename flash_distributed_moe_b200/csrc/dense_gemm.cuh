@@ -113,7 +113,8 @@ __device__ __forceinline__ uint32_t pack2(F2 a, bool bf16) {
   return pack2(lo, hi, bf16);
 }
 __device__ __forceinline__ F2 as_f2(uint32_t lo, uint32_t hi) { return F2(__uint_as_float(lo), __uint_as_float(hi)); }
-// 1 / (1 + 2^(-g log2 e)); an exponential that overflows gives 0.
+// 1 / (1 + 2^(-g log2 e)); an exponential that overflows gives 0.  The exponential is off by 2^-22 of itself and, for the
+// rounding of its argument, by |g| 2^-23; the sum and the reciprocal by 2^-24 and 2^-23.
 __device__ __forceinline__ F2 sigmoid(F2 g) {
   float lo, hi;
   (g * F2(-1.44269504f, -1.44269504f)).get(lo, hi);
@@ -254,7 +255,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
   if (warp == 1) {
     constexpr int kEmptyAcc = 2 * S::kStages + S::kAccs, kCount = kEmptyAcc + S::kAccs + 8 + 1;
     static_assert(kCount <= 32, "one barrier per lane");
-    if (lane < kCount) ptx::mbar_init(full + lane, lane >= kEmptyAcc && lane < kEmptyAcc + S::kAccs ? 16 : 1);  // 16: the epilogue warps of both
+    // an accumulator is given back by the epilogue warps of both CTAs
+    if (lane < kCount) ptx::mbar_init(full + lane, lane >= kEmptyAcc && lane < kEmptyAcc + S::kAccs ? 16 : 1);
     if (lane == 0) *abort_flag = 0;
     ptx::fence_mbar_init();
     __syncwarp();
@@ -527,7 +529,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
               for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int j = 0; j < kCols; j += 4) {
-                  const float4 f = ptx::ld_shared_f32x4(from + (r * kParts + q) * kBoxSums + j * 128 + (turned ^ (4 * k)) * 16);
+                  const float4 f =
+                      ptx::ld_shared_f32x4(from + (r * kParts + q) * kBoxSums + j * 128 + (turned ^ (4 * k)) * 16);
                   const float add[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
                   for (int e = 0; e < 4; ++e)
@@ -538,8 +541,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
             const uint32_t* const v0 = v[0][k];
             const uint32_t* const v1 = v[kParts - 1][k];
             const auto put = [&](void* to, int width, uint4 x) {  // 16 bytes; `to` has `width` times the columns
+              const int64_t at = (int64_t)(row + 4 * k) * pr.cols * width + col;
               if (row + 4 * k < pr.rows && col < pr.cols)
-                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(to) + ((int64_t)(row + 4 * k) * pr.cols * width + col) * (kF32 ? 4 : 2)) = x;
+                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(to) + at * (kF32 ? 4 : 2)) = x;
             };
             if constexpr (kF32) {
               float y[4];
@@ -548,7 +552,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
                 const F2 a = as_f2(v0[e], v0[e + 1]);
                 (kGated ? gate(a, as_f2(v1[e], v1[e + 1])) : a).get(y[e], y[e + 1]);
               }
-              put(p.to[0], 1, make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])));
+              put(p.to[0], 1, make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]),
+                                         __float_as_uint(y[3])));
             } else if constexpr (kGated) {
               put(p.to[0], 1, gate8<BF16>(v0, v1));
               if constexpr (EPI == FDMOE_EPI_GATED_SAVE) {
@@ -619,7 +624,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
           if (box >= boxes) break;
           if constexpr (S::kBoxes < kMost) boxes_free();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) stage16(buf + b * 4096, lane, i, w[j][4 * i], w[j][4 * i + 1], w[j][4 * i + 2], w[j][4 * i + 3]);
+          for (int i = 0; i < 8; ++i)
+            stage16(buf + b * 4096, lane, i, w[j][4 * i], w[j][4 * i + 1], w[j][4 * i + 2], w[j][4 * i + 3]);
           boxes_written();
           send(0, b, box);
           if (elected) ptx::bulk_commit_group();
@@ -662,7 +668,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm(const __grid_consta
             float y[4];
             gate(as_f2(g[j][4 * i], g[j][4 * i + 1]), as_f2(u[j][4 * i], u[j][4 * i + 1])).get(y[0], y[1]);
             gate(as_f2(g[j][4 * i + 2], g[j][4 * i + 3]), as_f2(u[j][4 * i + 2], u[j][4 * i + 3])).get(y[2], y[3]);
-            stage16(buf, lane, i, __float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+            stage16(buf, lane, i, __float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]),
+                    __float_as_uint(y[3]));
           }
           boxes_written();
           send(0, 0, box);
@@ -786,7 +793,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
   constexpr bool kGated = EPI == FDMOE_EPI_GATED || EPI == FDMOE_EPI_GATED_F32;
   constexpr int kParts = kGated ? 2 : 1;
   constexpr int kScales = MX4 ? (kParts + 1) * 2 * kScaleBlock : 0;
-  static_assert(!MX4 || FDMOE_STREAM_TOKENS_MX4 == 128, "where there are several tiles of tokens, each is a block of scales");
+  static_assert(!MX4 || FDMOE_STREAM_TOKENS_MX4 == 128, "each of several tiles of tokens is a block of scales");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
   const int nt = p.tile_tokens;
@@ -954,7 +961,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
       } else {
         uint16_t* out = static_cast<uint16_t*>(p.out);
         const bool odd = lane & 1;
-        const float a = __shfl_xor_sync(0xffffffffu, odd ? y[0] : y[2], 1), b = __shfl_xor_sync(0xffffffffu, odd ? y[1] : y[3], 1);
+        const float a = __shfl_xor_sync(0xffffffffu, odd ? y[0] : y[2], 1);
+        const float b = __shfl_xor_sync(0xffffffffu, odd ? y[1] : y[3], 1);
         const uint32_t w0 = odd ? pack2(a, y[2], p.bf16) : pack2(y[0], a, p.bf16);
         const uint32_t w1 = odd ? pack2(b, y[3], p.bf16) : pack2(y[1], b, p.bf16);
         const int r = row & ~1, i0 = odd ? 2 : 0;
@@ -1018,7 +1026,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_gemm(const __grid_const
 #pragma unroll
               for (int q = 0; q < kParts; ++q)
                 if (owner == rank)
-                  *reinterpret_cast<uint4*>(own + at + q * 2048) = make_uint4(v[q][i], v[q][i + 1], v[q][i + 2], v[q][i + 3]);
+                  *reinterpret_cast<uint4*>(own + at + q * 2048) =
+                      make_uint4(v[q][i], v[q][i + 1], v[q][i + 2], v[q][i + 3]);
                 else
                   ptx::st_async_u32x4(to + q * 2048, v[q][i], v[q][i + 1], v[q][i + 2], v[q][i + 3], bar);
             }

@@ -22,7 +22,10 @@ extern "C" int fdmoe_pair_launch(const FdmoePairParams* p, int epi, int mx4, int
 // of TMEM the occupancy calculator takes for all of an SM's.
 namespace {
 __global__ void __launch_bounds__(kPairThreads) pair_shape() {}
-__global__ void __launch_bounds__(kStreamThreads) stream_shape() { __shared__ volatile uint8_t barriers[256]; barriers[0] = 0; }
+__global__ void __launch_bounds__(kStreamThreads) stream_shape() {
+  __shared__ volatile uint8_t barriers[256];
+  barriers[0] = 0;
+}
 
 template <typename F>
 int count_clusters(F kernel, int threads, int smem, int size, int* out) {

@@ -51,7 +51,8 @@ cudaError_t launch_pair_of(const FdmoePairParams& p, int clusters, cudaStream_t 
 }
 template <bool MX4, int EPI>
 cudaError_t launch_pair(const FdmoePairParams& p, int clusters, cudaStream_t stream) {
-  if constexpr (EPI == FDMOE_EPI_F32 || EPI == FDMOE_EPI_GATED_F32) return launch_pair_of<MX4, EPI, true>(p, clusters, stream);
+  if constexpr (EPI == FDMOE_EPI_F32 || EPI == FDMOE_EPI_GATED_F32)
+    return launch_pair_of<MX4, EPI, true>(p, clusters, stream);
   return p.bf16 ? launch_pair_of<MX4, EPI, true>(p, clusters, stream) : launch_pair_of<MX4, EPI, false>(p, clusters, stream);
 }
 

@@ -304,7 +304,9 @@ int StreamProduct(const Call& c, const void* x, const void* w, void* out, int64_
 // [T, I], and h [T, I], 16 bits each.
 struct Saved {
   uint8_t *gu = nullptr, *lower = nullptr, *h = nullptr;
-  static size_t Bytes(int64_t T, int64_t I) { return fdmoe::AlignBytes((size_t)T * I * 4) + 2 * fdmoe::AlignBytes((size_t)T * I * 2); }
+  static size_t Bytes(int64_t T, int64_t I) {
+    return fdmoe::AlignBytes((size_t)T * I * 4) + 2 * fdmoe::AlignBytes((size_t)T * I * 2);
+  }
   Saved() = default;
   Saved(const void* base, int64_t T, int64_t I) {
     gu = static_cast<uint8_t*>(const_cast<void*>(base));
@@ -545,7 +547,8 @@ extern "C" int FlashMoeFfnBackward(const FlashMoeFfnConfig* cfg, const void* dy,
       !Aligned(savedBy) || !Aligned(workspace) || workspaceBytes < FlashMoeFfnWorkspaceBytes(cfg, T, 1))
     return (int)cudaErrorInvalidValue;
   if (!dx && !dw13 && !dw2) return 0;
-  DENSE_TRY(CheckApart({{dx, Bytes(T, H, 2)}, {dw13, Bytes(2 * I, H, 2)}, {dw2, Bytes(H, I, 2)}, {workspace, Bytes(T, I, 4)}},
+  DENSE_TRY(CheckApart({{dx, Bytes(T, H, 2)}, {dw13, Bytes(2 * I, H, 2)}, {dw2, Bytes(H, I, 2)},
+                        {workspace, Bytes(T, I, 4)}},
                        {{dy, Bytes(T, H, 2)}, {x, Bytes(T, H, 2)}, {w13, Bytes(2 * I, H, 2)}, {w2, Bytes(H, I, 2)},
                         {savedBy, Saved::Bytes(T, I)}}));
   Call c;

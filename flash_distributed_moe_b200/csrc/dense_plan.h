@@ -9,7 +9,8 @@
 
 namespace fdmoe {
 
-constexpr int kStreamSmemTwo = 112 * 1024;    // dynamic shared memory of a CTA when two share an SM (228 KB, 1 KB each reserved)
+// Dynamic shared memory of a CTA when two share an SM (228 KB, 1 KB each reserved), and of one alone.
+constexpr int kStreamSmemTwo = 112 * 1024;
 constexpr int kStreamSmemOne = 226 * 1024;
 constexpr int kStreamSlack = 1024;            // for the alignment of the stages
 
@@ -91,10 +92,11 @@ struct PairPlan {
 
 inline double BlockCycles(int tile_n) { return tile_n == 256 ? 520 : tile_n == 192 ? 455 : 365; }
 
-// `cols`: of the result; `kblocks` stages of k.  Time in cycles: the waves of tiles, each its k blocks (about 520,
-// 455 and 365 cycles at widths of 256, 192 and 128: what a stage's operands take to be written to and read from shared
-// memory, 128 bytes a cycle, is 512, 448 and 384, and its MMAs 512, 384 and 256) and once per launch, or per cluster where pairs share a tile, its
-// beginning and end; sharing also takes the partial sums' way through the cluster's shared memory, at 14 bytes a cycle.
+// `cols`: of the result; `kblocks` stages of k.  Time in cycles: the waves of tiles, each its k blocks, and once per
+// launch, or per cluster where pairs share a tile, its beginning and end; sharing also takes the partial sums' way
+// through the cluster's shared memory, at 14 bytes a cycle.  A k block is planned with 520, 455 and 365 cycles at widths
+// of 256, 192 and 128.  Its MMAs are 512, 384 and 256; at about 128 bytes a cycle its operands take 512, 448 and 384 to
+// be written to and read from shared memory, a rough figure: 365 to 400 were measured at a width of 128.
 // In us, for width / pairs per tile: 4096 x 2048 x 6144 (rows, columns, k) 69 with 256/1, 80 with 192/1, 95 with
 // 128/1, 90 with 256/2; 777 x 1000 x 5488 36, 32, 28 and 24, 19 with 128/2, 36 with 128/4.
 inline PairPlan MakePairPlan(int64_t rows, int64_t cols, int kblocks, bool gated, bool mx4, const DeviceSlots& dev) {

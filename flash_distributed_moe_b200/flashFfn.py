@@ -99,10 +99,20 @@ class _GatedFfn(torch.autograd.Function):
 
 
 def gated_ffn(x: torch.Tensor, w13: Weight, w2: Weight) -> torch.Tensor:
-    """x [..., H] -> [..., H].  Asynchronous on the current torch stream of x's device.  Differentiable in x, w13 and w2:
-    the gate and up projections of the tokens and silu(g) * u are kept for the backward pass, in 24 bits and in the dtype.  With Mx4Tensor
-    weights (w13 [2, I, H], w2 [H, I]) x and the activations are quantised to 4 bits too, and there is no gradient.
-    h = silu(g) * u is rounded to the dtype: in fp16 it is infinite beyond 65504, as in a program of torch operators.
+    """x [..., H] -> [..., H].  Asynchronous on the current torch stream of x's device.  Differentiable in x, w13 and w2
+    by torch's reverse mode, once: the gate and up projections of the tokens and silu(g) * u are kept for the backward
+    pass, in 24 bits and in the dtype.  With Mx4Tensor weights (w13 [2, I, H], w2 [H, I]) x and the activations are
+    quantised to 4 bits too, and there is no gradient.
+
+    Operands of a product are rounded to the dtype: h = silu(g) * u, and in the backward pass the gradients of g and u.
+    In fp16 all three are infinite beyond 65504 and vanish below 3e-8, as in a program of torch operators.
+
+    The same call gives the same bits.  A call that keeps nothing for a backward pass may use another kernel than one
+    that does, and another number of tokens another one again, whose sums have another order: results then differ by
+    the rounding of the sums, e.g. those of a checkpointed block from its recomputation.
+
+    Forward-mode derivatives and recorders of torch operators (torch.jit.trace, make_fx) are refused; torch.compile runs
+    the call between its graphs.
 
     A training step may be captured into a CUDA graph while no eager graph of the same leaves is alive: torch keeps the
     gradient accumulators of such a graph on its stream, which a captured backward pass of any operator, this one

@@ -6,7 +6,8 @@
 
 The values are E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), the scales E8M0; a block's scale is
 2^(floor(log2(largest magnitude)) - 2), elements are rounded to nearest even and saturate at 6, and a block that
-holds a NaN or an infinity stands for NaN.  Products are exact in their operands and accumulated in fp32.
+holds a NaN or an infinity stands for NaN.  Products are exact in their operands and accumulated in fp32; the sigmoid of
+a gate value g is off by at most 2^-21 + |g| 2^-23 of itself, which an fp32 result shows.
 None of these functions has a gradient: 4-bit weights are constants, and a product refuses activations whose origin needs
 one, where gradients are on.
 """
@@ -102,7 +103,7 @@ class Mx4Tensor:
         return self._split()[1]
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """The values that the matrix stands for.  Exact in fp32; in bf16 and fp16 unless they leave the type's range."""
+        """The values that the matrix stands for, exact unless they leave the type's range."""
         check_not_traced()
         code, shape, device = _check_dtype(dtype), self.shape, self.device
         if device.type != "cuda":

@@ -117,7 +117,9 @@ int FlashMoeLaunchNoAlloc(const void* gateWeights, const void* ffn1ExpertWeights
  * may overlap.  Matrices are contiguous, row-major, on the current device, and start on 16 bytes.  Results,
  * scratch and what is kept lie on no other memory of the call (cudaErrorInvalidValue), but for `y`, which may be
  * `x`, in the two forward calls.
- * Results are deterministic: the same call gives the same bits. */
+ * Results are deterministic: the same call gives the same bits.  Another number of tokens, or a forward
+ * call that keeps what the backward pass needs instead of one that does not, may use another kernel, whose
+ * sums have another order. */
 typedef struct {
   int32_t hiddenSize;       /* H, a multiple of 8 (4-bit weights: 32) */
   int32_t intermediateSize; /* I, a multiple of 8 (4-bit weights: 32) */
@@ -139,7 +141,8 @@ int FlashMoeFfnForward(const FlashMoeFfnConfig* config, const void* x, const voi
                        void* stream);
 
 /* Gradients of x [T,H], w13 [2I,H] and w2 [H,I] from that of y; each of the three may be NULL.  With no
- * tokens the gradients of the weights are zero. */
+ * tokens the gradients of the weights are zero.  The gradients of the projections are rounded to the dtype
+ * (fp16: infinite beyond 65504, zero below 3e-8) before the last products. */
 int FlashMoeFfnBackward(const FlashMoeFfnConfig* config, const void* dy, const void* x, const void* w13,
                         const void* w2, const void* saved, void* dx, void* dw13, void* dw2,
                         void* workspace, size_t workspaceBytes, int64_t tokensNum, void* stream);
